@@ -18,6 +18,7 @@ class CacheCell:
     kv_heads, head_dim / w, page_size, w] with w = `key_piece_width(head_dim)`, `values` is stored
     transposed in pieces of v = `value_piece_width(page_size)` keys, [pages, kv_heads, page_size / v, head_dim,
     v]; both are also attributes of the cell, and `key_rows` / `value_rows` give whole rows back.
+    For keys and values in 4 bits (`PackedKeyValue`): `packed`, uint8 [pages, kv_heads, bytes], which the kernel library packs and reads.
     For a per-request need: `state` is [slots, *shape] float32, indexed by `StepBatch.state_slots`.
     `writable` is False when the run reads a cell that another run owns.
     """
@@ -57,6 +58,11 @@ class CacheCell:
     @values.setter
     def values(self, tensor: torch.Tensor) -> None:
         self.fields["values"] = tensor
+
+    @property
+    def packed(self) -> torch.Tensor | None:
+        """The pages of keys and values in 4 bits (`PackedKeyValue`), uint8 [pages, kv_heads, bytes]."""
+        return self.fields.get("packed")
 
     def key_rows(self, pages: torch.Tensor, offsets: torch.Tensor) -> torch.Tensor:
         """The keys at (pages[i], offsets[i]) as whole rows, [n, kv_heads, head_dim]."""

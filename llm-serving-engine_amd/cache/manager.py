@@ -26,7 +26,7 @@ import torch
 
 from ..config.serving import CacheConfig
 from .cell import CacheCell
-from ..parts.base import PagedNeed, SlotNeed, needs_by_name
+from ..parts.base import PackedKeyValue, PagedNeed, SlotNeed, needs_by_name
 from ..parts.model import ModelSpec
 from .pool import CacheFullError, PagePool
 
@@ -103,6 +103,8 @@ class CacheManager:
                 if run.takes(name):
                     entries[name] = self._cell_of_run[run.reads][name]
                 elif isinstance(need, PagedNeed):
+                    if config.packed:
+                        need = need.packed(self.page_size)
                     if need not in by_need:
                         by_need[need] = len(self.groups)
                         tables = np.full((config.max_sequences, self.max_blocks_per_sequence), -1, np.int32)
@@ -123,7 +125,7 @@ class CacheManager:
         for group in self.groups:
             for field_name, shape in group.need.page_fields(self.page_size).items():
                 group.storage[field_name] = torch.zeros(
-                    (len(group.cells), config.num_blocks, *shape), dtype=dtype, device=self.device
+                    (len(group.cells), config.num_blocks, *shape), dtype=group.need.field_dtype(dtype), device=self.device
                 )
 
     # ------------------------------------------------------------------ views
@@ -326,7 +328,8 @@ class CacheManager:
         first, fields = self.gather_fields(request_id, run, name)
         if not fields:
             need = self._paged_cell(run, name)[0].need
-            empty = torch.empty((0, need.num_kv_heads, need.head_dim), dtype=self.dtype, device=self.device)
+            dtype = torch.float32 if isinstance(need, PackedKeyValue) else self.dtype
+            empty = torch.empty((0, need.num_kv_heads, need.head_dim), dtype=dtype, device=self.device)
             return first, empty, empty.clone()
         return first, fields["keys"], fields["values"]
 

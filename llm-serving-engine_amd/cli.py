@@ -63,7 +63,7 @@ def _engine(args, loaded, tokenizer, *, batch_size: int, mode: str):
     return LLMEngine(
         loaded,
         tokenizer,
-        cache_config=CacheConfig(args.block_size, args.num_blocks, max(batch_size, 1)),
+        cache_config=CacheConfig(args.block_size, args.num_blocks, max(batch_size, 1), args.packed_cache),
         scheduler_config=SchedulerConfig(batch_size, max(args.max_tokens_per_step, batch_size), args.policy),
         scheduler_mode=mode,
         prefill_chunk_size=args.prefill_chunk_size,
@@ -177,6 +177,7 @@ def _engine_options(parser: argparse.ArgumentParser) -> None:
     parser.add_argument("--device", default="auto")
     parser.add_argument("--dtype", choices=("bfloat16", "float32"), default="bfloat16")
     parser.add_argument("--block-size", type=int, default=16)
+    parser.add_argument("--packed-cache", action="store_true", help="keep keys and values in 4 bits (Qwen2; head sizes in steps of 32)")
     parser.add_argument("--num-blocks", type=int, default=1024)
     parser.add_argument("--prefill-chunk-size", type=int, default=16)
     parser.add_argument("--max-tokens-per-step", type=int, default=2048)

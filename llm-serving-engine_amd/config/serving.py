@@ -11,6 +11,7 @@ class CacheConfig:
     block_size: int = 16  # tokens per page
     num_blocks: int = 1_024  # pages in each group's pool
     max_sequences: int = 256  # live requests (block-table rows and state slots)
+    packed: bool = False  # keys and values in 4 bits instead of the run dtype (layers of plain attention, as Qwen2's)
 
     def __post_init__(self) -> None:
         if self.block_size <= 0 or self.num_blocks <= 0 or self.max_sequences <= 0:

@@ -47,6 +47,16 @@ def _pointer(tensor: torch.Tensor | None) -> int | None:
     return tensor.data_ptr()
 
 
+def _packed_pages(cell) -> torch.Tensor | None:
+    """The cell's pages of keys and values in 4 bits, if it keeps those."""
+    return getattr(cell, "packed", None)
+
+
+def _no_packed(cell, what: str) -> None:
+    if cell is not None and _packed_pages(cell) is not None:
+        raise KernelError(f"{what}: not over keys and values in 4 bits")
+
+
 def _in_pieces(*tensors: torch.Tensor) -> bool:
     """Whether rows can be read in 16-byte pieces: contiguous tensors that begin at one (rows of a whole number of pieces)."""
     for tensor in tensors:  # (a loop: a generator costs the host as much again, twice a layer of a step that is launched kernel by kernel)
@@ -138,6 +148,10 @@ _SIGNATURES = {
     "llmserve_convolved_heads": "piiiiiiiiiiiiifppipiippppipfipipppip",
     "llmserve_difference_heads": "pipiiiifffp",
     "llmserve_gate_columns": "piipiiiiipiip",
+    "llmserve_packed_store": "piiiiiipiipp",
+    "llmserve_packed_rows": "piiiipippip",
+    "llmserve_packed_attention": "piipippipippiiiiifiip",
+    "llmserve_place_tokens": "piiipppiiiipppppipip",
 }
 _TYPES = {"p": ctypes.c_void_p, "i": ctypes.c_int, "f": ctypes.c_float}
 
@@ -449,6 +463,12 @@ class HipKernels:
         tokens = qkv.shape[0]
         if qkv.shape[1] != layout.stride:
             raise KernelError("rotate_and_store: qkv does not have the layout's width")
+        if cell is not None and _packed_pages(cell) is not None:
+            if pairing != "none":
+                self.rotate_and_store(qkv, layout, batch, None, inverse_frequencies, pairing)
+            if cell.writable:
+                self.store_packed(qkv, layout, batch, cell)
+            return
         store = cell is not None and cell.writable
         group = batch.groups[cell.group] if store else None
         if store and (cell.keys.dtype != qkv.dtype or cell.values.shape[1:] != cell.need.page_fields(group.page_size)["values"]):
@@ -466,7 +486,7 @@ class HipKernels:
         """`linear(x, weights)` and `rotate_and_store` of its rows in one kernel, where it takes them and is ahead; else None, and nothing done.
         Neighbouring pairs alone: of half pairs a column's partner is dim / 2 away, in another tile."""
         rows, inner = x.shape
-        dim, store = layout.head_dim, cell is not None and cell.writable
+        dim, store = layout.head_dim, cell is not None and cell.writable and _packed_pages(cell) is None
         if (
             pairing != "adjacent" or not store or batch.max_query_length == 1 or rows <= 64 or dim % 16 or weights.out_features != layout.width
             or layout.stride != layout.width or inner != weights.in_features or inverse_frequencies.shape != (dim // 2,)
@@ -1198,11 +1218,16 @@ class HipKernels:
         cap), then minus slope * distance; `sinks` (float32 [heads]) add exp(sink) to a head's denominator; with
         `keep_first` a sequence's first so many keys stay visible behind the window, at their own positions.  The
         matrix-core kernels of both precisions take them (in bfloat16 not the forms that fuse the rotation or share
-        keys through LDS).  `chunk` is a mask instead of a window: a query sees the keys of its own chunk of so many positions.
+        keys through LDS).  Over a cell of keys and values in 4 bits (`PackedKeyValue`) none of these changes is taken, a window is.
+        `chunk` is a mask instead of a window: a query sees the keys of its own chunk of so many positions.
         With `out` (rows of the run dtype, as wide as the heads or wider) the result is its first columns.  With `vdim`, `distance_bias`
         or `gates` the results are heads of `vdim` side by side: in bfloat16 the matrix-core kernel adds the bias and writes them
         gated; elsewhere a kernel of its own brings them together behind the attention.  `maps` (of the kernels that are
         not for bfloat16 on the matrix cores): a query row holds so many maps side by side, and the result is one head a map."""
+        if _packed_pages(cell) is not None:
+            if any(given is not None for given in (score_slopes, soft_cap, sinks, vdim, distance_bias, gates)) or keep_first or chunk or maps != 1:
+                raise KernelError("paged_attention: over keys and values in 4 bits the scores and results are not changed")
+            return self._packed_attention(qkv, layout, batch, cell, scale, window, out)
         if vdim is not None or distance_bias is not None or gates is not None:
             if score_slopes is not None or soft_cap is not None or sinks is not None or keep_first or chunk or maps != 1:
                 raise KernelError("paged_attention: finished results go with no other change of the scores")
@@ -1257,6 +1282,7 @@ class HipKernels:
         """In bfloat16 one kernel (and one that merges key splits): both maps of a head walk the keys together, and their
         normed difference is what is written.  Elsewhere the maps are heads of the plain attention, put together behind it."""
         tokens, heads, dim = rows.shape[0], layout.num_heads, layout.head_dim
+        _no_packed(cell, "difference_attention")
         group = batch.groups[cell.group]
         if dim % 2 or not 0 < vdim <= dim:
             raise KernelError("difference_attention: two maps of one width, and values as wide as both or narrower")
@@ -1295,6 +1321,7 @@ class HipKernels:
         if temperature is not None and not every >= 1:
             raise KernelError("convolved_heads: a temperature grows every so many positions")
         out = self._empty((tokens, (heads + 2 * kv_heads) * width), x.dtype)
+        _no_packed(cell, "convolved_heads")
         store = cell is not None and cell.writable
         group = batch.groups[cell.group] if store else None
         if store and (cell.keys.dtype != x.dtype or cell.values.shape[1:] != cell.need.page_fields(group.page_size)["values"]
@@ -1632,6 +1659,7 @@ class HipKernels:
         if (
             batch.max_query_length == 1
             and cell.writable
+            and _packed_pages(cell) is None
             and qkv.dtype == torch.bfloat16
             and cell.keys.dtype == torch.bfloat16
             and group.page_size % 8 == 0
@@ -1688,6 +1716,109 @@ class HipKernels:
             return result, True
         self.rotate_and_store(qkv, layout, batch, cell, inverse_frequencies, pairing)
         return self.paged_attention(qkv, layout, batch, cell, scale, window, sinks=sinks, chunk=chunk, out=out), False
+
+    # ------------------------------------------------------------------ keys and values in 4 bits, index arrays on the device
+
+    def _packed_cell(self, cell, kv_heads: int, dim: int, page_size: int, what: str) -> torch.Tensor:
+        """The cell's pages, which the kernels read and write by address, after a look at their shape."""
+        pages = _packed_pages(cell)
+        if pages is None or pages.dtype != torch.uint8 or pages.ndim != 3 or (cell.need.num_kv_heads, cell.need.head_dim) != (kv_heads, dim):
+            raise KernelError(f"{what}: the cell keeps no keys and values in 4 bits for {kv_heads} heads of {dim}")
+        if page_size % 8 or pages.shape[1] != kv_heads or pages.shape[2] != page_size * (dim + dim // 16) or not self._here(pages):
+            raise KernelError(f"{what}: the cell's pages do not hold {page_size} tokens of {kv_heads} heads of {dim} in 4 bits on {self.device}")
+        return pages
+
+    def _indices(self, tensor: torch.Tensor, shape: tuple, what: str) -> None:
+        if tensor.dtype != torch.int32 or tuple(tensor.shape) != shape or not self._here(tensor):
+            raise KernelError(f"{what}: int32 {list(shape)} on {self.device}")
+
+    def store_packed(self, qkv, layout, batch, cell) -> None:
+        """The keys and values of `qkv`'s rows (as `rotate_and_store` leaves them), rounded to 4 bits, into the cell's pages at the step's
+        slots (a negative slot, or one beyond the pages: nowhere; every other slot once)."""
+        tokens, kv_heads, dim = qkv.shape[0], layout.num_kv_heads, layout.head_dim
+        group = batch.groups[cell.group]
+        pages = self._packed_cell(cell, kv_heads, dim, group.page_size, "store_packed")
+        if qkv.ndim != 2 or qkv.shape[1] != layout.stride or not self._here(qkv):
+            raise KernelError("store_packed: rows of the layout's width on the library's device")
+        self._indices(group.slot_mapping, (tokens,), "store_packed: the step's slots")
+        status = self._library_of("packed").llmserve_packed_store(
+            _pointer(qkv), _is_float(qkv), layout.stride, layout.num_heads * dim, tokens, kv_heads, dim, _pointer(pages), pages.shape[0], group.page_size,
+            _pointer(group.slot_mapping), self._stream,
+        )
+        _check(status, "store_packed")
+
+    def packed_rows(self, cell, slots: torch.Tensor, page_size: int) -> tuple[torch.Tensor, torch.Tensor]:
+        """(keys, values) [n, kv_heads, dim] in the run dtype of what the cell's pages hold at `slots` int32 [n], exactly; zeros for a
+        negative slot or one beyond the pages."""
+        need = cell.need
+        pages = self._packed_cell(cell, need.num_kv_heads, need.head_dim, page_size, "packed_rows")
+        self._indices(slots, (slots.numel(),), "packed_rows: slots")
+        both = self._empty((2, slots.shape[0], need.num_kv_heads, need.head_dim), self.dtype)
+        keys, values = both[0], both[1]
+        status = self._library_of("packed").llmserve_packed_rows(
+            _pointer(pages), pages.shape[0], need.num_kv_heads, need.head_dim, page_size, _pointer(slots), slots.shape[0], _pointer(keys), _pointer(values),
+            _is_float(both), self._stream,
+        )
+        _check(status, "packed_rows")
+        return keys, values
+
+    def _packed_library(self, head_dim: int):
+        key = f"packed_attention {head_dim}"
+        if key not in self._lazy:
+            self._lazy[key] = _declared(load_module("packed_attention", {"HEAD_DIM": head_dim}))
+        return self._lazy[key]
+
+    def _packed_attention(self, qkv, layout, batch, cell, scale: float, window: int | None, out):
+        tokens, heads, kv_heads, dim = qkv.shape[0], layout.num_heads, layout.num_kv_heads, layout.head_dim
+        group = batch.groups[cell.group]
+        pages = self._packed_cell(cell, kv_heads, dim, group.page_size, "paged_attention")
+        requests = batch.context_lengths.shape[0]
+        if qkv.ndim != 2 or qkv.shape[1] != layout.stride or not self._here(qkv):
+            raise KernelError("paged_attention: rows of the layout's width on the library's device")
+        self._indices(group.block_tables, (requests, group.width), "paged_attention: block tables")
+        self._indices(batch.query_start, (requests + 1,), "paged_attention: query starts")
+        self._indices(batch.context_lengths, (requests,), "paged_attention: context lengths")
+        out = self._attention_out(qkv, layout, out)
+        status = self._packed_library(dim).llmserve_packed_attention(
+            _pointer(qkv), _is_float(qkv), layout.stride, _pointer(out), out.shape[1], None, _pointer(pages), pages.shape[0], _pointer(group.block_tables), group.width,
+            _pointer(batch.query_start), _pointer(batch.context_lengths), requests, tokens, heads, kv_heads, group.page_size, scale, int(window or 0), 1, self._stream,
+        )
+        _check(status, "paged_attention over 4 bits")
+        return out
+
+    def place_tokens(self, tables, slots, starts, counts, page_size: int, tokens: int, width: int, out: tuple | None = None) -> tuple[torch.Tensor, ...]:
+        """A step's index arrays from its requests' lengths, made on the device: `tables` int32 [groups, rows, blocks] are the cache's block
+        tables (-1: no page), and request b has row slots[b], starts[b] tokens cached and counts[b] in this step (int32 [B]).  -> (positions
+        [tokens], request of every token [tokens], query starts [B + 1], context lengths [B], slot mapping [groups, tokens], block tables [groups, B,
+        width]), int32, or `out`, six such tensors, filled.  A token without a page is mapped to -1; a table row is -1 behind the request's last page.  A
+        request whose slot is not a row of the tables pads the step: its tokens are at position 0 and stored nowhere, its context is one token, its table
+        row 0.  Where the counts add up to less than `tokens`, the rows behind the last are such tokens of the last request; to more: what is too many is left out."""
+        requests = slots.shape[0]
+        if tables.ndim != 3 or tables.dtype != torch.int32 or not self._here(tables):
+            raise KernelError(f"place_tokens: tables are int32 [groups, rows, blocks] on {self.device}")
+        groups, rows, blocks = tables.shape
+        for name, tensor in (("slots", slots), ("starts", starts), ("counts", counts)):
+            self._indices(tensor, (requests,), f"place_tokens: {name}")
+        if out is None:
+            both = self._empty((2 * tokens + 2 * requests + 1 + groups * (tokens + requests * width),), torch.int32)
+            positions, sequence, query_start, contexts, mapping, compact = both.split(
+                (tokens, tokens, requests + 1, requests, groups * tokens, groups * requests * width))
+            out = positions, sequence, query_start, contexts, mapping.view(groups, tokens), compact.view(groups, requests, width)
+        else:
+            shapes = ((tokens,), (tokens,), (requests + 1,), (requests,), (groups, tokens), (groups, requests, width))
+            if len(out) != 6:
+                raise KernelError("place_tokens: six tensors to fill")
+            for tensor, shape in zip(out, shapes):
+                self._indices(tensor, shape, "place_tokens: a tensor to fill")
+            if not all(tensor[0].is_contiguous() for tensor in out[4:]) or not all(tensor.is_contiguous() for tensor in out[:4]):
+                raise KernelError("place_tokens: the tensors to fill are contiguous, a group's where there are several")
+        positions, sequence, query_start, contexts, mapping, compact = out
+        status = self._library_of("placing").llmserve_place_tokens(
+            _pointer(tables), groups, rows, blocks, _pointer(slots), _pointer(starts), _pointer(counts), requests, page_size, tokens, width, _pointer(positions),
+            _pointer(sequence), _pointer(query_start), _pointer(contexts), mapping.data_ptr(), mapping.stride(0), compact.data_ptr(), compact.stride(0), self._stream,
+        )
+        _check(status, "place_tokens")
+        return out
 
     # ------------------------------------------------------------------ layer norm, runs of columns
 
@@ -2126,6 +2257,7 @@ class HipKernels:
         if other is not None and (other.dtype != x.dtype or other.shape[0] != tokens):
             raise KernelError("assemble_heads: the other values are rows of the same type, one a token")
         out = self._empty((tokens, (heads + 2 * kv_heads) * width), x.dtype)
+        _no_packed(cell, "assemble_heads")
         store = cell is not None and cell.writable
         group = batch.groups[cell.group] if store else None
         if store and (cell.keys.dtype != x.dtype or cell.values.shape[1:] != cell.need.page_fields(group.page_size)["values"]

@@ -19,6 +19,10 @@ DEFAULT_VARIANTS: dict[str, list[dict[str, object]]] = {
     "streams": [{}],
     "recurrence": [{}],
     "convolved_heads": [{}],
+    "packed": [{}],
+    "placing": [{}],
+    # every head size that pages in 4 bits have
+    "packed_attention": [{"HEAD_DIM": d} for d in (32, 64, 96, 128, 160, 192, 224, 256)],
     # query/key sizes of the tests' and the benchmark's models with decaying linear attention
     "decay_attention": [{"HEAD_DIM": d} for d in (8, 16, 24, 32, 48, 64, 128)],
     # head sizes of the tests' models and kernel tests, and of the benchmark

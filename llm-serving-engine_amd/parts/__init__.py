@@ -8,6 +8,7 @@ from .base import (
     POSITIONS,
     CacheNeed,
     FixedState,
+    PackedKeyValue,
     PagedKeyValue,
     PagedNeed,
     SlotNeed,

@@ -88,7 +88,7 @@ class Attention(Mixer):
 
     @classmethod
     def cache_need(cls, spec: AttentionSpec) -> PagedKeyValue:
-        return PagedKeyValue(spec.num_kv_heads, spec.head_dim, spec.window)
+        return PagedKeyValue(spec.num_kv_heads, spec.head_dim, spec.window, packable=True)
 
     def __init__(self, spec: AttentionSpec, tensors, kernels) -> None:
         super().__init__(spec, tensors, kernels)

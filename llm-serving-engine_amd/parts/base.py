@@ -11,7 +11,7 @@ by registering a class: nothing else changes.
 from __future__ import annotations
 
 import math
-from dataclasses import dataclass
+from dataclasses import dataclass, field
 from typing import Any, ClassVar
 
 import torch
@@ -85,6 +85,14 @@ class PagedNeed(CacheNeed):
         [pages, *shape] in the run dtype, and a `CacheCell` shows them by these names."""
         raise NotImplementedError
 
+    def field_dtype(self, run_dtype: torch.dtype) -> torch.dtype:
+        """What the cache keeps the fields in."""
+        return run_dtype
+
+    def packed(self, page_size: int) -> "PagedNeed":
+        """The need of the same entries in 4 bits (`CacheConfig.packed`)."""
+        raise ValueError(f"this model keeps entries that have no form in 4 bits ({type(self).__name__}): packed caches are for layers of plain attention")
+
     def token_rows(self, page: dict[str, torch.Tensor], page_size: int) -> dict[str, torch.Tensor]:
         """One page's fields rearranged so that the token's offset in the page leads: name ->
         [page_size, ...].  The host-side read path (tests, debugging) walks pages through it; kernels
@@ -125,6 +133,8 @@ class PagedKeyValue(PagedNeed):
     window: int | None = None
     keep_first: int = 0
     chunk: int | None = None
+    # the part asks nothing of its pages that pages in 4 bits do not offer (no difference between two needs otherwise)
+    packable: bool = field(default=False, compare=False, repr=False)
 
     def __post_init__(self) -> None:
         if self.window is not None and self.chunk is not None:
@@ -134,7 +144,7 @@ class PagedKeyValue(PagedNeed):
         if not isinstance(other, PagedKeyValue) or (other.num_kv_heads, other.head_dim) != (self.num_kv_heads, self.head_dim):
             return None
         if other == self:
-            return self
+            return self if self.packable == other.packable else other if self.packable else self
         window = chunk = None
         if self.window is not None and other.window is not None:
             window = max(self.window, other.window)
@@ -144,7 +154,14 @@ class PagedKeyValue(PagedNeed):
             chunk = math.lcm(self.chunk, other.chunk)  # a chunk of either size lies in one of these
         if self.keep_first != other.keep_first:  # (readers say what a cell keeps: those of one cell agree on it)
             return None
-        return PagedKeyValue(self.num_kv_heads, self.head_dim, window, self.keep_first, chunk)
+        return PagedKeyValue(self.num_kv_heads, self.head_dim, window, self.keep_first, chunk, self.packable and other.packable)
+
+    def packed(self, page_size: int) -> "PackedKeyValue":
+        if not self.packable or self.keep_first or self.chunk is not None:
+            return super().packed(page_size)
+        need = PackedKeyValue(self.num_kv_heads, self.head_dim, self.window)
+        need.page_bytes(page_size)  # (refuses page sizes that it has no form for)
+        return need
 
     def page_fields(self, page_size: int) -> dict[str, tuple[int, ...]]:
         width = key_piece_width(self.head_dim)
@@ -157,6 +174,64 @@ class PagedKeyValue(PagedNeed):
         keys = page["keys"].permute(2, 0, 1, 3).reshape(page_size, self.num_kv_heads, self.head_dim)
         values = page["values"].permute(1, 3, 0, 2).reshape(page_size, self.num_kv_heads, self.head_dim)
         return {"keys": keys, "values": values}
+
+
+PACKED_BLOCK = 32  # elements that share a power of two (csrc/packed.h has the same number)
+
+
+@dataclass(frozen=True)
+class PackedKeyValue(PagedNeed):
+    """Keys and values in 4 bits: 32 neighbouring elements of one head of one token share a power of two 2^(b - 127), b one
+    byte, and an element is a sign and one of 0, 0.5, 1, 1.5, 2, 3, 4, 6 (17/32 of a byte an element in all, where bfloat16 takes
+    two).  b + 2 is the exponent of the block's largest magnitude as float32 has it, one more where its significand is 1.75 or
+    larger, kept within 4 .. 254; elements are rounded to the nearest of the sixteen numbers, ties to the even code, and to 6 at most. A
+    block with an infinity or a NaN has b = 255 and reads as NaN.  A page of one kv head is one run of bytes: key codes [page_size, D / 2]
+    (the lower half of a byte first), value codes [page_size / 8, D / 8, 8 keys, 4], key powers [page_size, D / 32], value powers
+    [page_size / 8, D / 32, 8 keys].  Heads of 32 to 256 elements in steps of 32; pages of a multiple of eight tokens."""
+
+    num_kv_heads: int
+    head_dim: int
+    window: int | None = None
+
+    def __post_init__(self) -> None:
+        if self.head_dim % PACKED_BLOCK or not PACKED_BLOCK <= self.head_dim <= 256:
+            raise ValueError(f"keys and values in 4 bits: heads of 32 to 256 elements in steps of 32, not {self.head_dim}")
+
+    def page_bytes(self, page_size: int) -> int:
+        """Bytes of one page of one kv head."""
+        if page_size <= 0 or page_size % VALUE_PIECE:
+            raise ValueError(f"keys and values in 4 bits: pages of a multiple of {VALUE_PIECE} tokens, not {page_size}")
+        return page_size * (self.head_dim + self.head_dim // 16)
+
+    def shared_with(self, other: CacheNeed) -> "PackedKeyValue | None":
+        if not isinstance(other, PackedKeyValue) or (other.num_kv_heads, other.head_dim) != (self.num_kv_heads, self.head_dim):
+            return None
+        window = None if self.window is None or other.window is None else max(self.window, other.window)
+        return PackedKeyValue(self.num_kv_heads, self.head_dim, window)
+
+    def field_dtype(self, run_dtype: torch.dtype) -> torch.dtype:
+        return torch.uint8
+
+    def page_fields(self, page_size: int) -> dict[str, tuple[int, ...]]:
+        return {"packed": (self.num_kv_heads, self.page_bytes(page_size))}
+
+    def token_rows(self, page: dict[str, torch.Tensor], page_size: int) -> dict[str, torch.Tensor]:
+        """(float32 rows: what the pages stand for, exactly.)"""
+        data, dim = page["packed"], self.head_dim
+        codes, powers = page_size * dim // 2, page_size * dim // PACKED_BLOCK
+        keys, values, key_powers, value_powers = torch.split(data, [codes, codes, powers, powers], dim=-1)
+        values = values.unflatten(-1, (page_size // 8, dim // 8, 8, 4)).transpose(-3, -2)  # [kv, pieces, keys, granules, bytes]
+        value_powers = value_powers.unflatten(-1, (page_size // 8, dim // PACKED_BLOCK, 8)).transpose(-2, -1)
+
+        def rows(codes: torch.Tensor, powers: torch.Tensor) -> torch.Tensor:
+            both = torch.stack((codes & 15, codes >> 4), -1).reshape(self.num_kv_heads, page_size, dim // PACKED_BLOCK, PACKED_BLOCK).int()
+            half = (both & 7).float() * 0.5  # codes 0 to 4 count halves; 5, 6, 7 are 3, 4, 6
+            size = torch.where((both & 7) < 5, half, torch.where((both & 7) == 7, 6.0, half + 0.5 + 0.5 * ((both & 7) - 5)))
+            power = powers.reshape(self.num_kv_heads, page_size, dim // PACKED_BLOCK, 1).float()
+            unit = torch.where(power == 255, torch.nan, torch.exp2(power - 127.0))
+            return (torch.where(both >= 8, -size, size) * unit).flatten(-2).transpose(0, 1)
+
+        return {"keys": rows(keys, key_powers), "values": rows(values, value_powers)}
 
 
 @dataclass(frozen=True)
