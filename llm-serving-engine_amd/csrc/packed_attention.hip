@@ -31,8 +31,10 @@ constexpr int SLICES = D / 32;                // MFMA steps over D, and four-byt
 constexpr int TILES = D / 16;                 // tiles of O^T
 constexpr int KEYS = 32;                      // keys a step
 constexpr int WAVES = 4;
-constexpr int SEGMENT = 8192;                 // keys whose pages lie in LDS at a time
-constexpr int ENTRIES = SEGMENT / 8 + 2;
+constexpr int STAGES = 2;                     // steps that a wave has asked for
+constexpr int PIECE = 8 * D + 16;             // bytes in LDS of the codes of eight keys and values (16 spare: the same rows of two pieces lie in other banks)
+constexpr int STAGE = 4 * PIECE + 2 * D;      // of a step: four pieces, and their powers
+constexpr int ASKS = 4 * ((D + 127) / 128 + 1);  // loads of a step
 constexpr float AHEAD = 8.f;                  // log2 units that a score may run ahead of its column's reference before the sums are rescaled
 constexpr float LOG2_E = 1.44269504088896f;
 constexpr int CHUNKS = D / 128 + (D % 128) / 64 + (D % 64) / 32;  // runs of 128, 64 or 32 elements of a value
@@ -51,16 +53,11 @@ struct Step {                                 // what a step takes from memory
   u32x2 value_powers[CHUNKS];
 };
 
-struct Pages {
-  const unsigned char* from;                  // of the kv head
-  size_t stride;                              // bytes from one page to the next
-  int per_page, shift;                        // pieces of eight keys a page; log2 of it, or -1
-  PackedPage page;
-};
-
 struct Walk {
   const int* tables;
   int table_width, num_pages;
+  int page_size, page_shift;                  // log2 of the pieces of eight keys that a page holds, or -1
+  unsigned page_reciprocal;                   // 2^32 over them, rounded up
   const int *query_start, *contexts;
   int requests, heads, kv_heads, window, single;
   int chunk, splits;                          // keys a workgroup walks, and the most workgroups that share a run of columns
@@ -119,33 +116,119 @@ __device__ __forceinline__ bool find_item(const Walk& w, int index, int most, It
   return true;
 }
 
-template <int N> __device__ __forceinline__ void load_dwords(unsigned* to, const unsigned char* from) {  // (aligned to the largest power of two up to 16 bytes that divides 4 N)
-  constexpr int ALIGN = N % 4 == 0 ? 16 : N % 2 == 0 ? 8 : 4;
-  __builtin_memcpy(to, __builtin_assume_aligned(from, ALIGN), N * 4);
+typedef const int __attribute__((address_space(4))) Scalar;  // read by scalar loads: what no kernel writes meanwhile
+
+// Where the four pieces of eight keys of a step lie: their pages and their numbers in them.
+struct Four {
+  unsigned of[4];
+};
+struct Place {
+  Four page, piece;
+};
+
+// (wave-uniform: table entries come through the scalar caches.  Entries beyond the table, and those that are no page, are page 0, whose
+// keys nobody sees then.)
+__device__ __forceinline__ void find_place(Place& to, const Walk& w, Scalar* table, int base) {
+  const unsigned per_page = (unsigned)w.page_size / 8;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const unsigned piece = (unsigned)base / 8 + i, at = w.page_shift >= 0 ? piece >> w.page_shift : __umulhi(piece, w.page_reciprocal);
+    const unsigned entry = at < (unsigned)w.table_width ? (unsigned)table[at] : 0u;
+    to.page.of[i] = entry < (unsigned)w.num_pages ? entry : 0u;
+    to.piece.of[i] = piece - at * per_page;
+  }
 }
 
-__device__ __forceinline__ void load_step(Step& s, const Pages& p, const int* entries, int first_entry, int base) {
-  const int lane = threadIdx.x % WAVE, r = lane & 15, g = lane >> 4;
-  {
-    const int piece = base / 8 + (r >> 2), entry = p.shift >= 0 ? piece >> p.shift : piece / p.per_page;
-    const unsigned char* mine = p.from + (size_t)entries[entry - first_entry] * p.stride;
-    const int offset = (piece - entry * p.per_page) * 8 + (r & 3);
+// Asks for a step: straight into LDS.  A load takes the key codes and the value codes of a piece, 16 bytes a lane (two where heads are wider than
+// 128), and one its powers, 4 bytes a lane; where a piece lies is the same for all lanes, what a lane takes of it the same for all pieces.
+struct LaneParts {
+  unsigned codes[(D + 127) / 128], powers;    // offsets from where the piece's key codes and key powers begin
+};
+__device__ __forceinline__ LaneParts parts_of_lane(int page_size) {
+  LaneParts found;
+  const int lane = threadIdx.x % WAVE;
 #pragma unroll
-    for (int t = 0; t < 2; ++t) {
-      load_dwords<SLICES>(s.keys[t], mine + p.page.key_codes(offset + 4 * t, g * SLICES));
+  for (int i = 0; i < (D + 127) / 128; ++i) {
+    const int unit = i * WAVE + lane;
+    found.codes[i] = unit < D / 4 ? unit * 16 : page_size * (D / 2) + (unit - D / 4) * 16;
+  }
+  found.powers = lane < D / 16 ? lane * 4 : page_size * (D / 32) + (lane - D / 16) * 4;
+  return found;
+}
+
+template <int SIZE> __device__ __forceinline__ void ask(const unsigned char* from, unsigned offset, unsigned char* to) {
+  if constexpr (SIZE == 16) __builtin_amdgcn_global_load_lds((const void __attribute__((address_space(1)))*)(from + offset), (void __attribute__((address_space(3)))*)to, 16, 0, 0);
+  else __builtin_amdgcn_global_load_lds((const void __attribute__((address_space(1)))*)(from + offset), (void __attribute__((address_space(3)))*)to, 4, 0, 0);
+}
+
+__device__ __forceinline__ void ask_step(unsigned char* stage, const unsigned char* from, const Walk& w, const Place& place, const LaneParts& parts) {
+  const int lane = threadIdx.x % WAVE;
+  const unsigned stride = (unsigned)w.kv_heads * (unsigned)(w.page_size * (D + D / 16));
 #pragma unroll
-      for (int i = 0; i < KEY_POWERS; ++i)
-        s.key_powers[t][i] = mine[p.page.key_power(offset + 4 * t, D % 128 == 0 ? g * KEY_POWERS + i : (g * SLICES + i) / 4)];
+  for (int i = 0; i < 4; ++i) {
+    const unsigned char* codes = from + (size_t)place.page.of[i] * stride + place.piece.of[i] * (4 * D);
+#pragma unroll
+    for (int j = 0; j < (D + 127) / 128; ++j)
+      if ((j + 1) * WAVE <= D / 2 || j * WAVE + lane < D / 2) ask<16>(codes, parts.codes[j], stage + i * PIECE + j * WAVE * 16);
+  }
+  if (lane < D / 8) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const unsigned char* powers = from + (size_t)place.page.of[i] * stride + ((unsigned)w.page_size * D + place.piece.of[i] * (D / 4));
+      ask<4>(powers, parts.powers, stage + 4 * PIECE + i * (D / 2));
     }
   }
-  const int piece = base / 8 + g, entry = p.shift >= 0 ? piece >> p.shift : piece / p.per_page;
-  const unsigned char* mine = p.from + (size_t)entries[entry - first_entry] * p.stride;
-  const int offset = (piece - entry * p.per_page) * 8;
+}
+
+template <int N> __device__ __forceinline__ void wait_for_asked() { asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory"); }
+
+// A step's codes and powers out of LDS.  The reads are written out, with the wait behind them: the compiler would have them wait for all that has been asked for.
+__device__ __forceinline__ void read_step(Step& s, const unsigned char* stage) {
+  const unsigned lane = threadIdx.x % WAVE, r = lane & 15, g = lane >> 4;
+  const unsigned at = (unsigned)(size_t)(const unsigned char __attribute__((address_space(3)))*)stage;
+  // key (r >> 2) * 8 + (r & 3) of tile 0, four further of tile 1
+  const unsigned keys = at + (r >> 2) * PIECE + (r & 3) * (D / 2) + g * (D / 8), key_powers = at + 4 * PIECE + (r >> 2) * (D / 2) + (r & 3) * (D / 32);
+  if constexpr (D == 128) {
+    u32x4 k0, k1;
+    asm volatile(
+        "ds_read_b128 %0, %7\n\tds_read_u8 %2, %9\n\tds_read_b128 %1, %7 offset:256\n\tds_read_u8 %3, %9 offset:16\n\tds_read_b128 %4, %8\n\tds_read_b128 %5, %8 offset:16\n\tds_read_b64 %6, %10\n\ts_waitcnt lgkmcnt(0)"
+        : "=&v"(k0), "=&v"(k1), "=&v"(s.key_powers[0][0]), "=&v"(s.key_powers[1][0]), "=&v"(s.values[0][0]), "=&v"(s.values[0][1]), "=&v"(s.value_powers[0])
+        : "v"(keys), "v"(at + g * PIECE + 4 * D + r * 32), "v"(key_powers + g), "v"(at + 4 * PIECE + g * (D / 2) + D / 4 + (r >> 2) * 8)
+        : "memory");
 #pragma unroll
-  for (int c = 0; c < CHUNKS; ++c) {
-    const int granule = chunk_first(c) / 8 + r * chunk_width(c) / 128;
-    load_dwords<8>((unsigned*)s.values[c], mine + p.page.value_codes(offset, granule));
-    load_dwords<2>((unsigned*)&s.value_powers[c], mine + p.page.value_power(offset, granule / 4));
+    for (int i = 0; i < 4; ++i) {
+      s.keys[0][i] = k0[i];
+      s.keys[1][i] = k1[i];
+    }
+  } else {
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+#pragma unroll
+      for (int i = 0; i < SLICES; ++i) asm volatile("ds_read_b32 %0, %1 offset:%2" : "=v"(s.keys[t][i]) : "v"(keys), "n"(t * 2 * D + i * 4) : "memory");
+#pragma unroll
+      for (int i = 0; i < KEY_POWERS; ++i) {
+        const unsigned block = D % 128 == 0 ? g * KEY_POWERS + i : (g * SLICES + i) / 4;
+        asm volatile("ds_read_u8 %0, %1 offset:%2" : "=v"(s.key_powers[t][i]) : "v"(key_powers + block), "n"(t * (D / 8)) : "memory");
+      }
+    }
+#pragma unroll
+    for (int c = 0; c < CHUNKS; ++c) {
+      const unsigned granule = chunk_first(c) / 8 + r * chunk_width(c) / 128, value = at + g * PIECE + 4 * D + granule * 32, power = at + 4 * PIECE + g * (D / 2) + D / 4 + granule / 4 * 8;
+      asm volatile("ds_read_b128 %0, %1" : "=v"(s.values[c][0]) : "v"(value) : "memory");
+      asm volatile("ds_read_b128 %0, %1 offset:16" : "=v"(s.values[c][1]) : "v"(value) : "memory");
+      asm volatile("ds_read_b64 %0, %1" : "=v"(s.value_powers[c]) : "v"(power) : "memory");
+    }
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    // used only after the wait
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+#pragma unroll
+      for (int i = 0; i < SLICES; ++i) asm volatile("" : "+v"(s.keys[t][i]));
+#pragma unroll
+      for (int i = 0; i < KEY_POWERS; ++i) asm volatile("" : "+v"(s.key_powers[t][i]));
+    }
+#pragma unroll
+    for (int c = 0; c < CHUNKS; ++c) asm volatile("" : "+v"(s.values[c][0]), "+v"(s.values[c][1]), "+v"(s.value_powers[c]));
   }
 }
 
@@ -161,35 +244,197 @@ template <typename T, int TERMS> __device__ __forceinline__ void split_eight(con
   }
 }
 
+// What a wave keeps of its columns.
+template <typename T, int CT> struct Columns {
+  static constexpr int TERMS = sizeof(T) == 4 ? 3 : 1;
+  Eight query[CT][TERMS][SLICES];
+  int position[CT];                           // of the lane's column's token
+  float reference[CT];                        // log2 of what weights are divided by
+  f32x4 total[CT];                            // sums of weights, the same number four times
+  f32x4 sum[CT][TILES];
+};
+
+__device__ __forceinline__ f32x4 multiply(const Eight& a, const Eight& b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a.v, b.v, c, 0, 0, 0); }
+
+__device__ __forceinline__ float largest_of(const float* x) { return fmaxf(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])), fmaxf(fmaxf(x[4], x[5]), fmaxf(x[6], x[7]))); }
+
+// One step of 32 keys from `base` on.  EDGE: some column does not see some of them.
+template <typename T, int CT, bool EDGE>
+__device__ __forceinline__ void take_step(Columns<T, CT>& columns, const Step& now, const Walk& w, const Item& item, int base) {
+  constexpr int TERMS = Columns<T, CT>::TERMS;
+  const int lane = threadIdx.x % WAVE, r = lane & 15, g = lane >> 4;
+  // scores: row 4 g + i of tile t is key 8 g + 4 t + i of the step
+  f32x4 score[CT][2];
+#pragma unroll
+  for (int t = 0; t < 2; ++t) {
+#pragma unroll
+    for (int ct = 0; ct < CT; ++ct) score[ct][t] = (f32x4){0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int s = 0; s < SLICES; ++s) {
+      const float power = packed_power(now.key_powers[t][D % 128 == 0 ? s / 4 : D <= 64 ? 0 : s]);
+      Eight key;
+      key.u = (u32x4){unpack_pair<0>(now.keys[t][s], power), unpack_pair<1>(now.keys[t][s], power), unpack_pair<2>(now.keys[t][s], power), unpack_pair<3>(now.keys[t][s], power)};
+#pragma unroll
+      for (int ct = 0; ct < CT; ++ct)
+#pragma unroll
+        for (int k = TERMS - 1; k >= 0; --k) score[ct][t] = multiply(key, columns.query[ct][k][s], score[ct][t]);
+    }
+  }
+  const auto sees = [&](int ct, int i) {
+    const int key = base + 8 * g + i;
+    return key <= columns.position[ct] && (w.window <= 0 || key > columns.position[ct] - w.window);
+  };
+  Eight weight[CT][TERMS];
+#pragma unroll
+  for (int ct = 0; ct < CT; ++ct) {
+    float x[8];  // log2 of the weights
+    const auto relative = [&]() {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const float y = __builtin_fmaf(score[ct][i / 4][i % 4], w.scale, -columns.reference[ct]);
+        x[i] = !EDGE || sees(ct, i) ? y : -INFINITY;
+      }
+    };
+    relative();
+    if (__any(largest_of(x) > AHEAD)) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) x[i] = !EDGE || sees(ct, i) ? score[ct][i / 4][i % 4] * w.scale : -INFINITY;
+      float largest = largest_of(x);
+      largest = fmaxf(largest, __shfl_xor(largest, 16));
+      largest = fmaxf(largest, __shfl_xor(largest, 32));
+      largest = fmaxf(largest, columns.reference[ct]);
+      const float change = columns.reference[ct] == largest ? 1.f : __builtin_amdgcn_exp2f(columns.reference[ct] - largest);
+      columns.reference[ct] = largest;
+      columns.total[ct] *= change;
+#pragma unroll
+      for (int t = 0; t < TILES; ++t) columns.sum[ct][t] *= change;
+      relative();
+    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const float y = __builtin_amdgcn_exp2f(x[i]);
+      x[i] = !EDGE || sees(ct, i) ? y : 0.f;
+    }
+    split_eight<T, TERMS>(x, weight[ct]);
+    // the weights that are multiplied are the weights that are added up: by a product with ones, over all 32 keys at once
+    Eight ones;
+    ones.u = (u32x4){0x3f803f80u, 0x3f803f80u, 0x3f803f80u, 0x3f803f80u};
+#pragma unroll
+    for (int k = TERMS - 1; k >= 0; --k) columns.total[ct] = multiply(ones, weight[ct][k], columns.total[ct]);
+  }
+#pragma unroll
+  for (int c = 0; c < CHUNKS; ++c) {
+    const int width = chunk_width(c), pairs = width / 32;  // pairs of elements that a lane takes of a key
+    u32x2 powers = now.value_powers[c];
+    bool poisoned = false;
+    Eight marks;
+    if (EDGE) {
+      // A value that a column does not see has no part in it, whatever it is: keys that no column sees get the smallest power; of the
+      // others, those that are no number are taken out, and put back where they are seen.
+      marks.u = (u32x4){0u, 0u, 0u, 0u};
+      bool mine = false;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const int key = base + 8 * g + j;
+        const unsigned shift = (j & 3) * 8, byte = (powers[j / 4] >> shift) & 255u;
+        const bool unseen = key > item.last_position || (w.window > 0 && key <= item.first_position - w.window), bad = byte == PACKED_NO_NUMBER;
+        if (unseen || bad) powers[j / 4] &= ~(255u << shift);
+        if (bad && !unseen) {
+          marks.u[j / 2] |= 0x3f80u << (j % 2 * 16);
+          mine = true;
+        }
+      }
+      poisoned = __any(mine);
+    }
+    float power[8];
+    unsigned codes[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      power[j] = __uint_as_float(j % 4 == 3 ? powers[j / 4] >> 1 : powers[j / 4] << (23 - j % 4 * 8));  // (only the exponent of it counts)
+      codes[j] = now.values[c][j / 4][j % 4];
+      if (width == 64) codes[j] >>= (r & 1) * 16;
+      if (width == 32) codes[j] >>= (r & 3) * 8;
+    }
+    const auto pair_of = [&](int j, int e) {
+      return e == 0 ? unpack_pair<0>(codes[j], power[j]) : e == 1 ? unpack_pair<1>(codes[j], power[j]) : e == 2 ? unpack_pair<2>(codes[j], power[j]) : unpack_pair<3>(codes[j], power[j]);
+    };
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      if (e >= pairs) continue;
+      Eight even, odd;                          // elements 2 e and 2 e + 1 of the lane's, of its eight keys
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const unsigned a = pair_of(2 * j, e), b = pair_of(2 * j + 1, e);
+        even.u[j] = __builtin_amdgcn_perm(b, a, 0x05040100u);
+        odd.u[j] = __builtin_amdgcn_perm(b, a, 0x07060302u);
+      }
+      const int t = chunk_first(c) / 16 + 2 * e;
+#pragma unroll
+      for (int ct = 0; ct < CT; ++ct)
+#pragma unroll
+        for (int k = TERMS - 1; k >= 0; --k) {
+          columns.sum[ct][t] = multiply(even, weight[ct][k], columns.sum[ct][t]);
+          columns.sum[ct][t + 1] = multiply(odd, weight[ct][k], columns.sum[ct][t + 1]);
+        }
+    }
+    if (EDGE && poisoned) {
+#pragma unroll
+      for (int ct = 0; ct < CT; ++ct) {
+        Eight seen;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) seen.v[i] = (bf16_t)(sees(ct, i) ? 1.f : 0.f);
+        const f32x4 hit = multiply(marks, seen, (f32x4){0.f, 0.f, 0.f, 0.f});
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          if (e >= 2 * pairs) continue;
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            if (hit[i] > 0.f) columns.sum[ct][chunk_first(c) / 16 + e][i] = __uint_as_float(0x7fc00000u);
+        }
+      }
+    }
+  }
+}
+
 template <typename T, int CT>
-__global__ void __launch_bounds__(WAVES * WAVE) packed_attention_kernel(const T* q, int q_stride, T* out, int out_stride, float* partial, const unsigned char* pages, int page_size, Walk w, int items, int whole) {
+__global__ void __launch_bounds__(WAVES * WAVE, 2) packed_attention_kernel(const T* q, int q_stride, T* out, int out_stride, float* partial, const unsigned char* pages, Walk w, int items, int whole) {
   constexpr int TERMS = sizeof(T) == 4 ? 3 : 1;
-  __shared__ int entries[ENTRIES];
-  __shared__ __attribute__((aligned(16))) float results[WAVES][16][D + 4];
+  constexpr int RING = WAVES * STAGES * STAGE, RESULTS = WAVES * 16 * (D + 4) * 4;
+  __shared__ __attribute__((aligned(16))) unsigned char memory[RING > RESULTS ? RING : RESULTS];  // the steps' codes, and the waves' sums behind them
+  float (*results)[16][D + 4] = (float (*)[16][D + 4])memory;
   __shared__ float sums[WAVES][16][2];
-  const int lane = threadIdx.x % WAVE, wave = threadIdx.x / WAVE, r = lane & 15, g = lane >> 4;
+  const int lane = threadIdx.x % WAVE, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / WAVE), r = lane & 15, g = lane >> 4;
   // the longest walks begin first: a request's last columns walk most keys
   const int all = items * w.kv_heads, at = blockIdx.x % all, split = blockIdx.x / all;
   const int kv_head = at % w.kv_heads;
   Item item;
   if (!find_item(w, items - 1 - at / w.kv_heads, 16 * CT, item)) return;
-  const int begin = item.from + split * w.chunk, end = min(item.to, begin + w.chunk);
-  if (begin >= item.to) return;
+  // as many parts as it takes, all of one length
   const int parts = (item.to - item.from + w.chunk - 1) / w.chunk;
-  Pages p;
-  p.page = {D, page_size};
-  p.per_page = page_size / 8;
-  p.shift = (p.per_page & (p.per_page - 1)) == 0 ? 31 - __clz(p.per_page) : -1;
-  p.from = pages + (size_t)kv_head * p.page.bytes();
-  p.stride = (size_t)w.kv_heads * p.page.bytes();
+  if (split >= parts) return;
+  const int each = ((item.to - item.from + parts - 1) / parts + WAVES * KEYS - 1) / (WAVES * KEYS) * (WAVES * KEYS);
+  const int begin = item.from + split * each, end = min(item.to, begin + each);
+  const unsigned char* from = pages + (size_t)kv_head * (w.page_size * (D + D / 16));
+  Scalar* table = (Scalar*)w.tables + (size_t)item.request * w.table_width;
 
-  // the queries, and where their tokens stand
-  Eight query[CT][TERMS][SLICES];
-  int position[CT];
+  unsigned char* ring = memory + wave * (STAGES * STAGE);
+  const LaneParts lane_parts = parts_of_lane(w.page_size);
+  const int own = __builtin_amdgcn_readfirstlane(begin + wave * KEYS);
+  Place place;
+  int asked = own;
+#pragma unroll
+  for (int s = 0; s < STAGES; ++s)
+    if (asked < end) {
+      find_place(place, w, table, asked);
+      ask_step(ring + s * STAGE, from, w, place, lane_parts);
+      asked += WAVES * KEYS;
+    }
+  if (asked < end) find_place(place, w, table, asked);
+  Columns<T, CT> columns;
 #pragma unroll
   for (int ct = 0; ct < CT; ++ct) {
     const int column = min(ct * 16 + r, item.columns - 1), flat = item.first + column, token = flat / item.group;
-    position[ct] = item.first_position - item.first / item.group + token;
+    columns.position[ct] = item.first_position - item.first / item.group + token;
     const T* row = q + (size_t)(item.first_row + token) * q_stride + (kv_head * item.group + flat - token * item.group) * D + g * (D / 4);
 #pragma unroll
     for (int s = 0; s < SLICES; ++s) {
@@ -207,169 +452,46 @@ __global__ void __launch_bounds__(WAVES * WAVE) packed_attention_kernel(const T*
       Eight terms[TERMS];
       split_eight<T, TERMS>(x, terms);
 #pragma unroll
-      for (int k = 0; k < TERMS; ++k) query[ct][k][s] = terms[k];
+      for (int k = 0; k < TERMS; ++k) columns.query[ct][k][s] = terms[k];
     }
-  }
-  f32x4 sum[CT][TILES];
-  float total[CT], reference[CT];
+    columns.reference[ct] = -INFINITY;
+    columns.total[ct] = (f32x4){0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-  for (int ct = 0; ct < CT; ++ct) {
-    total[ct] = 0.f;
-    reference[ct] = -INFINITY;
-#pragma unroll
-    for (int t = 0; t < TILES; ++t) sum[ct][t] = (f32x4){0.f, 0.f, 0.f, 0.f};
+    for (int t = 0; t < TILES; ++t) columns.sum[ct][t] = (f32x4){0.f, 0.f, 0.f, 0.f};
   }
 
-  for (int segment = begin; segment < end; segment += SEGMENT) {
-    const int segment_end = min(end, segment + SEGMENT), first_entry = segment / page_size, last_entry = (segment_end + KEYS - 1 - (segment_end + KEYS - 1) % KEYS - 1) / page_size;
-    __syncthreads();
-    for (int i = first_entry + threadIdx.x; i <= last_entry; i += WAVES * WAVE) {
-      const int entry = i < w.table_width ? w.tables[(size_t)item.request * w.table_width + i] : 0;
-      entries[i - first_entry] = (unsigned)entry < (unsigned)w.num_pages ? entry : 0;
+  // (the queries have come, and with them what was asked for before: from here on the loads that are counted are those of steps)
+#pragma unroll
+  for (int ct = 0; ct < CT; ++ct)
+#pragma unroll
+    for (int k = 0; k < TERMS; ++k)
+#pragma unroll
+      for (int s = 0; s < SLICES; ++s) asm volatile("" : "+v"(columns.query[ct][k][s].u));
+  wait_for_asked<0>();
+  int stage = 0, base = own;
+  const auto next_step = [&](Step& now) {
+    if (base + (STAGES - 1) * WAVES * KEYS < end) wait_for_asked<(STAGES - 1) * ASKS>();
+    else wait_for_asked<0>();
+    read_step(now, ring + stage * STAGE);
+    if (asked < end) {
+      ask_step(ring + stage * STAGE, from, w, place, lane_parts);
+      asked += WAVES * KEYS;
+      if (asked < end) find_place(place, w, table, asked);
     }
-    __syncthreads();
-    int base = segment + wave * KEYS;
-    if (base >= segment_end) continue;
+    stage = stage + 1 == STAGES ? 0 : stage + 1;
+  };
+  // the steps that all columns see whole lie side by side
+  const int whole_from = w.window > 0 ? item.last_position - w.window + 1 : 0, whole_to = min(end, item.first_position - KEYS + 2);
+  for (; base < end; base += WAVES * KEYS) {
+    for (; base >= whole_from && base < whole_to; base += WAVES * KEYS) {
+      Step now;
+      next_step(now);
+      take_step<T, CT, false>(columns, now, w, item, base);
+    }
+    if (base >= end) break;
     Step now;
-    load_step(now, p, entries, first_entry, base);
-    for (; base < segment_end; base += WAVES * KEYS) {
-      Step next;
-      const int following = base + WAVES * KEYS;
-      if (following < segment_end) load_step(next, p, entries, first_entry, following);
-      // scores: row 4 g + i of tile t is key 8 g + 4 t + i of the step
-      f32x4 score[CT][2];
-#pragma unroll
-      for (int t = 0; t < 2; ++t) {
-#pragma unroll
-        for (int ct = 0; ct < CT; ++ct) score[ct][t] = (f32x4){0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-        for (int s = 0; s < SLICES; ++s) {
-          const float power = packed_power(now.key_powers[t][D % 128 == 0 ? s / 4 : D <= 64 ? 0 : s]);
-          Eight key;
-          key.u = (u32x4){unpack_pair<0>(now.keys[t][s], power), unpack_pair<1>(now.keys[t][s], power), unpack_pair<2>(now.keys[t][s], power), unpack_pair<3>(now.keys[t][s], power)};
-#pragma unroll
-          for (int ct = 0; ct < CT; ++ct)
-#pragma unroll
-            for (int k = TERMS - 1; k >= 0; --k) score[ct][t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(key.v, query[ct][k][s].v, score[ct][t], 0, 0, 0);
-        }
-      }
-      const bool edge = base + KEYS - 1 > item.first_position || (w.window > 0 && base < item.last_position - w.window + 1);
-      Eight weight[CT][TERMS];
-#pragma unroll
-      for (int ct = 0; ct < CT; ++ct) {
-        float x[8];
-#pragma unroll
-        for (int i = 0; i < 8; ++i) x[i] = score[ct][i / 4][i % 4] * w.scale;
-        if (edge) {
-#pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            const int key = base + 8 * g + i;
-            if (key > position[ct] || (w.window > 0 && key <= position[ct] - w.window)) x[i] = -INFINITY;
-          }
-        }
-        float largest = fmaxf(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])), fmaxf(fmaxf(x[4], x[5]), fmaxf(x[6], x[7])));
-        if (__any(largest > reference[ct] + AHEAD)) {
-          largest = fmaxf(largest, __shfl_xor(largest, 16));
-          largest = fmaxf(largest, __shfl_xor(largest, 32));
-          largest = fmaxf(largest, reference[ct]);
-          const float change = reference[ct] == largest ? 1.f : __builtin_amdgcn_exp2f(reference[ct] - largest);
-          reference[ct] = largest;
-          total[ct] *= change;
-#pragma unroll
-          for (int t = 0; t < TILES; ++t) sum[ct][t] *= change;
-        }
-#pragma unroll
-        for (int i = 0; i < 8; ++i) x[i] = x[i] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(x[i] - reference[ct]);
-        split_eight<T, TERMS>(x, weight[ct]);
-        if (TERMS == 1) {  // the weights that are multiplied are the weights that are added up
-#pragma unroll
-          for (int i = 0; i < 8; ++i) x[i] = (float)weight[ct][0].v[i];
-        }
-        total[ct] += ((x[0] + x[1]) + (x[2] + x[3])) + ((x[4] + x[5]) + (x[6] + x[7]));
-      }
-#pragma unroll
-      for (int c = 0; c < CHUNKS; ++c) {
-        const int width = chunk_width(c), pairs = width / 32;  // pairs of elements that a lane takes of a key
-        u32x2 powers = now.value_powers[c];
-        bool poisoned = false;
-        Eight marks;
-        if (edge) {
-          // A value that a column does not see has no part in it, whatever it is: keys beyond the last that any column sees get the smallest power;
-          // of the others, those that are no number are taken out, and put back where they are seen.
-          marks.u = (u32x4){0u, 0u, 0u, 0u};
-          bool mine = false;
-#pragma unroll
-          for (int j = 0; j < 8; ++j) {
-            const int key = base + 8 * g + j;
-            const unsigned shift = (j & 3) * 8, byte = (powers[j / 4] >> shift) & 255u;
-            const bool unseen = key > item.last_position || (w.window > 0 && key <= item.first_position - w.window), bad = byte == PACKED_NO_NUMBER;
-            if (unseen || bad) powers[j / 4] &= ~(255u << shift);
-            if (bad && !unseen) {
-              marks.u[j / 2] |= 0x3f80u << (j % 2 * 16);
-              mine = true;
-            }
-          }
-          poisoned = __any(mine);
-        }
-        u32x4 turned[8];  // element e of the lane's, eight keys
-        {
-          unsigned raw[8][4];
-#pragma unroll
-          for (int j = 0; j < 8; ++j) {
-            const float power = __uint_as_float(j % 4 == 3 ? powers[j / 4] >> 1 : powers[j / 4] << (23 - j % 4 * 8));  // (only the exponent of it counts)
-            unsigned codes = now.values[c][j / 4][j % 4];
-            if (width == 64) codes >>= (r & 1) * 16;
-            if (width == 32) codes >>= (r & 3) * 8;
-            raw[j][0] = unpack_pair<0>(codes, power);
-            if (pairs > 1) raw[j][1] = unpack_pair<1>(codes, power);
-            if (pairs > 2) {
-              raw[j][2] = unpack_pair<2>(codes, power);
-              raw[j][3] = unpack_pair<3>(codes, power);
-            }
-          }
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            if (e >= pairs) continue;
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-              turned[2 * e][j] = __builtin_amdgcn_perm(raw[2 * j + 1][e], raw[2 * j][e], 0x05040100u);
-              turned[2 * e + 1][j] = __builtin_amdgcn_perm(raw[2 * j + 1][e], raw[2 * j][e], 0x07060302u);
-            }
-          }
-        }
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          if (e >= 2 * pairs) continue;
-          Eight value;
-          value.u = turned[e];
-          const int t = chunk_first(c) / 16 + e;
-#pragma unroll
-          for (int ct = 0; ct < CT; ++ct)
-#pragma unroll
-            for (int k = TERMS - 1; k >= 0; --k) sum[ct][t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(value.v, weight[ct][k].v, sum[ct][t], 0, 0, 0);
-        }
-        if (poisoned) {
-#pragma unroll
-          for (int ct = 0; ct < CT; ++ct) {
-            Eight seen;
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-              const int key = base + 8 * g + i;
-              seen.v[i] = (bf16_t)(key > position[ct] || (w.window > 0 && key <= position[ct] - w.window) ? 0.f : 1.f);
-            }
-            const f32x4 hit = __builtin_amdgcn_mfma_f32_16x16x32_bf16(marks.v, seen.v, (f32x4){0.f, 0.f, 0.f, 0.f}, 0, 0, 0);
-#pragma unroll
-            for (int e = 0; e < 8; ++e) {
-              if (e >= 2 * pairs) continue;
-#pragma unroll
-              for (int i = 0; i < 4; ++i)
-                if (hit[i] > 0.f) sum[ct][chunk_first(c) / 16 + e][i] = __uint_as_float(0x7fc00000u);
-            }
-          }
-        }
-      }
-      now = next;
-    }
+    next_step(now);
+    take_step<T, CT, true>(columns, now, w, item, base);
   }
 
   // the waves' sums, brought together
@@ -377,12 +499,9 @@ __global__ void __launch_bounds__(WAVES * WAVE) packed_attention_kernel(const T*
   for (int ct = 0; ct < CT; ++ct) {
     if (ct * 16 >= item.columns) break;
     __syncthreads();
-    float wave_total = total[ct];
-    wave_total += __shfl_xor(wave_total, 16);
-    wave_total += __shfl_xor(wave_total, 32);
     if (g == 0) {
-      sums[wave][r][0] = reference[ct];
-      sums[wave][r][1] = wave_total;
+      sums[wave][r][0] = columns.reference[ct];
+      sums[wave][r][1] = columns.total[ct][0];
     }
 #pragma unroll
     for (int c = 0; c < CHUNKS; ++c) {
@@ -391,7 +510,7 @@ __global__ void __launch_bounds__(WAVES * WAVE) packed_attention_kernel(const T*
       for (int i = 0; i < 4; ++i)
 #pragma unroll
         for (int e = 0; e < 8; ++e)
-          if (e < each) results[wave][r][chunk_first(c) + (4 * g + i) * each + e] = sum[ct][chunk_first(c) / 16 + e][i];
+          if (e < each) results[wave][r][chunk_first(c) + (4 * g + i) * each + e] = columns.sum[ct][chunk_first(c) / 16 + e][i];
     }
     __syncthreads();
     const int columns = min(16, item.columns - ct * 16);
@@ -414,65 +533,67 @@ __global__ void __launch_bounds__(WAVES * WAVE) packed_attention_kernel(const T*
         const float over = 1.f / weights;
 #pragma unroll
         for (int i = 0; i < 4; ++i) out[row * out_stride + head * D + d + i] = from_float<T>(result[i] * over);
+        if (d == 0 && w.splits > 1) partial[(row * w.heads + head) * w.splits * (D + 4) + D + 2] = __int_as_float(1);
       } else {
         float* to = partial + ((row * w.heads + head) * w.splits + split) * (D + 4);
         *(f32x4*)(to + d) = result;
-        if (d == 0) {
-          to[D] = largest;
-          to[D + 1] = weights;
-        }
+        if (d == 0) *(f32x4*)(to + D) = (f32x4){largest, weights, __int_as_float(parts), 0.f};
       }
     }
   }
 }
 
-// A wave a (token, head) whose keys were split: its parts joined.
+// A wave a (token, head) whose keys were split: its parts joined.  A part is D sums, the reference that their weights are relative to, the weights' sum, and
+// (in the first one) how many parts there are; all of them are asked for at once.
+constexpr int JOIN_LANES = D / 4, JOINED = WAVE / JOIN_LANES;  // lanes a part, parts side by side
+constexpr int MOST_PARTS = WAVE;
+
 template <typename T>
-__global__ void __launch_bounds__(WAVE) packed_join_kernel(T* out, int out_stride, const float* partial, Walk w, int most) {
-  const int token = blockIdx.x, head = blockIdx.y, lane = threadIdx.x, group = w.heads / w.kv_heads;
-  int low = 0, high = w.requests;  // the first request that ends behind the token
-  while (low < high) {
-    const int middle = (low + high) / 2;
-    if (w.query_start[middle + 1] > token) high = middle;
-    else low = middle + 1;
+__global__ void __launch_bounds__(WAVE) packed_join_kernel(T* out, int out_stride, const float* partial, const int* query_start, int requests, int heads, int splits) {
+  const int token = blockIdx.x, head = blockIdx.y, lane = threadIdx.x;
+  const float* mine = partial + ((size_t)token * heads + head) * splits * (D + 4);
+  const int tokens = query_start[requests], parts = min(__float_as_int(mine[D + 2]), splits);
+  if (token >= tokens || parts <= 1) return;
+  const int which = min(lane / JOIN_LANES, JOINED - 1), d = lane % JOIN_LANES * 4;
+  float reference = -INFINITY, total = 0.f;
+  if (lane < parts) {
+    reference = mine[lane * (D + 4) + D];
+    total = mine[lane * (D + 4) + D + 1];
   }
-  if (low == w.requests || token < w.query_start[low]) return;
-  const int start = w.query_start[low], count = w.query_start[low + 1] - start, past = w.contexts[low] - count;
-  const int first = ((token - start) * group + head % group) / most * most, columns = min(most, count * group - first);
-  const int from = w.window > 0 ? max(0, past + first / group - w.window + 1) / KEYS * KEYS : 0, to = past + (first + columns - 1) / group + 1;
-  const int parts = (to - from + w.chunk - 1) / w.chunk;
-  if (parts <= 1) return;
-  const float* mine = partial + ((size_t)token * w.heads + head) * w.splits * (D + 4);
-  float largest = -INFINITY;
-  for (int i = 0; i < parts; ++i) largest = fmaxf(largest, mine[(size_t)i * (D + 4) + D]);
-  constexpr int EACH = (D + WAVE - 1) / WAVE;
-  float result[EACH] = {}, weights = 0.f;
-  for (int i = 0; i < parts; ++i) {
-    const float* part = mine + (size_t)i * (D + 4);
-    const float share = part[D] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(part[D] - largest);
-    weights += share * part[D + 1];
-#pragma unroll
-    for (int e = 0; e < EACH; ++e)
-      if (lane + e * WAVE < D) result[e] += share * part[lane + e * WAVE];
+  const float largest = wave_max(reference), share = reference == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(reference - largest);
+  f32x4 result = (f32x4){0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+  for (int i = 0; i < parts; i += JOINED) {
+    const float weight = __shfl(share, min(i + which, WAVE - 1));
+    if (i + which < parts) result += weight * *(const f32x4*)(mine + (i + which) * (D + 4) + d);
   }
+  const float weights = wave_sum(share * total);
 #pragma unroll
-  for (int e = 0; e < EACH; ++e)
-    if (lane + e * WAVE < D) out[(size_t)token * out_stride + head * D + lane + e * WAVE] = from_float<T>(result[e] / weights);
+  for (int other = 1; other < JOINED; ++other)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float far = __shfl(result[i], min(lane + other * JOIN_LANES, WAVE - 1));
+      if (lane < JOIN_LANES) result[i] += far;
+    }
+  if (lane >= JOIN_LANES) return;
+  const float over = 1.f / weights;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) out[(size_t)token * out_stride + head * D + d + i] = from_float<T>(result[i] * over);
 }
 
 template <typename T>
-static int launch(const void* q, int q_stride, void* out, int out_stride, float* partial, const void* pages, int page_size, const Walk& w, int tokens, int column_tiles, hipStream_t stream) {
+static int launch(const void* q, int q_stride, void* out, int out_stride, float* partial, const void* pages, const Walk& w, int tokens, int column_tiles, hipStream_t stream) {
   const int group = w.heads / w.kv_heads, most = 16 * column_tiles;
   const long items = w.single ? (long)w.requests * ((group + most - 1) / most) : ((long)tokens * group + most - 1) / most + w.requests;
   const long blocks = items * w.kv_heads * w.splits;
   if (items >= (1L << 31) || blocks >= (1L << 31)) return ERR_BAD_ARGUMENT;
   const int piece = sizeof(T) == 4 ? 4 : 8, whole = (size_t)q % 16 == 0 && q_stride % piece == 0;
   if (column_tiles == 1)
-    packed_attention_kernel<T, 1><<<(unsigned)blocks, WAVES * WAVE, 0, stream>>>((const T*)q, q_stride, (T*)out, out_stride, partial, (const unsigned char*)pages, page_size, w, (int)items, whole);
+    packed_attention_kernel<T, 1><<<(unsigned)blocks, WAVES * WAVE, 0, stream>>>((const T*)q, q_stride, (T*)out, out_stride, partial, (const unsigned char*)pages, w, (int)items, whole);
   else
-    packed_attention_kernel<T, 2><<<(unsigned)blocks, WAVES * WAVE, 0, stream>>>((const T*)q, q_stride, (T*)out, out_stride, partial, (const unsigned char*)pages, page_size, w, (int)items, whole);
+    packed_attention_kernel<T, 2><<<(unsigned)blocks, WAVES * WAVE, 0, stream>>>((const T*)q, q_stride, (T*)out, out_stride, partial, (const unsigned char*)pages, w, (int)items, whole);
   if (int status = LAUNCH_STATUS()) return status;
-  if (w.splits > 1) packed_join_kernel<T><<<dim3(tokens, w.heads), WAVE, 0, stream>>>((T*)out, out_stride, partial, w, most);
+  if (w.splits > 1) packed_join_kernel<T><<<dim3(tokens, w.heads), WAVE, 0, stream>>>((T*)out, out_stride, partial, w.query_start, w.requests, w.heads, w.splits);
   return LAUNCH_STATUS();
 }
 
@@ -484,10 +605,14 @@ extern "C" int llmserve_packed_attention(const void* q, int is_float, int q_stri
                                          int chunk, int splits, hipStream_t stream) {
   if (tokens == 0 || requests == 0) return 0;
   if (!q || !out || !pages || !tables || !query_start || !contexts || requests < 0 || tokens < 0 || kv_heads <= 0 || heads <= 0 || heads % kv_heads || num_pages <= 0 || table_width <= 0 ||
-      !packed_fits(D, page_size) || (size_t)pages % 16 || q_stride < heads * D || out_stride < heads * D || window < 0 || column_tiles < 1 || column_tiles > 2 || chunk < 128 || chunk % 128 ||
-      splits < 1 || splits > 65535 || (splits > 1 && (!partial || (size_t)partial % 16)) || heads > 65535)
+      !packed_fits(D, page_size) || (long)page_size * D * kv_heads >= (1L << 30) || !(scale > 0.f) || (size_t)pages % 16 || q_stride < heads * D || out_stride < heads * D || window < 0 || column_tiles < 1 || column_tiles > 2 || chunk < 128 || chunk % 128 ||
+      splits < 1 || splits > MOST_PARTS || (splits > 1 && (!partial || (size_t)partial % 16)) || heads > 65535)
     return ERR_BAD_ARGUMENT;
-  const Walk w = {tables, table_width, num_pages, query_start, contexts, requests, heads, kv_heads, window, single, chunk, splits, scale * LOG2_E};
-  if (is_float) return launch<float>(q, q_stride, out, out_stride, (float*)partial, pages, page_size, w, tokens, column_tiles, stream);
-  return launch<bf16_t>(q, q_stride, out, out_stride, (float*)partial, pages, page_size, w, tokens, column_tiles, stream);
+  const unsigned per_page = (unsigned)page_size / 8;
+  const bool power_of_two = (per_page & (per_page - 1)) == 0;
+  // (a quotient by the reciprocal is exact below 2^32 over the divisor)
+  if (!power_of_two && (unsigned long)(table_width + 1) * per_page * per_page >= (1UL << 32)) return ERR_BAD_ARGUMENT;
+  const Walk w = {tables, table_width, num_pages, page_size, power_of_two ? 31 - __builtin_clz(per_page) : -1, (unsigned)(((1UL << 32) + per_page - 1) / per_page), query_start, contexts, requests, heads, kv_heads, window, single, chunk, splits, scale * LOG2_E};
+  if (is_float) return launch<float>(q, q_stride, out, out_stride, (float*)partial, pages, w, tokens, column_tiles, stream);
+  return launch<bf16_t>(q, q_stride, out, out_stride, (float*)partial, pages, w, tokens, column_tiles, stream);
 }

@@ -1778,7 +1778,7 @@ class HipKernels:
         walk = min(batch.max_context_length, window + batch.max_query_length) + 31 if window else batch.max_context_length
         blocks = items * kv_heads
         chunk = max(256, -(-walk * blocks // 1024))
-        chunk = -(-chunk // 128) * 128
+        chunk = max(-(-chunk // 128) * 128, -(-walk // (64 * 128)) * 128)
         return tiles, chunk, max(1, -(-walk // chunk))
 
     def _packed_attention(self, qkv, layout, batch, cell, scale: float, window: int | None, out):
