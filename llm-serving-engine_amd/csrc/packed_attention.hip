@@ -30,7 +30,8 @@ constexpr int D = HEAD_DIM;
 constexpr int SLICES = D / 32;                // MFMA steps over D, and four-byte pieces of codes that a lane takes of a key
 constexpr int TILES = D / 16;                 // tiles of O^T
 constexpr int KEYS = 32;                      // keys a step
-constexpr int WAVES = 4;
+constexpr int WAVES = 8;                      // of a workgroup over single tokens
+constexpr int UNIT = WAVES * KEYS;            // keys that its waves take side by side: what work is counted in
 constexpr int STAGES = 2;                     // steps that a wave has asked for
 constexpr int PIECE = 8 * D + 16;             // bytes in LDS of the codes of eight keys and values (16 spare: the same rows of two pieces lie in other banks)
 constexpr int STAGE = 4 * PIECE + 2 * D;      // of a step: four pieces, and their powers
@@ -59,8 +60,7 @@ struct Walk {
   int page_size, page_shift;                  // log2 of the pieces of eight keys that a page holds, or -1
   unsigned page_reciprocal;                   // 2^32 over them, rounded up
   const int *query_start, *contexts;
-  int requests, heads, kv_heads, window, single;
-  int chunk, splits;                          // keys a workgroup walks, and the most workgroups that share a run of columns
+  int requests, heads, kv_heads, window;
   float scale;                                // times log2 e
 };
 
@@ -68,52 +68,55 @@ struct Item {                                 // a run of columns
   int request, first_row, group, first, columns, first_position, last_position, from, to;
 };
 
-// Item `index`: the requests' columns in runs of `most`, one request's behind the other's.  False: there is no such item.
-__device__ __forceinline__ bool find_item(const Walk& w, int index, int most, Item& item) {
-  item.group = w.heads / w.kv_heads;
-  int request, inside;
-  if (w.single) {                             // no request brings more than one token
-    const int each = (item.group + most - 1) / most;
-    request = index / each;
-    inside = index - request * each;
-  } else {                                    // each wave for itself: 64 requests at a time
-    const int lane = threadIdx.x % WAVE;
-    int before = 0;
-    request = -1;
-    for (int base = 0; base < w.requests; base += WAVE) {
-      const int b = base + lane;
-      const int items = b < w.requests ? ((w.query_start[b + 1] - w.query_start[b]) * item.group + most - 1) / most : 0;
-      int sum = items;
-#pragma unroll
-      for (int step = 1; step < WAVE; step <<= 1) {
-        const int other = __shfl_up(sum, step);
-        if (lane >= step) sum += other;
-      }
-      const unsigned long long found = __ballot(before + sum > index);
-      if (found) {
-        const int which = __ffsll((unsigned long long)found) - 1;
-        request = base + which;
-        inside = index - before - __shfl(sum - items, which);
-        break;
-      }
-      before += __shfl(sum, WAVE - 1);
-    }
-    if (request < 0) return false;
-  }
-  request = __builtin_amdgcn_readfirstlane(request);
-  if (request >= w.requests) return false;
-  const int start = w.query_start[request], count = w.query_start[request + 1] - start;
-  item.request = request;
-  item.first = __builtin_amdgcn_readfirstlane(inside) * most;
-  item.columns = min(most, count * item.group - item.first);
-  if (item.columns <= 0) return false;
-  item.first_row = start;
-  const int past = w.contexts[request] - count;
-  item.first_position = past + item.first / item.group;
-  item.last_position = past + (item.first + item.columns - 1) / item.group;
+// Few columns: those of a single token, or of some that fit one tile of 16.
+__device__ __forceinline__ bool few_columns(int count, int group) { return count == 1 || count * group <= 16; }
+
+struct Request {
+  int start, count, context;                  // rows in the step, keys behind it
+};
+__device__ __forceinline__ Request load_request(const Walk& w, int request) {
+  const int start = w.query_start[request];
+  return {start, w.query_start[request + 1] - start, w.contexts[request]};
+}
+
+// The run of up to `most` columns from `first` on of a request.  False: it has none there.
+__device__ __forceinline__ bool make_item(const Walk& w, int index, const Request& request, int first, int most, Item& item) {
+  const int group = w.heads / w.kv_heads;
+  item.request = index;
+  item.group = group;
+  item.first = first;
+  item.columns = min(most, request.count * group - first);
+  item.first_row = request.start;
+  const int past = request.context - request.count;
+  item.first_position = past + first / group;
+  item.last_position = past + (first + item.columns - 1) / group;
   item.from = w.window > 0 ? max(0, item.first_position - w.window + 1) / KEYS * KEYS : 0;
   item.to = item.last_position + 1;
-  return true;
+  return item.columns > 0 && item.to > item.from;
+}
+
+// Item `index` of the requests of many columns, in runs of `most`, one request's behind the other's.  False: there is no such item.  (each wave for itself, 64 requests at a time)
+__device__ __forceinline__ bool find_item(const Walk& w, int index, int most, Item& item) {
+  const int lane = threadIdx.x % WAVE, group = w.heads / w.kv_heads;
+  int before = 0;
+  for (int base = 0; base < w.requests; base += WAVE) {
+    const int b = base + lane, count = b < w.requests ? w.query_start[b + 1] - w.query_start[b] : 0;
+    const int items = few_columns(count, group) ? 0 : (count * group + most - 1) / most;
+    int sum = items;
+#pragma unroll
+    for (int step = 1; step < WAVE; step <<= 1) {
+      const int other = __shfl_up(sum, step);
+      if (lane >= step) sum += other;
+    }
+    const unsigned long long found = __ballot(before + sum > index);
+    if (found) {
+      const int which = __ffsll((unsigned long long)found) - 1, inside = index - before - __shfl(sum - items, which);
+      const int request = __builtin_amdgcn_readfirstlane(base + which);
+      return make_item(w, request, load_request(w, request), __builtin_amdgcn_readfirstlane(inside) * most, most, item);
+    }
+    before += __shfl(sum, WAVE - 1);
+  }
+  return false;
 }
 
 typedef const int __attribute__((address_space(4))) Scalar;  // read by scalar loads: what no kernel writes meanwhile
@@ -396,41 +399,11 @@ __device__ __forceinline__ void take_step(Columns<T, CT>& columns, const Step& n
   }
 }
 
+// Rows in memory as a wave's queries.
 template <typename T, int CT>
-__global__ void __launch_bounds__(WAVES * WAVE, 2) packed_attention_kernel(const T* q, int q_stride, T* out, int out_stride, float* partial, const unsigned char* pages, Walk w, int items, int whole) {
-  constexpr int TERMS = sizeof(T) == 4 ? 3 : 1;
-  constexpr int RING = WAVES * STAGES * STAGE, RESULTS = WAVES * 16 * (D + 4) * 4;
-  __shared__ __attribute__((aligned(16))) unsigned char memory[RING > RESULTS ? RING : RESULTS];  // the steps' codes, and the waves' sums behind them
-  float (*results)[16][D + 4] = (float (*)[16][D + 4])memory;
-  __shared__ float sums[WAVES][16][2];
-  const int lane = threadIdx.x % WAVE, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / WAVE), r = lane & 15, g = lane >> 4;
-  // the longest walks begin first: a request's last columns walk most keys
-  const int all = items * w.kv_heads, at = blockIdx.x % all, split = blockIdx.x / all;
-  const int kv_head = at % w.kv_heads;
-  Item item;
-  if (!find_item(w, items - 1 - at / w.kv_heads, 16 * CT, item)) return;
-  // as many parts as it takes, all of one length
-  const int parts = (item.to - item.from + w.chunk - 1) / w.chunk;
-  if (split >= parts) return;
-  const int each = ((item.to - item.from + parts - 1) / parts + WAVES * KEYS - 1) / (WAVES * KEYS) * (WAVES * KEYS);
-  const int begin = item.from + split * each, end = min(item.to, begin + each);
-  const unsigned char* from = pages + (size_t)kv_head * (w.page_size * (D + D / 16));
-  Scalar* table = (Scalar*)w.tables + (size_t)item.request * w.table_width;
-
-  unsigned char* ring = memory + wave * (STAGES * STAGE);
-  const LaneParts lane_parts = parts_of_lane(w.page_size);
-  const int own = __builtin_amdgcn_readfirstlane(begin + wave * KEYS);
-  Place place;
-  int asked = own;
-#pragma unroll
-  for (int s = 0; s < STAGES; ++s)
-    if (asked < end) {
-      find_place(place, w, table, asked);
-      ask_step(ring + s * STAGE, from, w, place, lane_parts);
-      asked += WAVES * KEYS;
-    }
-  if (asked < end) find_place(place, w, table, asked);
-  Columns<T, CT> columns;
+__device__ __forceinline__ void load_queries(Columns<T, CT>& columns, const T* q, int q_stride, const Item& item, int kv_head, bool whole) {
+  constexpr int TERMS = Columns<T, CT>::TERMS;
+  const int lane = threadIdx.x % WAVE, r = lane & 15, g = lane >> 4;
 #pragma unroll
   for (int ct = 0; ct < CT; ++ct) {
     const int column = min(ct * 16 + r, item.columns - 1), flat = item.first + column, token = flat / item.group;
@@ -459,31 +432,48 @@ __global__ void __launch_bounds__(WAVES * WAVE, 2) packed_attention_kernel(const
 #pragma unroll
     for (int t = 0; t < TILES; ++t) columns.sum[ct][t] = (f32x4){0.f, 0.f, 0.f, 0.f};
   }
+}
 
+// A wave's steps of the keys begin .. end (begin a multiple of 32): every W-th from its own on.  ring: STAGES stages of LDS that are its own.
+template <typename T, int CT, int W>
+__device__ __forceinline__ void walk_keys(Columns<T, CT>& columns, const T* q, int q_stride, const unsigned char* pages, const Walk& w, const Item& item, int kv_head, bool whole, int begin, int end, int wave, unsigned char* ring) {
+  const unsigned char* from = pages + (size_t)kv_head * (w.page_size * (D + D / 16));
+  Scalar* table = (Scalar*)w.tables + (size_t)item.request * w.table_width;
+  const LaneParts lane_parts = parts_of_lane(w.page_size);
+  Place place;
+  int base = __builtin_amdgcn_readfirstlane(begin + wave * KEYS), asked = base, stage = 0;
+#pragma unroll
+  for (int s = 0; s < STAGES; ++s)
+    if (asked < end) {
+      find_place(place, w, table, asked);
+      ask_step(ring + s * STAGE, from, w, place, lane_parts);
+      asked += W * KEYS;
+    }
+  if (asked < end) find_place(place, w, table, asked);
+  load_queries(columns, q, q_stride, item, kv_head, whole);
   // (the queries have come, and with them what was asked for before: from here on the loads that are counted are those of steps)
 #pragma unroll
   for (int ct = 0; ct < CT; ++ct)
 #pragma unroll
-    for (int k = 0; k < TERMS; ++k)
+    for (int k = 0; k < Columns<T, CT>::TERMS; ++k)
 #pragma unroll
       for (int s = 0; s < SLICES; ++s) asm volatile("" : "+v"(columns.query[ct][k][s].u));
   wait_for_asked<0>();
-  int stage = 0, base = own;
   const auto next_step = [&](Step& now) {
-    if (base + (STAGES - 1) * WAVES * KEYS < end) wait_for_asked<(STAGES - 1) * ASKS>();
+    if (base + (STAGES - 1) * W * KEYS < end) wait_for_asked<(STAGES - 1) * ASKS>();
     else wait_for_asked<0>();
     read_step(now, ring + stage * STAGE);
     if (asked < end) {
       ask_step(ring + stage * STAGE, from, w, place, lane_parts);
-      asked += WAVES * KEYS;
+      asked += W * KEYS;
       if (asked < end) find_place(place, w, table, asked);
     }
     stage = stage + 1 == STAGES ? 0 : stage + 1;
   };
   // the steps that all columns see whole lie side by side
   const int whole_from = w.window > 0 ? item.last_position - w.window + 1 : 0, whole_to = min(end, item.first_position - KEYS + 2);
-  for (; base < end; base += WAVES * KEYS) {
-    for (; base >= whole_from && base < whole_to; base += WAVES * KEYS) {
+  for (; base < end; base += W * KEYS) {
+    for (; base >= whole_from && base < whole_to; base += W * KEYS) {
       Step now;
       next_step(now);
       take_step<T, CT, false>(columns, now, w, item, base);
@@ -493,81 +483,198 @@ __global__ void __launch_bounds__(WAVES * WAVE, 2) packed_attention_kernel(const
     next_step(now);
     take_step<T, CT, true>(columns, now, w, item, base);
   }
+}
 
-  // the waves' sums, brought together
+// The sums of W waves over a tile of 16 columns, brought together through LDS: take(column, d, four sums from element d on, the weights' reference, their sum).
+// memory: W * 16 * (D + 6) floats, free when all waves have come here.
+template <typename T, int CT, int W, typename Take>
+__device__ __forceinline__ void bring_together(const Columns<T, CT>& columns, int ct, int count, int wave, unsigned char* memory, Take take) {
+  float (*results)[16][D + 4] = (float (*)[16][D + 4])memory;
+  float (*sums)[16][2] = (float (*)[16][2])(memory + W * 16 * (D + 4) * 4);
+  const int lane = threadIdx.x % WAVE, r = lane & 15, g = lane >> 4;
+  __syncthreads();
+  if (g == 0) {
+    sums[wave][r][0] = columns.reference[ct];
+    sums[wave][r][1] = columns.total[ct][0];
+  }
 #pragma unroll
-  for (int ct = 0; ct < CT; ++ct) {
-    if (ct * 16 >= item.columns) break;
-    __syncthreads();
-    if (g == 0) {
-      sums[wave][r][0] = columns.reference[ct];
-      sums[wave][r][1] = columns.total[ct][0];
+  for (int c = 0; c < CHUNKS; ++c) {
+    const int each = chunk_width(c) / 16;  // neighbouring elements of a row of the tiles
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+        if (e < each) results[wave][r][chunk_first(c) + (4 * g + i) * each + e] = columns.sum[ct][chunk_first(c) / 16 + e][i];
+  }
+  __syncthreads();
+  for (int at = threadIdx.x; at < count * (D / 4); at += W * WAVE) {
+    const int column = at / (D / 4), d = (at - column * (D / 4)) * 4;
+    float largest = sums[0][column][0];
+#pragma unroll
+    for (int v = 1; v < W; ++v) largest = fmaxf(largest, sums[v][column][0]);
+    f32x4 result = (f32x4){0.f, 0.f, 0.f, 0.f};
+    float weights = 0.f;
+#pragma unroll
+    for (int v = 0; v < W; ++v) {
+      const float share = sums[v][column][0] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(sums[v][column][0] - largest);
+      weights += share * sums[v][column][1];
+      result += share * *(const f32x4*)&results[v][column][d];
     }
-#pragma unroll
-    for (int c = 0; c < CHUNKS; ++c) {
-      const int each = chunk_width(c) / 16;  // neighbouring elements of a row of the tiles
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-#pragma unroll
-        for (int e = 0; e < 8; ++e)
-          if (e < each) results[wave][r][chunk_first(c) + (4 * g + i) * each + e] = columns.sum[ct][chunk_first(c) / 16 + e][i];
-    }
-    __syncthreads();
-    const int columns = min(16, item.columns - ct * 16);
-    for (int at = threadIdx.x; at < columns * (D / 4); at += WAVES * WAVE) {
-      const int column = at / (D / 4), d = (at - column * (D / 4)) * 4;
-      float largest = sums[0][column][0];
-#pragma unroll
-      for (int v = 1; v < WAVES; ++v) largest = fmaxf(largest, sums[v][column][0]);
-      f32x4 result = (f32x4){0.f, 0.f, 0.f, 0.f};
-      float weights = 0.f;
-#pragma unroll
-      for (int v = 0; v < WAVES; ++v) {
-        const float share = sums[v][column][0] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(sums[v][column][0] - largest);
-        weights += share * sums[v][column][1];
-        result += share * *(const f32x4*)&results[v][column][d];
-      }
-      const int flat = item.first + ct * 16 + column, token = flat / item.group, head = kv_head * item.group + flat - token * item.group;
-      const size_t row = item.first_row + token;
-      if (parts == 1) {
-        const float over = 1.f / weights;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) out[row * out_stride + head * D + d + i] = from_float<T>(result[i] * over);
-        if (d == 0 && w.splits > 1) partial[(row * w.heads + head) * w.splits * (D + 4) + D + 2] = __int_as_float(1);
-      } else {
-        float* to = partial + ((row * w.heads + head) * w.splits + split) * (D + 4);
-        *(f32x4*)(to + d) = result;
-        if (d == 0) *(f32x4*)(to + D) = (f32x4){largest, weights, __int_as_float(parts), 0.f};
-      }
-    }
+    take(column, d, result, largest, weights);
   }
 }
 
-// A wave a (token, head) whose keys were split: its parts joined.  A part is D sums, the reference that their weights are relative to, the weights' sum, and
-// (in the first one) how many parts there are; all of them are asked for at once.
-constexpr int JOIN_LANES = D / 4, JOINED = WAVE / JOIN_LANES;  // lanes a part, parts side by side
-constexpr int MOST_PARTS = WAVE;
+template <typename T> __device__ __forceinline__ void write_four(T* to, f32x4 x) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) to[i] = from_float<T>(x[i]);
+}
+
+template <int W> constexpr int memory_of() {
+  constexpr int RING = W * STAGES * STAGE, RESULTS = W * 16 * (D + 6) * 4;
+  return RING > RESULTS ? RING : RESULTS;
+}
+
+// ---------------------------------------------------------------------------------------------------------------- few columns
+//
+// Single tokens read all their keys for a handful of columns: the path from memory is what bounds them.  The walks of all (request, tile of 16 columns, kv
+// head) lie behind each other, counted in units of 256 keys, and every workgroup takes an equal run of units, wherever in a walk it begins or ends: ragged contexts leave no workgroup
+// with more than another.  A walk that one workgroup takes whole is written as it ends.  Of one that is cut every workgroup leaves its part, in a place of its
+// own: a workgroup has at most two such, the one that it begins with (place 0) and the one that it breaks off (place 1); who begins a
+// walk and breaks it off notes it for the join.
+struct Cut {
+  int first_row, group, first, columns, kv_head, parts, place, spare;  // parts 0: none; place: of the first part, the others lie at place 0 of the workgroups behind
+};
+constexpr int PART = 16 * (D + 4);  // floats of a part: 16 columns of D sums, their reference, the sum of their weights, two spare
+
+struct Streams {
+  float* parts;                               // [workgroups][2][PART]
+  Cut* cuts;                                  // [workgroups]
+  int least;                                  // units a workgroup takes at least; 0: a workgroup takes one walk whole
+};
+
+__device__ __forceinline__ int units_of(const Walk& w, const Request& request) {  // of all its columns and kv heads
+  const int group = w.heads / w.kv_heads;
+  Item item;
+  if (!few_columns(request.count, group) || !make_item(w, 0, request, 0, 1 << 20, item)) return 0;
+  return (item.to - item.from + UNIT - 1) / UNIT * ((request.count * group + 15) / 16) * w.kv_heads;
+}
 
 template <typename T>
-__global__ void __launch_bounds__(WAVE) packed_join_kernel(T* out, int out_stride, const float* partial, const int* query_start, int requests, int heads, int splits) {
-  const int token = blockIdx.x, head = blockIdx.y, lane = threadIdx.x;
-  const float* mine = partial + ((size_t)token * heads + head) * splits * (D + 4);
-  const int tokens = query_start[requests], parts = min(__float_as_int(mine[D + 2]), splits);
-  if (token >= tokens || parts <= 1) return;
+__global__ void __launch_bounds__(WAVES * WAVE, 2) packed_streams_kernel(const T* q, int q_stride, T* out, int out_stride, const unsigned char* pages, Walk w, Streams streams, int whole) {
+  __shared__ __attribute__((aligned(16))) unsigned char memory[memory_of<WAVES>()];
+  __shared__ int ends[WAVES * WAVE];          // units of the requests up to a thread's
+  __shared__ Request held[WAVES * WAVE];      // the requests, if there are no more than threads
+  __shared__ int wave_sums[WAVES];
+  const int lane = threadIdx.x % WAVE, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / WAVE), group = w.heads / w.kv_heads;
+  unsigned char* ring = memory + wave * (STAGES * STAGE);
+  const auto take_walk = [&](const Item& item, int kv_head, int begin, int end, float* part) {
+    Columns<T, 1> columns;
+    walk_keys<T, 1, WAVES>(columns, q, q_stride, pages, w, item, kv_head, whole, begin, end, wave, ring);
+    bring_together<T, 1, WAVES>(columns, 0, item.columns, wave, memory, [&](int column, int d, f32x4 result, float largest, float weights) {
+      if (part) {
+        *(f32x4*)(part + column * (D + 4) + d) = result;
+        if (d == 0) *(f32x4*)(part + column * (D + 4) + D) = (f32x4){largest, weights, 0.f, 0.f};
+      } else {
+        const int flat = item.first + column, token = flat / item.group, head = kv_head * item.group + flat - token * item.group;
+        write_four(out + (size_t)(item.first_row + token) * out_stride + head * D + d, result * (1.f / weights));
+      }
+    });
+  };
+  if (streams.least == 0) {
+    const int tiles = (group + 15) / 16, request = blockIdx.x / (tiles * w.kv_heads), inside = blockIdx.x - request * (tiles * w.kv_heads);
+    const Request mine = load_request(w, request);
+    Item item;
+    if (!few_columns(mine.count, group) || !make_item(w, request, mine, inside / w.kv_heads * 16, 16, item)) return;
+    take_walk(item, inside % w.kv_heads, item.from, item.to, nullptr);
+    return;
+  }
+  // where the requests' units end: a run of requests a thread, the threads' sums added up
+  const int run = (w.requests + WAVES * WAVE - 1) / (WAVES * WAVE), first_request = threadIdx.x * run;
+  int mine = 0;
+  for (int b = first_request; b < min(first_request + run, w.requests); ++b) {
+    const Request request = load_request(w, b);
+    mine += units_of(w, request);
+    if (run == 1) held[b] = request;
+  }
+#pragma unroll
+  for (int step = 1; step < WAVE; step <<= 1) {
+    const int other = __shfl_up(mine, step);
+    if (lane >= step) mine += other;
+  }
+  if (lane == WAVE - 1) wave_sums[wave] = mine;
+  __syncthreads();
+  for (int v = 0; v < wave; ++v) mine += wave_sums[v];
+  ends[threadIdx.x] = mine;
+  __syncthreads();
+  const int total = __builtin_amdgcn_readfirstlane(ends[WAVES * WAVE - 1]), share = max(streams.least, (total + (int)gridDim.x - 1) / (int)gridDim.x);
+  const int first = min(blockIdx.x * (long)share, (long)total), last = min(first + share, total);
+  if (threadIdx.x == 0) streams.cuts[blockIdx.x].parts = 0;
+  for (int at = first; at < last;) {
+    int low = 0, high = WAVES * WAVE - 1;     // the run of requests that the unit lies in
+    while (low < high) {
+      const int middle = (low + high) / 2;
+      if (ends[middle] > at) high = middle;
+      else low = middle + 1;
+    }
+    int index = __builtin_amdgcn_readfirstlane(low) * run, inside = __builtin_amdgcn_readfirstlane(at - (low > 0 ? ends[low - 1] : 0)), all = 0;
+    Request request = {0, 0, 0};
+    for (; index < w.requests; ++index) {
+      request = run == 1 ? held[index] : load_request(w, index);
+      request.start = __builtin_amdgcn_readfirstlane(request.start);
+      request.count = __builtin_amdgcn_readfirstlane(request.count);
+      request.context = __builtin_amdgcn_readfirstlane(request.context);
+      all = units_of(w, request);
+      if (inside < all) break;
+      inside -= all;
+    }
+    if (index >= w.requests) break;
+    const int each = all / ((request.count * group + 15) / 16 * w.kv_heads);
+    const int walk = inside / each, unit = inside - walk * each, units = min(each - unit, last - at);
+    Item item;
+    // (a request of few columns has several tiles only if it is a single token: all of them walk the same keys)
+    if (make_item(w, index, request, walk / w.kv_heads * 16, 16, item)) {
+      const int begin = item.from + unit * UNIT, end = min(item.to, begin + units * UNIT), place = at == first ? 0 : 1;
+      __syncthreads();                        // (the ring's place has been read)
+      take_walk(item, walk % w.kv_heads, begin, end, units == each ? nullptr : streams.parts + ((size_t)blockIdx.x * 2 + place) * PART);
+      if (unit == 0 && units < each && threadIdx.x == 0)
+        streams.cuts[blockIdx.x] = {item.first_row, item.group, item.first, item.columns, walk % w.kv_heads, (at + each - 1) / share - (int)blockIdx.x + 1, place, 0};
+    }
+    at += units;
+  }
+}
+
+// A wave a column of a walk that was cut: its parts joined.  All of them are asked for at once.
+constexpr int JOIN_LANES = D / 4, JOINED = WAVE / JOIN_LANES;  // lanes a part, parts side by side
+
+template <typename T>
+__global__ void __launch_bounds__(WAVE) packed_join_kernel(T* out, int out_stride, Streams streams) {
+  const int workgroup = blockIdx.x, column = blockIdx.y, lane = threadIdx.x;
+  const Cut cut = streams.cuts[workgroup];
+  if (column >= cut.columns || cut.parts == 0) return;
+  const int parts = min(cut.parts, (int)gridDim.x - workgroup);
+  const float* mine = streams.parts + (size_t)workgroup * 2 * PART + column * (D + 4);
+  const auto part_of = [&](int i) { return mine + (size_t)i * 2 * PART + (i == 0 ? cut.place * PART : 0); };
   const int which = min(lane / JOIN_LANES, JOINED - 1), d = lane % JOIN_LANES * 4;
-  float reference = -INFINITY, total = 0.f;
-  if (lane < parts) {
-    reference = mine[lane * (D + 4) + D];
-    total = mine[lane * (D + 4) + D + 1];
-  }
-  const float largest = wave_max(reference), share = reference == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(reference - largest);
   f32x4 result = (f32x4){0.f, 0.f, 0.f, 0.f};
+  float weights = 0.f, largest = -INFINITY;
+  for (int base = 0; base < parts; base += WAVE) {
+    float reference = -INFINITY, total = 0.f;
+    if (base + lane < parts) {
+      const float* part = part_of(base + lane);
+      reference = part[D];
+      total = part[D + 1];
+    }
+    const float larger = fmaxf(largest, wave_max(reference)), change = largest == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(largest - larger);
+    const float share = reference == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(reference - larger);
+    largest = larger;
+    result *= change;
+    weights = weights * change + wave_sum(share * total);
 #pragma unroll 4
-  for (int i = 0; i < parts; i += JOINED) {
-    const float weight = __shfl(share, min(i + which, WAVE - 1));
-    if (i + which < parts) result += weight * *(const f32x4*)(mine + (i + which) * (D + 4) + d);
+    for (int i = base; i < min(base + WAVE, parts); i += JOINED) {
+      const float weight = __shfl(share, min(i - base + which, WAVE - 1));
+      if (i + which < parts) result += weight * *(const f32x4*)(part_of(i + which) + d);
+    }
   }
-  const float weights = wave_sum(share * total);
 #pragma unroll
   for (int other = 1; other < JOINED; ++other)
 #pragma unroll
@@ -576,43 +683,76 @@ __global__ void __launch_bounds__(WAVE) packed_join_kernel(T* out, int out_strid
       if (lane < JOIN_LANES) result[i] += far;
     }
   if (lane >= JOIN_LANES) return;
-  const float over = 1.f / weights;
-#pragma unroll
-  for (int i = 0; i < 4; ++i) out[(size_t)token * out_stride + head * D + d + i] = from_float<T>(result[i] * over);
+  const int flat = cut.first + column, token = flat / cut.group, head = cut.kv_head * cut.group + flat - token * cut.group;
+  write_four(out + (size_t)(cut.first_row + token) * out_stride + head * D + d, result * (1.f / weights));
 }
 
+// ---------------------------------------------------------------------------------------------------------------- portions
+
+constexpr int PORTION_WAVES = 4;
+
+template <typename T, int CT>
+__global__ void __launch_bounds__(PORTION_WAVES * WAVE, 2) packed_portions_kernel(const T* q, int q_stride, T* out, int out_stride, const unsigned char* pages, Walk w, int items, int whole) {
+  __shared__ __attribute__((aligned(16))) unsigned char memory[memory_of<PORTION_WAVES>()];
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / WAVE), kv_head = blockIdx.x % w.kv_heads;
+  // the longest walks begin first: a request's last columns walk most keys
+  Item item;
+  if (!find_item(w, items - 1 - blockIdx.x / w.kv_heads, 16 * CT, item)) return;
+  Columns<T, CT> columns;
+  walk_keys<T, CT, PORTION_WAVES>(columns, q, q_stride, pages, w, item, kv_head, whole, item.from, item.to, wave, memory + wave * (STAGES * STAGE));
+#pragma unroll
+  for (int ct = 0; ct < CT; ++ct) {
+    if (ct * 16 >= item.columns) break;
+    bring_together<T, CT, PORTION_WAVES>(columns, ct, min(16, item.columns - ct * 16), wave, memory, [&](int column, int d, f32x4 result, float largest, float weights) {
+      const int flat = item.first + ct * 16 + column, token = flat / item.group, head = kv_head * item.group + flat - token * item.group;
+      write_four(out + (size_t)(item.first_row + token) * out_stride + head * D + d, result * (1.f / weights));
+    });
+  }
+}
+
+// ---------------------------------------------------------------------------------------------------------------- launches
+
+constexpr int WORKGROUPS = 512;               // two a CU, as many as its LDS holds
+
 template <typename T>
-static int launch(const void* q, int q_stride, void* out, int out_stride, float* partial, const void* pages, const Walk& w, int tokens, int column_tiles, hipStream_t stream) {
-  const int group = w.heads / w.kv_heads, most = 16 * column_tiles;
-  const long items = w.single ? (long)w.requests * ((group + most - 1) / most) : ((long)tokens * group + most - 1) / most + w.requests;
-  const long blocks = items * w.kv_heads * w.splits;
-  if (items >= (1L << 31) || blocks >= (1L << 31)) return ERR_BAD_ARGUMENT;
-  const int piece = sizeof(T) == 4 ? 4 : 8, whole = (size_t)q % 16 == 0 && q_stride % piece == 0;
-  if (column_tiles == 1)
-    packed_attention_kernel<T, 1><<<(unsigned)blocks, WAVES * WAVE, 0, stream>>>((const T*)q, q_stride, (T*)out, out_stride, partial, (const unsigned char*)pages, w, (int)items, whole);
-  else
-    packed_attention_kernel<T, 2><<<(unsigned)blocks, WAVES * WAVE, 0, stream>>>((const T*)q, q_stride, (T*)out, out_stride, partial, (const unsigned char*)pages, w, (int)items, whole);
-  if (int status = LAUNCH_STATUS()) return status;
-  if (w.splits > 1) packed_join_kernel<T><<<dim3(tokens, w.heads), WAVE, 0, stream>>>((T*)out, out_stride, partial, w.query_start, w.requests, w.heads, w.splits);
+static int launch(const void* q, int q_stride, void* out, int out_stride, const void* pages, const Walk& w, const Streams& streams, int tokens, bool few, bool many, hipStream_t stream) {
+  constexpr int CT = sizeof(T) == 4 || D > 128 ? 1 : 2;
+  const int group = w.heads / w.kv_heads, piece = sizeof(T) == 4 ? 4 : 8, whole = (size_t)q % 16 == 0 && q_stride % piece == 0;
+  if (few) {
+    const long blocks = streams.least ? WORKGROUPS : (long)w.requests * ((group + 15) / 16) * w.kv_heads;
+    if (blocks >= (1L << 31)) return ERR_BAD_ARGUMENT;
+    packed_streams_kernel<T><<<(unsigned)blocks, WAVES * WAVE, 0, stream>>>((const T*)q, q_stride, (T*)out, out_stride, (const unsigned char*)pages, w, streams, whole);
+    if (int status = LAUNCH_STATUS()) return status;
+    if (streams.least) packed_join_kernel<T><<<dim3(WORKGROUPS, 16), WAVE, 0, stream>>>((T*)out, out_stride, streams);
+    if (int status = LAUNCH_STATUS()) return status;
+  }
+  if (many) {
+    const long items = ((long)tokens * group + 16 * CT - 1) / (16 * CT) + w.requests, blocks = items * w.kv_heads;
+    if (blocks >= (1L << 31)) return ERR_BAD_ARGUMENT;
+    packed_portions_kernel<T, CT><<<(unsigned)blocks, PORTION_WAVES * WAVE, 0, stream>>>((const T*)q, q_stride, (T*)out, out_stride, (const unsigned char*)pages, w, (int)items, whole);
+  }
   return LAUNCH_STATUS();
 }
 
-// q's heads are the first columns of rows of q_stride; tokens, requests: as many rows and requests as the arrays hold; single: no request brings more than one token.  A
-// workgroup walks up to `chunk` keys (a multiple of 128), at most `splits` share a run of columns: splits * chunk covers every walk.  partial, where splits > 1:
-// float32 [tokens][heads][splits][D + 4].
-extern "C" int llmserve_packed_attention(const void* q, int is_float, int q_stride, void* out, int out_stride, void* partial, const void* pages, int num_pages, const int* tables, int table_width,
-                                         const int* query_start, const int* contexts, int requests, int tokens, int heads, int kv_heads, int page_size, float scale, int window, int single, int column_tiles,
-                                         int chunk, int splits, hipStream_t stream) {
+// Floats of workspace that requests of few columns need where walks may be cut.
+extern "C" int llmserve_packed_attention_workspace() { return WORKGROUPS * (2 * PART + (int)(sizeof(Cut) / 4)); }
+
+// q's heads are the first columns of rows of q_stride; tokens, requests: as many rows and requests as the arrays hold.  kinds: 1: some requests may have few columns (a
+// single token, or no more than 16 of them in all), 2: some may have more.  least: 0: a walk over the keys of few columns is taken whole by one workgroup; else every workgroup takes at least so many
+// units of 256 keys, walks are cut, and there is a workspace.
+extern "C" int llmserve_packed_attention(const void* q, int is_float, int q_stride, void* out, int out_stride, void* workspace, const void* pages, int num_pages, const int* tables, int table_width,
+                                         const int* query_start, const int* contexts, int requests, int tokens, int heads, int kv_heads, int page_size, float scale, int window, int kinds, int least, hipStream_t stream) {
   if (tokens == 0 || requests == 0) return 0;
   if (!q || !out || !pages || !tables || !query_start || !contexts || requests < 0 || tokens < 0 || kv_heads <= 0 || heads <= 0 || heads % kv_heads || num_pages <= 0 || table_width <= 0 ||
-      !packed_fits(D, page_size) || (long)page_size * D * kv_heads >= (1L << 30) || !(scale > 0.f) || (size_t)pages % 16 || q_stride < heads * D || out_stride < heads * D || window < 0 || column_tiles < 1 || column_tiles > 2 || chunk < 128 || chunk % 128 ||
-      splits < 1 || splits > MOST_PARTS || (splits > 1 && (!partial || (size_t)partial % 16)) || heads > 65535)
+      !packed_fits(D, page_size) || (long)page_size * D * kv_heads >= (1L << 30) || !(scale > 0.f) || (size_t)pages % 16 || q_stride < heads * D || out_stride < heads * D || window < 0 ||
+      kinds < 1 || kinds > 3 || least < 0 || (least > 0 && (!workspace || (size_t)workspace % 16)))
     return ERR_BAD_ARGUMENT;
   const unsigned per_page = (unsigned)page_size / 8;
   const bool power_of_two = (per_page & (per_page - 1)) == 0;
   // (a quotient by the reciprocal is exact below 2^32 over the divisor)
   if (!power_of_two && (unsigned long)(table_width + 1) * per_page * per_page >= (1UL << 32)) return ERR_BAD_ARGUMENT;
-  const Walk w = {tables, table_width, num_pages, page_size, power_of_two ? 31 - __builtin_clz(per_page) : -1, (unsigned)(((1UL << 32) + per_page - 1) / per_page), query_start, contexts, requests, heads, kv_heads, window, single, chunk, splits, scale * LOG2_E};
-  if (is_float) return launch<float>(q, q_stride, out, out_stride, (float*)partial, pages, w, tokens, column_tiles, stream);
-  return launch<bf16_t>(q, q_stride, out, out_stride, (float*)partial, pages, w, tokens, column_tiles, stream);
+  const Walk w = {tables, table_width, num_pages, page_size, power_of_two ? 31 - __builtin_clz(per_page) : -1, (unsigned)(((1UL << 32) + per_page - 1) / per_page), query_start, contexts, requests, heads, kv_heads, window, scale * LOG2_E};
+  const Streams streams = {(float*)workspace, (Cut*)((float*)workspace + WORKGROUPS * 2 * PART), least};
+  if (is_float) return launch<float>(q, q_stride, out, out_stride, pages, w, streams, tokens, kinds & 1, kinds & 2, stream);
+  return launch<bf16_t>(q, q_stride, out, out_stride, pages, w, streams, tokens, kinds & 1, kinds & 2, stream);
 }

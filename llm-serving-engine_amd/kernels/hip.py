@@ -150,7 +150,8 @@ _SIGNATURES = {
     "llmserve_gate_columns": "piipiiiiipiip",
     "llmserve_packed_store": "piiiiiipiipp",
     "llmserve_packed_rows": "piiiipippip",
-    "llmserve_packed_attention": "piipippipippiiiiifiiiiip",
+    "llmserve_packed_attention_workspace": "",
+    "llmserve_packed_attention": "piipippipippiiiiifiiip",
     "llmserve_place_tokens": "piiipppiiiipppppipip",
 }
 _TYPES = {"p": ctypes.c_void_p, "i": ctypes.c_int, "f": ctypes.c_float}
@@ -1769,17 +1770,12 @@ class HipKernels:
         return self._lazy[key]
 
     @staticmethod
-    def _packed_shape(batch, dtype, tokens: int, requests: int, heads: int, kv_heads: int, dim: int, window: int) -> tuple[int, int, int]:
-        """(column tiles a wave, keys a workgroup walks, workgroups that share a run of columns)"""
-        group = heads // kv_heads
-        single = batch.max_query_length <= 1
-        tiles = 1 if single or dtype == torch.float32 or dim > 128 else 2
-        items = requests * -(-group // 16) if single else -(-tokens * group // (16 * tiles))
-        walk = min(batch.max_context_length, window + batch.max_query_length) + 31 if window else batch.max_context_length
-        blocks = items * kv_heads
-        chunk = max(256, -(-walk * blocks // 1024))
-        chunk = max(-(-chunk // 128) * 128, -(-walk // (64 * 128)) * 128)
-        return tiles, chunk, max(1, -(-walk // chunk))
+    def _packed_least(batch, requests: int, heads: int, kv_heads: int, window: int) -> int:
+        """Units of 256 keys that a workgroup takes at least of walks over the keys of few columns, which are cut anywhere; 0: every walk is taken whole."""
+        walk = min(batch.max_context_length, window + 31) if window else batch.max_context_length
+        if walk <= 1024 or requests * kv_heads * -(-heads // kv_heads // 16) >= 2048:
+            return 0
+        return 4
 
     def _packed_attention(self, qkv, layout, batch, cell, scale: float, window: int | None, out):
         tokens, heads, kv_heads, dim = qkv.shape[0], layout.num_heads, layout.num_kv_heads, layout.head_dim
@@ -1793,12 +1789,12 @@ class HipKernels:
         self._indices(batch.context_lengths, (requests,), "paged_attention: context lengths")
         out = self._attention_out(qkv, layout, out)
         window = int(window or 0)
-        column_tiles, chunk, splits = self._packed_shape(batch, qkv.dtype, tokens, requests, heads, kv_heads, dim, window)
-        partial = self._empty((tokens * heads * splits * (dim + 4),), torch.float32) if splits > 1 else None
-        status = self._packed_library(dim).llmserve_packed_attention(
-            _pointer(qkv), _is_float(qkv), layout.stride, _pointer(out), out.shape[1], _pointer(partial), _pointer(pages), pages.shape[0], _pointer(group.block_tables), group.width,
-            _pointer(batch.query_start), _pointer(batch.context_lengths), requests, tokens, heads, kv_heads, group.page_size, scale, window, batch.max_query_length <= 1, column_tiles,
-            chunk, splits, self._stream,
+        library, most = self._packed_library(dim), batch.max_query_length
+        least = self._packed_least(batch, requests, heads, kv_heads, window)
+        workspace = self._empty((library.llmserve_packed_attention_workspace(),), torch.float32) if least else None
+        status = library.llmserve_packed_attention(
+            _pointer(qkv), _is_float(qkv), layout.stride, _pointer(out), out.shape[1], _pointer(workspace), _pointer(pages), pages.shape[0], _pointer(group.block_tables), group.width,
+            _pointer(batch.query_start), _pointer(batch.context_lengths), requests, tokens, heads, kv_heads, group.page_size, scale, window, 1 if most <= 1 else 3, least, self._stream,
         )
         _check(status, "paged_attention over 4 bits")
         return out
