@@ -38,6 +38,7 @@ constexpr int STAGE = 4 * PIECE + 2 * D;      // of a step: four pieces, and the
 constexpr int ASKS = 4 * ((D + 127) / 128 + 1);  // loads of a step
 constexpr float AHEAD = 8.f;                  // log2 units that a score may run ahead of its column's reference before the sums are rescaled
 constexpr float LOG2_E = 1.44269504088896f;
+constexpr float NO_SCORE = -1e30f;            // the reference of a column that has seen no key: finite, so that what is masked (-infinity) stays that when it is taken off
 constexpr int CHUNKS = D / 128 + (D % 128) / 64 + (D % 64) / 32;  // runs of 128, 64 or 32 elements of a value
 __host__ __device__ constexpr int chunk_width(int c) { return c < D / 128 ? 128 : (D % 128 >= 64 && c == D / 128) ? 64 : 32; }
 __host__ __device__ constexpr int chunk_first(int c) { return c <= D / 128 ? c * 128 : D / 128 * 128 + 64; }
@@ -644,47 +645,59 @@ __global__ void __launch_bounds__(WAVES * WAVE, 2) packed_streams_kernel(const T
 }
 
 // A wave a column of a walk that was cut: its parts joined.  All of them are asked for at once.
-constexpr int JOIN_LANES = D / 4, JOINED = WAVE / JOIN_LANES;  // lanes a part, parts side by side
+constexpr int JOIN_LANES = D / 4, JOINED = WAVE / JOIN_LANES, TOGETHER = 4;  // lanes a part, parts side by side, loads under way
 
 template <typename T>
-__global__ void __launch_bounds__(WAVE) packed_join_kernel(T* out, int out_stride, Streams streams) {
-  const int workgroup = blockIdx.x, column = blockIdx.y, lane = threadIdx.x;
+__global__ void __launch_bounds__(4 * WAVE) packed_join_kernel(T* out, int out_stride, Streams streams, int part_columns) {
+  const int workgroup = blockIdx.x, lane = threadIdx.x % WAVE, which = min(lane / JOIN_LANES, JOINED - 1), d = lane % JOIN_LANES * 4;
   const Cut cut = streams.cuts[workgroup];
-  if (column >= cut.columns || cut.parts == 0) return;
+  if (cut.parts == 0) return;
   const int parts = min(cut.parts, (int)gridDim.x - workgroup);
-  const float* mine = streams.parts + (size_t)workgroup * 2 * PART + column * (D + 4);
-  const auto part_of = [&](int i) { return mine + (size_t)i * 2 * PART + (i == 0 ? cut.place * PART : 0); };
-  const int which = min(lane / JOIN_LANES, JOINED - 1), d = lane % JOIN_LANES * 4;
-  f32x4 result = (f32x4){0.f, 0.f, 0.f, 0.f};
-  float weights = 0.f, largest = -INFINITY;
-  for (int base = 0; base < parts; base += WAVE) {
-    float reference = -INFINITY, total = 0.f;
-    if (base + lane < parts) {
-      const float* part = part_of(base + lane);
-      reference = part[D];
-      total = part[D + 1];
+  const size_t part_size = (size_t)part_columns * (D + 4);
+  for (int column = blockIdx.y * 4 + threadIdx.x / WAVE; column < cut.columns; column += gridDim.y * 4) {
+    const float* mine = streams.parts + (size_t)workgroup * 2 * part_size + column * (D + 4);
+    const auto part_of = [&](int i) { return mine + (size_t)i * 2 * part_size + (i == 0 ? cut.place * part_size : 0); };
+    f32x4 result = (f32x4){0.f, 0.f, 0.f, 0.f};
+    float weights = 0.f, largest = -INFINITY;
+    for (int base = 0; base < parts; base += WAVE) {
+      float reference = -INFINITY, total = 0.f;
+      if (base + lane < parts) {
+        const float* part = part_of(base + lane);
+        reference = part[D];
+        total = part[D + 1];
+      }
+      const float larger = fmaxf(largest, wave_max(reference)), change = largest == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(largest - larger);
+      const float share = reference == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(reference - larger);
+      largest = larger;
+      result *= change;
+      weights = weights * change + wave_sum(share * total);
+      const int end = min(base + WAVE, parts);
+      for (int i = base; i < end; i += TOGETHER * JOINED) {
+        f32x4 part[TOGETHER];
+        float weight[TOGETHER];
+#pragma unroll
+        for (int k = 0; k < TOGETHER; ++k) {
+          const int at = i + k * JOINED + which;
+          part[k] = *(const f32x4*)(part_of(min(at, end - 1)) + d);
+          weight[k] = __shfl(share, min(at, end - 1) - base);
+          if (at >= end) weight[k] = 0.f;
+        }
+#pragma unroll
+        for (int k = 0; k < TOGETHER; ++k)
+          if (weight[k] != 0.f) result += weight[k] * part[k];
+      }
     }
-    const float larger = fmaxf(largest, wave_max(reference)), change = largest == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(largest - larger);
-    const float share = reference == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(reference - larger);
-    largest = larger;
-    result *= change;
-    weights = weights * change + wave_sum(share * total);
-#pragma unroll 4
-    for (int i = base; i < min(base + WAVE, parts); i += JOINED) {
-      const float weight = __shfl(share, min(i - base + which, WAVE - 1));
-      if (i + which < parts) result += weight * *(const f32x4*)(part_of(i + which) + d);
-    }
+#pragma unroll
+    for (int other = 1; other < JOINED; ++other)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float far = __shfl(result[i], min(lane + other * JOIN_LANES, WAVE - 1));
+        if (lane < JOIN_LANES) result[i] += far;
+      }
+    if (lane >= JOIN_LANES) continue;
+    const int flat = cut.first + column, token = flat / cut.group, head = cut.kv_head * cut.group + flat - token * cut.group;
+    write_four(out + (size_t)(cut.first_row + token) * out_stride + head * D + d, result * (1.f / weights));
   }
-#pragma unroll
-  for (int other = 1; other < JOINED; ++other)
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const float far = __shfl(result[i], min(lane + other * JOIN_LANES, WAVE - 1));
-      if (lane < JOIN_LANES) result[i] += far;
-    }
-  if (lane >= JOIN_LANES) return;
-  const int flat = cut.first + column, token = flat / cut.group, head = cut.kv_head * cut.group + flat - token * cut.group;
-  write_four(out + (size_t)(cut.first_row + token) * out_stride + head * D + d, result * (1.f / weights));
 }
 
 // ---------------------------------------------------------------------------------------------------------------- portions
@@ -710,49 +723,432 @@ __global__ void __launch_bounds__(PORTION_WAVES * WAVE, 2) packed_portions_kerne
   }
 }
 
+// ---------------------------------------------------------------------------------------------------------------- bfloat16 portions
+//
+// Many columns see the same keys: what bounds them is the matrix cores, and how often a key is made a bfloat16 beside them.  A workgroup takes 128 columns, 32 a
+// wave, and makes tiles of 64 keys and values bfloat16 in LDS once for its four waves, the next tile's while it multiplies with this one's:
+//   S^T = K Q^T, O^T += V^T P^T with v_mfma_f32_32x32x16_bf16, which does 1.8 PFLOP/s here where 16x16x32 does 1.1.
+// The keys of 32 are dealt to the rows of the first product so that a lane ends with the weights of two pieces of eight neighbouring keys, the slices that the
+// second product takes.  In LDS keys lie in pieces of eight elements, a piece of all 64 keys side by side, values in pieces of eight keys, a piece of all elements side by
+// side (eight neighbours exchanged by the number of their 16, so that the writers of one element write to different banks): all reads are whole lines.
+// Walks are counted in tiles and cut as those of few columns are.
+constexpr int TILE = 64, WIDE = 128;          // keys, columns
+constexpr int SHARED_THREADS = 256;
+constexpr int UNITS_ROUNDS = (2 * D + SHARED_THREADS - 1) / SHARED_THREADS;  // 16-byte units of codes a thread takes of a tile's keys, and of its values
+constexpr int WIDE_PART = WIDE * (D + 4);
+
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+
+struct Codes {                                // of a thread, of a tile
+  u32x4 keys[UNITS_ROUNDS], values[UNITS_ROUNDS];
+  unsigned key_power[UNITS_ROUNDS], value_powers[UNITS_ROUNDS];
+};
+struct Entries {                              // table entries of a thread's units
+  int key[UNITS_ROUNDS], value[UNITS_ROUNDS];
+};
+
+struct SharedTiles {
+  const unsigned char* from;                  // of the kv head
+  const int* table;
+  unsigned page_stride;
+  PackedPage page;
+};
+
+__device__ __forceinline__ unsigned page_of(const Walk& w, unsigned piece) { return w.page_shift >= 0 ? piece >> w.page_shift : __umulhi(piece, w.page_reciprocal); }
+
+// unit u of a tile's keys: key u % 64, block u / 64; of its values: half u % 2 of the eight keys of piece u / (D / 4), granule (u / 2) % (D / 8)
+__device__ __forceinline__ void load_entries(Entries& e, const Walk& w, const SharedTiles& tiles, int base) {
+#pragma unroll
+  for (int i = 0; i < UNITS_ROUNDS; ++i) {
+    const unsigned unit = i * SHARED_THREADS + threadIdx.x, key_at = page_of(w, (base + unit % TILE) / 8), value_at = page_of(w, base / 8 + unit / (D / 4));
+    e.key[i] = key_at < (unsigned)w.table_width ? tiles.table[key_at] : 0;
+    e.value[i] = value_at < (unsigned)w.table_width ? tiles.table[value_at] : 0;
+  }
+}
+__device__ __forceinline__ void load_codes(Codes& c, const Entries& e, const Walk& w, const SharedTiles& tiles, int base) {
+  const unsigned per_page = (unsigned)w.page_size / 8;
+#pragma unroll
+  for (int i = 0; i < UNITS_ROUNDS; ++i) {
+    const unsigned unit = i * SHARED_THREADS + threadIdx.x;
+    if (2 * D % SHARED_THREADS && unit >= 2 * D) continue;
+    {
+      const unsigned key = base + unit % TILE, block = unit / TILE, offset = key - page_of(w, key / 8) * per_page * 8;
+      const unsigned char* mine = tiles.from + (size_t)((unsigned)e.key[i] < (unsigned)w.num_pages ? (unsigned)e.key[i] : 0u) * tiles.page_stride;
+      c.keys[i] = *(const u32x4*)(mine + tiles.page.key_codes(offset, block * 4));
+      c.key_power[i] = mine[tiles.page.key_power(offset, block)];
+    }
+    const unsigned piece = base / 8 + unit / (D / 4), half = unit % 2, granule = unit / 2 % (D / 8), offset = (piece - page_of(w, piece) * per_page) * 8;
+    const unsigned char* mine = tiles.from + (size_t)((unsigned)e.value[i] < (unsigned)w.num_pages ? (unsigned)e.value[i] : 0u) * tiles.page_stride;
+    c.values[i] = *(const u32x4*)(mine + tiles.page.value_codes(offset + half * 4, granule));
+    c.value_powers[i] = *(const unsigned*)(mine + tiles.page.value_power(offset + half * 4, granule / 4));
+  }
+}
+
+// A thread's codes as bfloat16 into LDS: keys [D / 8][64][8], values [8][D][8].  `bad`: per block of 32 elements, the keys whose value is no number: it counts as zero, and as what
+// it is where it is seen.  Keys beyond `last`, which nobody sees, are made small numbers, whatever lies there.
+__device__ __forceinline__ void unpack_tile(const Codes& c, unsigned char* keys, unsigned char* values, unsigned long long* bad, int base, int last) {
+#pragma unroll
+  for (int i = 0; i < UNITS_ROUNDS; ++i) {
+    const unsigned unit = i * SHARED_THREADS + threadIdx.x;
+    if (2 * D % SHARED_THREADS && unit >= 2 * D) continue;
+    {
+      const unsigned key = unit % TILE, block = unit / TILE;
+      const float power = packed_power(c.key_power[i]);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const unsigned codes = c.keys[i][j];
+        *(u32x4*)(keys + ((block * 4 + j) * TILE + key) * 16) = (u32x4){unpack_pair<0>(codes, power), unpack_pair<1>(codes, power), unpack_pair<2>(codes, power), unpack_pair<3>(codes, power)};
+      }
+    }
+    const unsigned piece = unit / (D / 4), half = unit % 2, granule = unit / 2 % (D / 8);
+    const int first = piece * 8 + half * 4;   // key of the tile
+    unsigned powers = c.value_powers[i];
+    const unsigned no_number = powers & (powers >> 4) & 0x0f0f0f0fu;  // (bytes of 255: all of these eight bits)
+    if (base + first + 3 > last || (((no_number & (no_number >> 2)) & 0x03030303u) != 0u)) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const bool unseen = base + first + j > last, none = ((powers >> (8 * j)) & 255u) == PACKED_NO_NUMBER;
+        if (none && !unseen) atomicOr(&bad[granule / 4], 1ull << (first + j));
+        if (none || unseen) powers &= ~(255u << (8 * j));
+      }
+    }
+    unsigned raw[4][4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const float power = __uint_as_float(j == 3 ? powers >> 1 : powers << (23 - j * 8));
+      const unsigned codes = c.values[i][j];
+      raw[j][0] = unpack_pair<0>(codes, power);
+      raw[j][1] = unpack_pair<1>(codes, power);
+      raw[j][2] = unpack_pair<2>(codes, power);
+      raw[j][3] = unpack_pair<3>(codes, power);
+    }
+    unsigned char* to = values + (piece * D + granule * 8) * 16 + half * 8;
+    const unsigned exchange = (granule >> 1) & 7;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      *(u32x2*)(to + ((2 * e) ^ exchange) * 16) = (u32x2){__builtin_amdgcn_perm(raw[1][e], raw[0][e], 0x05040100u), __builtin_amdgcn_perm(raw[3][e], raw[2][e], 0x05040100u)};
+      *(u32x2*)(to + ((2 * e + 1) ^ exchange) * 16) = (u32x2){__builtin_amdgcn_perm(raw[1][e], raw[0][e], 0x07060302u), __builtin_amdgcn_perm(raw[3][e], raw[2][e], 0x07060302u)};
+    }
+  }
+}
+
+struct WideColumns {                          // a wave's 32
+  Eight query[D / 16];
+  int position;                               // of the lane's column's token
+  int first_position, last_position;          // of the wave's
+  float reference, total;                     // total: of the lane's half of the keys
+  f32x16 sum[D / 32];
+};
+
+// 32 keys of a tile, from `base` on (`sub` the first or the second of the tile).  edge: some column does not see some of them.
+__device__ __forceinline__ void take_half(WideColumns& columns, const unsigned char* keys, const unsigned char* values, const Walk& w, int base, int sub, bool edge) {
+  const int lane = threadIdx.x % WAVE, n = lane & 31, h = lane >> 5;
+  const int row = (n & 0x13) | ((n & 4) << 1) | ((n & 8) >> 1);  // the key that row n of the product is
+  f32x16 score;
+#pragma unroll
+  for (int i = 0; i < 16; ++i) score[i] = 0.f;
+  const unsigned char* mine = keys + (h * TILE + sub * 32 + row) * 16;
+#pragma unroll
+  for (int s = 0; s < D / 16; ++s) {
+    Eight key;
+    key.u = *(const u32x4*)(mine + 2 * s * TILE * 16);
+    score = __builtin_amdgcn_mfma_f32_32x32x16_bf16(key.v, columns.query[s].v, score, 0, 0, 0);
+  }
+  if (edge) {
+    const int highest = columns.position - base - 8 * h, lowest = w.window > 0 ? highest - w.window + 1 : -(1 << 30);
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      const int key = 16 * (i / 8) + i % 8;
+      if (key > highest || key < lowest) score[i] = -INFINITY;
+    }
+  }
+  float x[16];
+#pragma unroll
+  for (int i = 0; i < 16; ++i) x[i] = __builtin_fmaf(score[i], w.scale, -columns.reference);
+  if (__any(fmaxf(largest_of(x), largest_of(x + 8)) > AHEAD)) {
+#pragma unroll
+    for (int i = 0; i < 16; ++i) x[i] = score[i] * w.scale;
+    float largest = fmaxf(largest_of(x), largest_of(x + 8));
+    largest = fmaxf(fmaxf(largest, __shfl_xor(largest, 32)), columns.reference);
+    const float change = __builtin_amdgcn_exp2f(columns.reference - largest);
+    columns.reference = largest;
+    columns.total *= change;
+#pragma unroll
+    for (int t = 0; t < D / 32; ++t) columns.sum[t] *= change;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) x[i] -= largest;
+  }
+  const unsigned char* first = values + ((sub * 4 + h) * D + n / 8 * 8) * 16;
+#pragma unroll
+  for (int u = 0; u < 2; ++u) {
+    Eight weight;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) weight.v[j] = (bf16_t)__builtin_amdgcn_exp2f(x[8 * u + j]);
+    // the weights that are multiplied are the weights that are added up
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      union { unsigned u; packed_bf16x2 v; } pair, ones;
+      pair.u = weight.u[j];
+      ones.u = 0x3f803f80u;
+      columns.total = __builtin_amdgcn_fdot2_f32_bf16(pair.v, ones.v, columns.total, false);
+    }
+#pragma unroll
+    for (int t = 0; t < D / 32; ++t) {
+      Eight value;
+      value.u = *(const u32x4*)(first + (2 * u * D + t * 32) * 16 + ((n & 7) ^ ((t * 2 + (n >> 4)) & 7)) * 16);
+      columns.sum[t] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(value.v, weight.v, columns.sum[t], 0, 0, 0);
+    }
+  }
+}
+
+__device__ __forceinline__ int wide_units(const Walk& w, const Item& item) { return (item.to - item.from / TILE * TILE + TILE - 1) / TILE; }
+
+__global__ void __launch_bounds__(SHARED_THREADS, D <= 128 ? 2 : 1)
+packed_shared_kernel(const bf16_t* q, int q_stride, bf16_t* out, int out_stride, const unsigned char* pages, Walk w, Streams streams, int items, int whole, int whole_out) {
+  constexpr int TILE_BYTES = TILE * D * 2;
+  __shared__ __attribute__((aligned(16))) unsigned char memory[2][2 * TILE_BYTES];
+  __shared__ unsigned long long bad[3][D / 32];
+  __shared__ int item_ends[SHARED_THREADS], ends[SHARED_THREADS], wave_sums[2][SHARED_THREADS / WAVE];
+  __shared__ Request held[SHARED_THREADS];
+  const int lane = threadIdx.x % WAVE, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / WAVE), n = lane & 31, h = lane >> 5, group = w.heads / w.kv_heads;
+
+  const auto take_walk = [&](const Item& item, int kv_head, int begin, int end, float* part) {
+    SharedTiles tiles;
+    tiles.page = {D, w.page_size};
+    tiles.from = pages + (size_t)kv_head * tiles.page.bytes();
+    tiles.table = w.tables + (size_t)item.request * w.table_width;
+    tiles.page_stride = (unsigned)w.kv_heads * tiles.page.bytes();
+    Entries entries[3];
+#pragma unroll
+    for (int i = 0; i < 3; ++i) load_entries(entries[i], w, tiles, begin + i * TILE);
+    Codes now, next;
+    load_codes(now, entries[0], w, tiles, begin);
+    load_codes(next, entries[1], w, tiles, begin + TILE);
+    WideColumns columns;
+    const int first_column = wave * 32, column = min(first_column + n, item.columns - 1), flat = item.first + column, token = flat / group;
+    const int token_zero = item.first_position - item.first / group;  // the position that the request's first token of the step is at
+    columns.position = token_zero + token;
+    columns.first_position = token_zero + (item.first + min(first_column, item.columns - 1)) / group;
+    columns.last_position = first_column < item.columns ? token_zero + (item.first + min(first_column + 31, item.columns - 1)) / group : -1;
+    const bf16_t* row = q + (size_t)(item.first_row + token) * q_stride + (kv_head * group + flat - token * group) * D + h * 8;
+#pragma unroll
+    for (int s = 0; s < D / 16; ++s) {
+      if (whole) {
+        columns.query[s].u = *(const u32x4*)(row + s * 16);
+      } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) columns.query[s].v[e] = row[s * 16 + e];
+      }
+    }
+    columns.reference = NO_SCORE;
+    columns.total = 0.f;
+#pragma unroll
+    for (int t = 0; t < D / 32; ++t)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) columns.sum[t][i] = 0.f;
+    __syncthreads();                          // (a walk before this one has been read, and what it marked)
+    if (threadIdx.x < 3 * (D / 32)) (&bad[0][0])[threadIdx.x] = 0ull;
+    __syncthreads();
+    unpack_tile(now, memory[0], memory[0] + TILE_BYTES, bad[0], begin, item.last_position);
+    int turn = 0, third = 0;                  // of the tile that is multiplied: its place in LDS, that of its marks
+    for (int base = begin; base < end; base += TILE) {
+      __syncthreads();
+      now = next;
+      entries[1] = entries[2];
+      load_codes(next, entries[1], w, tiles, base + 2 * TILE);
+      load_entries(entries[2], w, tiles, base + 3 * TILE);
+      if (threadIdx.x < D / 32) bad[third == 0 ? 2 : third - 1][threadIdx.x] = 0ull;  // (those of the tile before, which are those of the next but one)
+      const unsigned char *keys = memory[turn], *values = memory[turn] + TILE_BYTES;
+#pragma unroll 1
+      for (int sub = 0; sub < 2; ++sub) {
+        const int from = base + sub * 32;
+        if (from < end && from <= columns.last_position && (w.window <= 0 || from + 31 > columns.first_position - w.window))
+          take_half(columns, keys, values, w, from, sub, from + 31 > columns.first_position || (w.window > 0 && from < columns.last_position - w.window + 1));
+      }
+#pragma unroll
+      for (int t = 0; t < D / 32; ++t) {
+        const unsigned long long marked = bad[third][t];
+        if (marked) {                         // hardly ever: values that are no number, for the columns that see them
+          const int lowest = w.window > 0 ? max(columns.position - w.window + 1 - base, 0) : 0, highest = min(columns.position - base, TILE - 1);
+          const unsigned long long seen = highest < lowest ? 0ull : ((2ull << highest) - 1ull) & ~((1ull << lowest) - 1ull);
+          if (marked & seen)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) columns.sum[t][i] = __uint_as_float(0x7fc00000u);
+        }
+      }
+      turn ^= 1;
+      third = third == 2 ? 0 : third + 1;
+      if (base + TILE < end) unpack_tile(now, memory[turn], memory[turn] + TILE_BYTES, bad[third], base + TILE, item.last_position);
+    }
+    const float weights = columns.total + __shfl_xor(columns.total, 32);
+    if (first_column + n >= item.columns) return;
+    if (part) {
+      float* to = part + (first_column + n) * (D + 4);
+#pragma unroll
+      for (int t = 0; t < D / 32; ++t)
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          *(f32x4*)(to + t * 32 + 8 * i + 4 * h) = (f32x4){columns.sum[t][4 * i], columns.sum[t][4 * i + 1], columns.sum[t][4 * i + 2], columns.sum[t][4 * i + 3]};
+      if (h == 0) *(f32x4*)(to + D) = (f32x4){columns.reference, weights, 0.f, 0.f};
+    } else {
+      const float over = 1.f / weights;
+      bf16_t* to = out + (size_t)(item.first_row + token) * out_stride + (kv_head * group + flat - token * group) * D;
+#pragma unroll
+      for (int t = 0; t < D / 32; ++t)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          union { bf16_t e[4]; u32x2 u; } four;
+#pragma unroll
+          for (int j = 0; j < 4; ++j) four.e[j] = (bf16_t)(columns.sum[t][4 * i + j] * over);
+          if (whole_out) {
+            *(u32x2*)(to + t * 32 + 8 * i + 4 * h) = four.u;
+          } else {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) to[t * 32 + 8 * i + 4 * h + j] = four.e[j];
+          }
+        }
+    }
+  };
+  // where the requests' items end, then where the items' units end (no more requests than threads; a run of items a thread)
+  const auto added_up = [&](int mine, int* sums) {
+#pragma unroll
+    for (int step = 1; step < WAVE; step <<= 1) {
+      const int other = __shfl_up(mine, step);
+      if (lane >= step) mine += other;
+    }
+    if (lane == WAVE - 1) sums[wave] = mine;
+    __syncthreads();
+    for (int v = 0; v < wave; ++v) mine += sums[v];
+    return mine;
+  };
+  int all_items = 0, run = 0, share = 1, first = 0, last = 1;
+  const auto item_at = [&](int index, Item& item) {
+    int low = 0, high = SHARED_THREADS - 1;
+    while (low < high) {
+      const int middle = (low + high) / 2;
+      if (item_ends[middle] > index) high = middle;
+      else low = middle + 1;
+    }
+    return make_item(w, low, held[low], (index - (low > 0 ? item_ends[low - 1] : 0)) * WIDE, WIDE, item);
+  };
+  if (streams.least > 0) {
+    int count = 0;
+    if ((int)threadIdx.x < w.requests) {
+      held[threadIdx.x] = load_request(w, threadIdx.x);
+      const int tokens = held[threadIdx.x].count;
+      count = few_columns(tokens, group) ? 0 : (max(tokens, 0) * group + WIDE - 1) / WIDE;
+    }
+    item_ends[threadIdx.x] = added_up(count, wave_sums[0]);
+    __syncthreads();
+    all_items = __builtin_amdgcn_readfirstlane(item_ends[SHARED_THREADS - 1]);
+    run = (all_items + SHARED_THREADS - 1) / SHARED_THREADS;
+    int units = 0;
+    for (int i = threadIdx.x * run; i < min((int)(threadIdx.x + 1) * run, all_items); ++i) {
+      Item item;
+      if (item_at(i, item)) units += wide_units(w, item) * w.kv_heads;
+    }
+    ends[threadIdx.x] = added_up(units, wave_sums[1]);
+    __syncthreads();
+    const int total = __builtin_amdgcn_readfirstlane(ends[SHARED_THREADS - 1]);
+    share = max(streams.least, (total + (int)gridDim.x - 1) / (int)gridDim.x);
+    first = min(blockIdx.x * (long)share, (long)total);
+    last = min(first + share, total);
+    if (threadIdx.x == 0) streams.cuts[blockIdx.x].parts = 0;
+  }
+  for (int at = first; at < last;) {
+    Item item;
+    int kv_head, begin, taken = 1, each = 1, unit = 0, place = 0;
+    if (streams.least == 0) {                 // a walk whole; the longest begin first: a request's last columns walk most keys
+      if (!find_item(w, items - 1 - blockIdx.x / w.kv_heads, WIDE, item)) return;
+      kv_head = blockIdx.x % w.kv_heads;
+      begin = item.from / TILE * TILE;
+    } else {
+      int low = 0, high = SHARED_THREADS - 1;
+      while (low < high) {
+        const int middle = (low + high) / 2;
+        if (ends[middle] > at) high = middle;
+        else low = middle + 1;
+      }
+      int index = __builtin_amdgcn_readfirstlane(low) * run, inside = __builtin_amdgcn_readfirstlane(at - (low > 0 ? ends[low - 1] : 0));
+      for (; index < all_items; ++index) {
+        each = __builtin_amdgcn_readfirstlane(item_at(index, item) ? wide_units(w, item) : 0);
+        if (inside < each * w.kv_heads) break;
+        inside -= each * w.kv_heads;
+      }
+      if (index >= all_items) break;
+      kv_head = inside / each;
+      unit = inside - kv_head * each;
+      taken = min(each - unit, last - at);
+      place = at == first ? 0 : 1;
+      begin = __builtin_amdgcn_readfirstlane(item.from) / TILE * TILE + unit * TILE;
+    }
+    item.request = __builtin_amdgcn_readfirstlane(item.request);
+    item.first_row = __builtin_amdgcn_readfirstlane(item.first_row);
+    item.first = __builtin_amdgcn_readfirstlane(item.first);
+    item.columns = __builtin_amdgcn_readfirstlane(item.columns);
+    item.first_position = __builtin_amdgcn_readfirstlane(item.first_position);
+    item.last_position = __builtin_amdgcn_readfirstlane(item.last_position);
+    item.to = __builtin_amdgcn_readfirstlane(item.to);
+    const bool cut = taken < each;
+    take_walk(item, kv_head, begin, streams.least == 0 || unit + taken == each ? item.to : begin + taken * TILE, cut ? streams.parts + ((size_t)blockIdx.x * 2 + place) * WIDE_PART : nullptr);
+    if (cut && unit == 0 && threadIdx.x == 0)
+      streams.cuts[blockIdx.x] = {item.first_row, group, item.first, item.columns, kv_head, (at + each - 1) / share - (int)blockIdx.x + 1, place, 0};
+    at += taken;
+  }
+}
+
 // ---------------------------------------------------------------------------------------------------------------- launches
 
-constexpr int WORKGROUPS = 512;               // two a CU, as many as its LDS holds
+constexpr int WORKGROUPS = 512;               // two a CU, as many as its LDS holds (one where heads are wider than 128)
 
 template <typename T>
-static int launch(const void* q, int q_stride, void* out, int out_stride, const void* pages, const Walk& w, const Streams& streams, int tokens, bool few, bool many, hipStream_t stream) {
-  constexpr int CT = sizeof(T) == 4 || D > 128 ? 1 : 2;
-  const int group = w.heads / w.kv_heads, piece = sizeof(T) == 4 ? 4 : 8, whole = (size_t)q % 16 == 0 && q_stride % piece == 0;
-  if (few) {
-    const long blocks = streams.least ? WORKGROUPS : (long)w.requests * ((group + 15) / 16) * w.kv_heads;
+static int launch(const void* q, int q_stride, void* out, int out_stride, const void* pages, const Walk& w, const Streams& few, const Streams& many, int tokens, int kinds, hipStream_t stream) {
+  const int group = w.heads / w.kv_heads, piece = sizeof(T) == 4 ? 4 : 8, whole = (size_t)q % 16 == 0 && q_stride % piece == 0, whole_out = (size_t)out % 8 == 0 && out_stride % 4 == 0;
+  if (kinds & 1) {
+    const long blocks = few.least ? WORKGROUPS : (long)w.requests * ((group + 15) / 16) * w.kv_heads;
     if (blocks >= (1L << 31)) return ERR_BAD_ARGUMENT;
-    packed_streams_kernel<T><<<(unsigned)blocks, WAVES * WAVE, 0, stream>>>((const T*)q, q_stride, (T*)out, out_stride, (const unsigned char*)pages, w, streams, whole);
+    packed_streams_kernel<T><<<(unsigned)blocks, WAVES * WAVE, 0, stream>>>((const T*)q, q_stride, (T*)out, out_stride, (const unsigned char*)pages, w, few, whole);
     if (int status = LAUNCH_STATUS()) return status;
-    if (streams.least) packed_join_kernel<T><<<dim3(WORKGROUPS, 16), WAVE, 0, stream>>>((T*)out, out_stride, streams);
+    if (few.least) packed_join_kernel<T><<<dim3(WORKGROUPS, 4), 4 * WAVE, 0, stream>>>((T*)out, out_stride, few, 16);
     if (int status = LAUNCH_STATUS()) return status;
   }
-  if (many) {
-    const long items = ((long)tokens * group + 16 * CT - 1) / (16 * CT) + w.requests, blocks = items * w.kv_heads;
+  if (!(kinds & 2)) return 0;
+  if constexpr (sizeof(T) == 4) {
+    const long items = ((long)tokens * group + 15) / 16 + w.requests, blocks = items * w.kv_heads;
     if (blocks >= (1L << 31)) return ERR_BAD_ARGUMENT;
-    packed_portions_kernel<T, CT><<<(unsigned)blocks, PORTION_WAVES * WAVE, 0, stream>>>((const T*)q, q_stride, (T*)out, out_stride, (const unsigned char*)pages, w, (int)items, whole);
+    packed_portions_kernel<T, 1><<<(unsigned)blocks, PORTION_WAVES * WAVE, 0, stream>>>((const T*)q, q_stride, (T*)out, out_stride, (const unsigned char*)pages, w, (int)items, whole);
+  } else {
+    const long items = ((long)tokens * group + WIDE - 1) / WIDE + w.requests, blocks = many.least ? WORKGROUPS : items * w.kv_heads;
+    if (blocks >= (1L << 31)) return ERR_BAD_ARGUMENT;
+    packed_shared_kernel<<<(unsigned)blocks, SHARED_THREADS, 0, stream>>>((const T*)q, q_stride, (T*)out, out_stride, (const unsigned char*)pages, w, many, (int)items, whole, whole_out);
+    if (int status = LAUNCH_STATUS()) return status;
+    if (many.least) packed_join_kernel<T><<<dim3(WORKGROUPS, 8), 4 * WAVE, 0, stream>>>((T*)out, out_stride, many, WIDE);
   }
   return LAUNCH_STATUS();
 }
 
-// Floats of workspace that requests of few columns need where walks may be cut.
-extern "C" int llmserve_packed_attention_workspace() { return WORKGROUPS * (2 * PART + (int)(sizeof(Cut) / 4)); }
+// Floats of workspace that requests of few columns, or of many (bfloat16), need where walks may be cut.
+extern "C" int llmserve_packed_attention_workspace(int many) { return WORKGROUPS * (2 * (many ? WIDE_PART : PART) + (int)(sizeof(Cut) / 4)); }
 
 // q's heads are the first columns of rows of q_stride; tokens, requests: as many rows and requests as the arrays hold.  kinds: 1: some requests may have few columns (a
-// single token, or no more than 16 of them in all), 2: some may have more.  least: 0: a walk over the keys of few columns is taken whole by one workgroup; else every workgroup takes at least so many
-// units of 256 keys, walks are cut, and there is a workspace.
-extern "C" int llmserve_packed_attention(const void* q, int is_float, int q_stride, void* out, int out_stride, void* workspace, const void* pages, int num_pages, const int* tables, int table_width,
-                                         const int* query_start, const int* contexts, int requests, int tokens, int heads, int kv_heads, int page_size, float scale, int window, int kinds, int least, hipStream_t stream) {
+// single token, or no more than 16 of them in all), 2: some may have more.  few_least, many_least: 0: a walk over the keys of few (many) columns is taken whole by one workgroup; else every
+// workgroup takes at least so many units of 256 (64) keys, walks are cut, and there is a workspace.  Those of many columns are cut in bfloat16 and for up to 256 requests alone.
+extern "C" int llmserve_packed_attention(const void* q, int is_float, int q_stride, void* out, int out_stride, void* few_workspace, void* many_workspace, const void* pages, int num_pages, const int* tables,
+                                         int table_width, const int* query_start, const int* contexts, int requests, int tokens, int heads, int kv_heads, int page_size, float scale, int window, int kinds,
+                                         int few_least, int many_least, hipStream_t stream) {
   if (tokens == 0 || requests == 0) return 0;
   if (!q || !out || !pages || !tables || !query_start || !contexts || requests < 0 || tokens < 0 || kv_heads <= 0 || heads <= 0 || heads % kv_heads || num_pages <= 0 || table_width <= 0 ||
       !packed_fits(D, page_size) || (long)page_size * D * kv_heads >= (1L << 30) || !(scale > 0.f) || (size_t)pages % 16 || q_stride < heads * D || out_stride < heads * D || window < 0 ||
-      kinds < 1 || kinds > 3 || least < 0 || (least > 0 && (!workspace || (size_t)workspace % 16)))
+      kinds < 1 || kinds > 3 || few_least < 0 || (few_least > 0 && (!few_workspace || (size_t)few_workspace % 16)) || many_least < 0 ||
+      (many_least > 0 && (!many_workspace || (size_t)many_workspace % 16 || is_float || requests > SHARED_THREADS)))
     return ERR_BAD_ARGUMENT;
   const unsigned per_page = (unsigned)page_size / 8;
   const bool power_of_two = (per_page & (per_page - 1)) == 0;
-  // (a quotient by the reciprocal is exact below 2^32 over the divisor)
-  if (!power_of_two && (unsigned long)(table_width + 1) * per_page * per_page >= (1UL << 32)) return ERR_BAD_ARGUMENT;
+  // (a quotient by the reciprocal is exact below 2^32 over the divisor; pieces up to a few tiles beyond the tables are asked for)
+  if (!power_of_two && ((unsigned long)table_width * per_page + 64) * per_page >= (1UL << 32)) return ERR_BAD_ARGUMENT;
   const Walk w = {tables, table_width, num_pages, page_size, power_of_two ? 31 - __builtin_clz(per_page) : -1, (unsigned)(((1UL << 32) + per_page - 1) / per_page), query_start, contexts, requests, heads, kv_heads, window, scale * LOG2_E};
-  const Streams streams = {(float*)workspace, (Cut*)((float*)workspace + WORKGROUPS * 2 * PART), least};
-  if (is_float) return launch<float>(q, q_stride, out, out_stride, pages, w, streams, tokens, kinds & 1, kinds & 2, stream);
-  return launch<bf16_t>(q, q_stride, out, out_stride, pages, w, streams, tokens, kinds & 1, kinds & 2, stream);
+  const Streams few = {(float*)few_workspace, (Cut*)((float*)few_workspace + WORKGROUPS * 2 * PART), few_least};
+  const Streams many = {(float*)many_workspace, (Cut*)((float*)many_workspace + WORKGROUPS * 2 * WIDE_PART), many_least};
+  if (is_float) return launch<float>(q, q_stride, out, out_stride, pages, w, few, many, tokens, kinds, stream);
+  return launch<bf16_t>(q, q_stride, out, out_stride, pages, w, few, many, tokens, kinds, stream);
 }

@@ -150,8 +150,8 @@ _SIGNATURES = {
     "llmserve_gate_columns": "piipiiiiipiip",
     "llmserve_packed_store": "piiiiiipiipp",
     "llmserve_packed_rows": "piiiipippip",
-    "llmserve_packed_attention_workspace": "",
-    "llmserve_packed_attention": "piipippipippiiiiifiiip",
+    "llmserve_packed_attention_workspace": "i",
+    "llmserve_packed_attention": "piipipppipippiiiiifiiiip",
     "llmserve_place_tokens": "piiipppiiiipppppipip",
 }
 _TYPES = {"p": ctypes.c_void_p, "i": ctypes.c_int, "f": ctypes.c_float}
@@ -1770,12 +1770,17 @@ class HipKernels:
         return self._lazy[key]
 
     @staticmethod
-    def _packed_least(batch, requests: int, heads: int, kv_heads: int, window: int) -> int:
-        """Units of 256 keys that a workgroup takes at least of walks over the keys of few columns, which are cut anywhere; 0: every walk is taken whole."""
+    def _packed_least(batch, dtype, tokens: int, requests: int, heads: int, kv_heads: int, window: int) -> tuple[int, int]:
+        """(units of 256 keys that a workgroup takes at least of walks over the keys of few columns, units of 64 keys of those of many): walks are cut anywhere.  0: every
+        walk is taken whole."""
+        group = heads // kv_heads
         walk = min(batch.max_context_length, window + 31) if window else batch.max_context_length
-        if walk <= 1024 or requests * kv_heads * -(-heads // kv_heads // 16) >= 2048:
-            return 0
-        return 4
+        pairs = requests * kv_heads * -(-group // 16)
+        few = 0 if walk <= 1024 or 22 * walk <= 50000 + 3 * pairs * walk // 10 else 4
+        most = batch.max_query_length
+        items = kv_heads * -(-tokens * group // 128)
+        many = 0 if most <= 1 or dtype == torch.float32 or requests > 256 or items >= 1024 or walk <= 512 else 8
+        return few, many
 
     def _packed_attention(self, qkv, layout, batch, cell, scale: float, window: int | None, out):
         tokens, heads, kv_heads, dim = qkv.shape[0], layout.num_heads, layout.num_kv_heads, layout.head_dim
@@ -1790,11 +1795,12 @@ class HipKernels:
         out = self._attention_out(qkv, layout, out)
         window = int(window or 0)
         library, most = self._packed_library(dim), batch.max_query_length
-        least = self._packed_least(batch, requests, heads, kv_heads, window)
-        workspace = self._empty((library.llmserve_packed_attention_workspace(),), torch.float32) if least else None
+        few, many = self._packed_least(batch, qkv.dtype, tokens, requests, heads, kv_heads, window)
+        spaces = [self._empty((library.llmserve_packed_attention_workspace(kind),), torch.float32) if least else None for kind, least in ((0, few), (1, many))]
         status = library.llmserve_packed_attention(
-            _pointer(qkv), _is_float(qkv), layout.stride, _pointer(out), out.shape[1], _pointer(workspace), _pointer(pages), pages.shape[0], _pointer(group.block_tables), group.width,
-            _pointer(batch.query_start), _pointer(batch.context_lengths), requests, tokens, heads, kv_heads, group.page_size, scale, window, 1 if most <= 1 else 3, least, self._stream,
+            _pointer(qkv), _is_float(qkv), layout.stride, _pointer(out), out.shape[1], _pointer(spaces[0]), _pointer(spaces[1]), _pointer(pages), pages.shape[0],
+            _pointer(group.block_tables), group.width, _pointer(batch.query_start), _pointer(batch.context_lengths), requests, tokens, heads, kv_heads, group.page_size, scale, window,
+            1 if most <= 1 else 3, few, many, self._stream,
         )
         _check(status, "paged_attention over 4 bits")
         return out
