@@ -38,7 +38,6 @@ constexpr int STAGE = 4 * PIECE + 2 * D;      // of a step: four pieces, and the
 constexpr int ASKS = 4 * ((D + 127) / 128 + 1);  // loads of a step
 constexpr float AHEAD = 8.f;                  // log2 units that a score may run ahead of its column's reference before the sums are rescaled
 constexpr float LOG2_E = 1.44269504088896f;
-constexpr float NO_SCORE = -1e30f;            // the reference of a column that has seen no key: finite, so that what is masked (-infinity) stays that when it is taken off
 constexpr int CHUNKS = D / 128 + (D % 128) / 64 + (D % 64) / 32;  // runs of 128, 64 or 32 elements of a value
 __host__ __device__ constexpr int chunk_width(int c) { return c < D / 128 ? 128 : (D % 128 >= 64 && c == D / 128) ? 64 : 32; }
 __host__ __device__ constexpr int chunk_first(int c) { return c <= D / 128 ? c * 128 : D / 128 * 128 + 64; }
@@ -263,7 +262,7 @@ __device__ __forceinline__ f32x4 multiply(const Eight& a, const Eight& b, f32x4 
 __device__ __forceinline__ float largest_of(const float* x) { return fmaxf(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])), fmaxf(fmaxf(x[4], x[5]), fmaxf(x[6], x[7]))); }
 
 // One step of 32 keys from `base` on.  EDGE: some column does not see some of them.
-template <typename T, int CT, bool EDGE>
+template <bool EDGE, typename T, int CT>
 __device__ __forceinline__ void take_step(Columns<T, CT>& columns, const Step& now, const Walk& w, const Item& item, int base) {
   constexpr int TERMS = Columns<T, CT>::TERMS;
   const int lane = threadIdx.x % WAVE, r = lane & 15, g = lane >> 4;
@@ -435,9 +434,19 @@ __device__ __forceinline__ void load_queries(Columns<T, CT>& columns, const T* q
   }
 }
 
+// What a wave holds of its queries stays in registers from here on.
+template <typename T, int CT> __device__ __forceinline__ void settle(Columns<T, CT>& columns) {
+#pragma unroll
+  for (int ct = 0; ct < CT; ++ct)
+#pragma unroll
+    for (int k = 0; k < Columns<T, CT>::TERMS; ++k)
+#pragma unroll
+      for (int s = 0; s < SLICES; ++s) asm volatile("" : "+v"(columns.query[ct][k][s].u));
+}
+
 // A wave's steps of the keys begin .. end (begin a multiple of 32): every W-th from its own on.  ring: STAGES stages of LDS that are its own.
-template <typename T, int CT, int W>
-__device__ __forceinline__ void walk_keys(Columns<T, CT>& columns, const T* q, int q_stride, const unsigned char* pages, const Walk& w, const Item& item, int kv_head, bool whole, int begin, int end, int wave, unsigned char* ring) {
+template <typename T, typename Taken, int W, typename Cols>
+__device__ __forceinline__ void walk_keys(Cols& columns, const T* q, int q_stride, const unsigned char* pages, const Walk& w, const Item& item, int kv_head, bool whole, int begin, int end, int wave, unsigned char* ring) {
   const unsigned char* from = pages + (size_t)kv_head * (w.page_size * (D + D / 16));
   Scalar* table = (Scalar*)w.tables + (size_t)item.request * w.table_width;
   const LaneParts lane_parts = parts_of_lane(w.page_size);
@@ -453,14 +462,9 @@ __device__ __forceinline__ void walk_keys(Columns<T, CT>& columns, const T* q, i
   if (asked < end) find_place(place, w, table, asked);
   load_queries(columns, q, q_stride, item, kv_head, whole);
   // (the queries have come, and with them what was asked for before: from here on the loads that are counted are those of steps)
-#pragma unroll
-  for (int ct = 0; ct < CT; ++ct)
-#pragma unroll
-    for (int k = 0; k < Columns<T, CT>::TERMS; ++k)
-#pragma unroll
-      for (int s = 0; s < SLICES; ++s) asm volatile("" : "+v"(columns.query[ct][k][s].u));
+  settle(columns);
   wait_for_asked<0>();
-  const auto next_step = [&](Step& now) {
+  const auto next_step = [&](Taken& now) {
     if (base + (STAGES - 1) * W * KEYS < end) wait_for_asked<(STAGES - 1) * ASKS>();
     else wait_for_asked<0>();
     read_step(now, ring + stage * STAGE);
@@ -475,39 +479,20 @@ __device__ __forceinline__ void walk_keys(Columns<T, CT>& columns, const T* q, i
   const int whole_from = w.window > 0 ? item.last_position - w.window + 1 : 0, whole_to = min(end, item.first_position - KEYS + 2);
   for (; base < end; base += W * KEYS) {
     for (; base >= whole_from && base < whole_to; base += W * KEYS) {
-      Step now;
+      Taken now;
       next_step(now);
-      take_step<T, CT, false>(columns, now, w, item, base);
+      take_step<false>(columns, now, w, item, base);
     }
     if (base >= end) break;
-    Step now;
+    Taken now;
     next_step(now);
-    take_step<T, CT, true>(columns, now, w, item, base);
+    take_step<true>(columns, now, w, item, base);
   }
 }
 
-// The sums of W waves over a tile of 16 columns, brought together through LDS: take(column, d, four sums from element d on, the weights' reference, their sum).
-// memory: W * 16 * (D + 6) floats, free when all waves have come here.
-template <typename T, int CT, int W, typename Take>
-__device__ __forceinline__ void bring_together(const Columns<T, CT>& columns, int ct, int count, int wave, unsigned char* memory, Take take) {
-  float (*results)[16][D + 4] = (float (*)[16][D + 4])memory;
-  float (*sums)[16][2] = (float (*)[16][2])(memory + W * 16 * (D + 4) * 4);
-  const int lane = threadIdx.x % WAVE, r = lane & 15, g = lane >> 4;
-  __syncthreads();
-  if (g == 0) {
-    sums[wave][r][0] = columns.reference[ct];
-    sums[wave][r][1] = columns.total[ct][0];
-  }
-#pragma unroll
-  for (int c = 0; c < CHUNKS; ++c) {
-    const int each = chunk_width(c) / 16;  // neighbouring elements of a row of the tiles
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-#pragma unroll
-      for (int e = 0; e < 8; ++e)
-        if (e < each) results[wave][r][chunk_first(c) + (4 * g + i) * each + e] = columns.sum[ct][chunk_first(c) / 16 + e][i];
-  }
-  __syncthreads();
+// What W waves have of up to 16 columns, joined: take(column, d, four sums from element d on, the weights' reference, their sum).
+template <int W, typename Take>
+__device__ __forceinline__ void join_waves(const float (*results)[16][D + 4], const float (*sums)[16][2], int count, Take take) {
   for (int at = threadIdx.x; at < count * (D / 4); at += W * WAVE) {
     const int column = at / (D / 4), d = (at - column * (D / 4)) * 4;
     float largest = sums[0][column][0];
@@ -523,6 +508,30 @@ __device__ __forceinline__ void bring_together(const Columns<T, CT>& columns, in
     }
     take(column, d, result, largest, weights);
   }
+}
+
+// The sums of W waves, brought together through LDS.  memory: W * 16 * (D + 6) floats, free when all waves have come here.
+template <int W, typename T, typename Take>
+__device__ __forceinline__ void bring_together(const Columns<T, 1>& columns, int count, int wave, unsigned char* memory, Take take) {
+  float (*results)[16][D + 4] = (float (*)[16][D + 4])memory;
+  float (*sums)[16][2] = (float (*)[16][2])(memory + W * 16 * (D + 4) * 4);
+  const int lane = threadIdx.x % WAVE, r = lane & 15, g = lane >> 4;
+  __syncthreads();
+  if (g == 0) {
+    sums[wave][r][0] = columns.reference[0];
+    sums[wave][r][1] = columns.total[0][0];
+  }
+#pragma unroll
+  for (int c = 0; c < CHUNKS; ++c) {
+    const int each = chunk_width(c) / 16;  // neighbouring elements of a row of the tiles
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+        if (e < each) results[wave][r][chunk_first(c) + (4 * g + i) * each + e] = columns.sum[0][chunk_first(c) / 16 + e][i];
+  }
+  __syncthreads();
+  join_waves<W>(results, sums, count, take);
 }
 
 template <typename T> __device__ __forceinline__ void write_four(T* to, f32x4 x) {
@@ -570,8 +579,8 @@ __global__ void __launch_bounds__(WAVES * WAVE, 2) packed_streams_kernel(const T
   unsigned char* ring = memory + wave * (STAGES * STAGE);
   const auto take_walk = [&](const Item& item, int kv_head, int begin, int end, float* part) {
     Columns<T, 1> columns;
-    walk_keys<T, 1, WAVES>(columns, q, q_stride, pages, w, item, kv_head, whole, begin, end, wave, ring);
-    bring_together<T, 1, WAVES>(columns, 0, item.columns, wave, memory, [&](int column, int d, f32x4 result, float largest, float weights) {
+    walk_keys<T, Step, WAVES>(columns, q, q_stride, pages, w, item, kv_head, whole, begin, end, wave, ring);
+    bring_together<WAVES>(columns, item.columns, wave, memory, [&](int column, int d, f32x4 result, float largest, float weights) {
       if (part) {
         *(f32x4*)(part + column * (D + 4) + d) = result;
         if (d == 0) *(f32x4*)(part + column * (D + 4) + D) = (f32x4){largest, weights, 0.f, 0.f};
@@ -701,184 +710,111 @@ __global__ void __launch_bounds__(4 * WAVE) packed_join_kernel(T* out, int out_s
 }
 
 // ---------------------------------------------------------------------------------------------------------------- portions
-
-constexpr int PORTION_WAVES = 4;
-
-template <typename T, int CT>
-__global__ void __launch_bounds__(PORTION_WAVES * WAVE, 2) packed_portions_kernel(const T* q, int q_stride, T* out, int out_stride, const unsigned char* pages, Walk w, int items, int whole) {
-  __shared__ __attribute__((aligned(16))) unsigned char memory[memory_of<PORTION_WAVES>()];
-  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / WAVE), kv_head = blockIdx.x % w.kv_heads;
-  // the longest walks begin first: a request's last columns walk most keys
-  Item item;
-  if (!find_item(w, items - 1 - blockIdx.x / w.kv_heads, 16 * CT, item)) return;
-  Columns<T, CT> columns;
-  walk_keys<T, CT, PORTION_WAVES>(columns, q, q_stride, pages, w, item, kv_head, whole, item.from, item.to, wave, memory + wave * (STAGES * STAGE));
-#pragma unroll
-  for (int ct = 0; ct < CT; ++ct) {
-    if (ct * 16 >= item.columns) break;
-    bring_together<T, CT, PORTION_WAVES>(columns, ct, min(16, item.columns - ct * 16), wave, memory, [&](int column, int d, f32x4 result, float largest, float weights) {
-      const int flat = item.first + ct * 16 + column, token = flat / item.group, head = kv_head * item.group + flat - token * item.group;
-      write_four(out + (size_t)(item.first_row + token) * out_stride + head * D + d, result * (1.f / weights));
-    });
-  }
-}
-
-// ---------------------------------------------------------------------------------------------------------------- bfloat16 portions
 //
-// Many columns see the same keys: what bounds them is the matrix cores, and how often a key is made a bfloat16 beside them.  A workgroup takes 128 columns, 32 a
-// wave, and makes tiles of 64 keys and values bfloat16 in LDS once for its four waves, the next tile's while it multiplies with this one's:
-//   S^T = K Q^T, O^T += V^T P^T with v_mfma_f32_32x32x16_bf16, which does 1.8 PFLOP/s here where 16x16x32 does 1.1.
-// The keys of 32 are dealt to the rows of the first product so that a lane ends with the weights of two pieces of eight neighbouring keys, the slices that the
-// second product takes.  In LDS keys lie in pieces of eight elements, a piece of all 64 keys side by side, values in pieces of eight keys, a piece of all elements side by
-// side (eight neighbours exchanged by the number of their 16, so that the writers of one element write to different banks): all reads are whole lines.
-// Walks are counted in tiles and cut as those of few columns are.
-constexpr int TILE = 64, WIDE = 128;          // keys, columns
-constexpr int SHARED_THREADS = 256;
-constexpr int UNITS_ROUNDS = (2 * D + SHARED_THREADS - 1) / SHARED_THREADS;  // 16-byte units of codes a thread takes of a tile's keys, and of its values
-constexpr int WIDE_PART = WIDE * (D + 4);
+// Many columns see the same keys: the matrix cores and the instructions that make codes bfloat16 bound these.  In bfloat16, at heads of a multiple of 64, a wave
+// takes 32 columns with v_mfma_f32_32x32x16_bf16, which does 1.8 PFLOP/s here where 16x16x32 does 1.1; a step's codes are made bfloat16 once for them.  Everything else is as
+// above: a lane takes D / 2 neighbouring elements of a key, keys are dealt to rows so that a lane ends with the weights of two pieces of eight neighbouring keys, and of the values it takes
+// D / 32 neighbouring elements of those keys.  (Tiles made bfloat16 once for four such waves, in LDS, take as many instructions a wave, the barriers and the way through LDS counted:
+// 2,048 tokens behind 30,000 keys at 12/2 heads took 480 us so.)
+constexpr int PORTION_WAVES = 4, PORTION_THREADS = PORTION_WAVES * WAVE;
+constexpr int PORTION_UNIT = PORTION_WAVES * KEYS;  // keys
+constexpr int BEGINNING = 4;                  // units that a walk's beginning and end take as long as
 
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 
-struct Codes {                                // of a thread, of a tile
-  u32x4 keys[UNITS_ROUNDS], values[UNITS_ROUNDS];
-  unsigned key_power[UNITS_ROUNDS], value_powers[UNITS_ROUNDS];
+constexpr int HALF_BLOCKS = D >= 64 ? D / 64 : 1;
+
+struct WideStep {
+  u32x4 keys[HALF_BLOCKS];                    // a block of 32 elements each
+  unsigned key_powers[HALF_BLOCKS];
+  u32x4 values[2][CHUNKS][2];                 // of pieces h and 2 + h
+  u32x2 value_powers[2][CHUNKS];
 };
-struct Entries {                              // table entries of a thread's units
-  int key[UNITS_ROUNDS], value[UNITS_ROUNDS];
-};
-
-struct SharedTiles {
-  const unsigned char* from;                  // of the kv head
-  const int* table;
-  unsigned page_stride;
-  PackedPage page;
-};
-
-__device__ __forceinline__ unsigned page_of(const Walk& w, unsigned piece) { return w.page_shift >= 0 ? piece >> w.page_shift : __umulhi(piece, w.page_reciprocal); }
-
-// unit u of a tile's keys: key u % 64, block u / 64; of its values: half u % 2 of the eight keys of piece u / (D / 4), granule (u / 2) % (D / 8)
-__device__ __forceinline__ void load_entries(Entries& e, const Walk& w, const SharedTiles& tiles, int base) {
-#pragma unroll
-  for (int i = 0; i < UNITS_ROUNDS; ++i) {
-    const unsigned unit = i * SHARED_THREADS + threadIdx.x, key_at = page_of(w, (base + unit % TILE) / 8), value_at = page_of(w, base / 8 + unit / (D / 4));
-    e.key[i] = key_at < (unsigned)w.table_width ? tiles.table[key_at] : 0;
-    e.value[i] = value_at < (unsigned)w.table_width ? tiles.table[value_at] : 0;
-  }
-}
-__device__ __forceinline__ void load_codes(Codes& c, const Entries& e, const Walk& w, const SharedTiles& tiles, int base) {
-  const unsigned per_page = (unsigned)w.page_size / 8;
-#pragma unroll
-  for (int i = 0; i < UNITS_ROUNDS; ++i) {
-    const unsigned unit = i * SHARED_THREADS + threadIdx.x;
-    if (2 * D % SHARED_THREADS && unit >= 2 * D) continue;
-    {
-      const unsigned key = base + unit % TILE, block = unit / TILE, offset = key - page_of(w, key / 8) * per_page * 8;
-      const unsigned char* mine = tiles.from + (size_t)((unsigned)e.key[i] < (unsigned)w.num_pages ? (unsigned)e.key[i] : 0u) * tiles.page_stride;
-      c.keys[i] = *(const u32x4*)(mine + tiles.page.key_codes(offset, block * 4));
-      c.key_power[i] = mine[tiles.page.key_power(offset, block)];
-    }
-    const unsigned piece = base / 8 + unit / (D / 4), half = unit % 2, granule = unit / 2 % (D / 8), offset = (piece - page_of(w, piece) * per_page) * 8;
-    const unsigned char* mine = tiles.from + (size_t)((unsigned)e.value[i] < (unsigned)w.num_pages ? (unsigned)e.value[i] : 0u) * tiles.page_stride;
-    c.values[i] = *(const u32x4*)(mine + tiles.page.value_codes(offset + half * 4, granule));
-    c.value_powers[i] = *(const unsigned*)(mine + tiles.page.value_power(offset + half * 4, granule / 4));
-  }
-}
-
-// A thread's codes as bfloat16 into LDS: keys [D / 8][64][8], values [8][D][8].  `bad`: per block of 32 elements, the keys whose value is no number: it counts as zero, and as what
-// it is where it is seen.  Keys beyond `last`, which nobody sees, are made small numbers, whatever lies there.
-__device__ __forceinline__ void unpack_tile(const Codes& c, unsigned char* keys, unsigned char* values, unsigned long long* bad, int base, int last) {
-#pragma unroll
-  for (int i = 0; i < UNITS_ROUNDS; ++i) {
-    const unsigned unit = i * SHARED_THREADS + threadIdx.x;
-    if (2 * D % SHARED_THREADS && unit >= 2 * D) continue;
-    {
-      const unsigned key = unit % TILE, block = unit / TILE;
-      const float power = packed_power(c.key_power[i]);
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const unsigned codes = c.keys[i][j];
-        *(u32x4*)(keys + ((block * 4 + j) * TILE + key) * 16) = (u32x4){unpack_pair<0>(codes, power), unpack_pair<1>(codes, power), unpack_pair<2>(codes, power), unpack_pair<3>(codes, power)};
-      }
-    }
-    const unsigned piece = unit / (D / 4), half = unit % 2, granule = unit / 2 % (D / 8);
-    const int first = piece * 8 + half * 4;   // key of the tile
-    unsigned powers = c.value_powers[i];
-    const unsigned no_number = powers & (powers >> 4) & 0x0f0f0f0fu;  // (bytes of 255: all of these eight bits)
-    if (base + first + 3 > last || (((no_number & (no_number >> 2)) & 0x03030303u) != 0u)) {
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const bool unseen = base + first + j > last, none = ((powers >> (8 * j)) & 255u) == PACKED_NO_NUMBER;
-        if (none && !unseen) atomicOr(&bad[granule / 4], 1ull << (first + j));
-        if (none || unseen) powers &= ~(255u << (8 * j));
-      }
-    }
-    unsigned raw[4][4];
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const float power = __uint_as_float(j == 3 ? powers >> 1 : powers << (23 - j * 8));
-      const unsigned codes = c.values[i][j];
-      raw[j][0] = unpack_pair<0>(codes, power);
-      raw[j][1] = unpack_pair<1>(codes, power);
-      raw[j][2] = unpack_pair<2>(codes, power);
-      raw[j][3] = unpack_pair<3>(codes, power);
-    }
-    unsigned char* to = values + (piece * D + granule * 8) * 16 + half * 8;
-    const unsigned exchange = (granule >> 1) & 7;
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      *(u32x2*)(to + ((2 * e) ^ exchange) * 16) = (u32x2){__builtin_amdgcn_perm(raw[1][e], raw[0][e], 0x05040100u), __builtin_amdgcn_perm(raw[3][e], raw[2][e], 0x05040100u)};
-      *(u32x2*)(to + ((2 * e + 1) ^ exchange) * 16) = (u32x2){__builtin_amdgcn_perm(raw[1][e], raw[0][e], 0x07060302u), __builtin_amdgcn_perm(raw[3][e], raw[2][e], 0x07060302u)};
-    }
-  }
-}
 
 struct WideColumns {                          // a wave's 32
   Eight query[D / 16];
   int position;                               // of the lane's column's token
-  int first_position, last_position;          // of the wave's
   float reference, total;                     // total: of the lane's half of the keys
+  bool begun;                                 // some key has been seen; before, the reference is 0
   f32x16 sum[D / 32];
 };
 
-// 32 keys of a tile, from `base` on (`sub` the first or the second of the tile).  edge: some column does not see some of them.
-__device__ __forceinline__ void take_half(WideColumns& columns, const unsigned char* keys, const unsigned char* values, const Walk& w, int base, int sub, bool edge) {
+__device__ __forceinline__ f32x16 multiply(const Eight& a, const Eight& b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a.v, b.v, c, 0, 0, 0); }
+
+__device__ __forceinline__ void read_step(WideStep& s, const unsigned char* stage) {
+  const unsigned lane = threadIdx.x % WAVE, n = lane & 31, h = lane >> 5, at = (unsigned)(size_t)(const unsigned char __attribute__((address_space(3)))*)stage;
+  const unsigned row = (n & 0x13) | ((n & 4) << 1) | ((n & 8) >> 1);  // the key that row n of the first product is
+  const unsigned keys = at + (row >> 3) * PIECE + (row & 7) * (D / 2) + h * (D / 4), key_powers = at + 4 * PIECE + (row >> 3) * (D / 2) + (row & 7) * (D / 32) + h * (D / 64);
+  if constexpr (D == 128) {
+    const unsigned values = at + h * PIECE + 4 * D + (n >> 1) * 32, value_powers = at + 4 * PIECE + h * (D / 2) + D / 4 + (n >> 3) * 8;
+    asm volatile(
+        "ds_read_b128 %0, %10\n\tds_read_b128 %1, %10 offset:16\n\tds_read_u8 %2, %11\n\tds_read_u8 %3, %11 offset:1\n\tds_read_b128 %4, %12\n\tds_read_b128 %5, %12 offset:16\n\t"
+        "ds_read_b64 %8, %13\n\tds_read_b128 %6, %12 offset:%14\n\tds_read_b128 %7, %12 offset:%15\n\tds_read_b64 %9, %13 offset:%16\n\ts_waitcnt lgkmcnt(0)"
+        : "=&v"(s.keys[0]), "=&v"(s.keys[1]), "=&v"(s.key_powers[0]), "=&v"(s.key_powers[1]), "=&v"(s.values[0][0][0]), "=&v"(s.values[0][0][1]), "=&v"(s.values[1][0][0]),
+          "=&v"(s.values[1][0][1]), "=&v"(s.value_powers[0][0]), "=&v"(s.value_powers[1][0])
+        : "v"(keys), "v"(key_powers), "v"(values), "v"(value_powers), "n"(2 * PIECE), "n"(2 * PIECE + 16), "n"(D)
+        : "memory");
+  } else {
+#pragma unroll
+    for (int i = 0; i < HALF_BLOCKS; ++i) {
+      asm volatile("ds_read_b128 %0, %1 offset:%2" : "=v"(s.keys[i]) : "v"(keys), "n"(i * 16) : "memory");
+      asm volatile("ds_read_u8 %0, %1 offset:%2" : "=v"(s.key_powers[i]) : "v"(key_powers), "n"(i) : "memory");
+    }
+#pragma unroll
+    for (int u = 0; u < 2; ++u)
+#pragma unroll
+      for (int c = 0; c < CHUNKS; ++c) {
+        const unsigned granule = chunk_first(c) / 8 + n * chunk_width(c) / 256, value = at + (2 * u + h) * PIECE + 4 * D + granule * 32;
+        asm volatile("ds_read_b128 %0, %1" : "=v"(s.values[u][c][0]) : "v"(value) : "memory");
+        asm volatile("ds_read_b128 %0, %1 offset:16" : "=v"(s.values[u][c][1]) : "v"(value) : "memory");
+        asm volatile("ds_read_b64 %0, %1" : "=v"(s.value_powers[u][c]) : "v"(at + 4 * PIECE + (2 * u + h) * (D / 2) + D / 4 + granule / 4 * 8) : "memory");
+      }
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    // used only after the wait
+#pragma unroll
+    for (int i = 0; i < HALF_BLOCKS; ++i) asm volatile("" : "+v"(s.keys[i]), "+v"(s.key_powers[i]));
+#pragma unroll
+    for (int u = 0; u < 2; ++u)
+#pragma unroll
+      for (int c = 0; c < CHUNKS; ++c) asm volatile("" : "+v"(s.values[u][c][0]), "+v"(s.values[u][c][1]), "+v"(s.value_powers[u][c]));
+  }
+}
+
+template <bool EDGE> __device__ __forceinline__ void take_step(WideColumns& columns, const WideStep& now, const Walk& w, const Item& item, int base) {
   const int lane = threadIdx.x % WAVE, n = lane & 31, h = lane >> 5;
-  const int row = (n & 0x13) | ((n & 4) << 1) | ((n & 8) >> 1);  // the key that row n of the product is
+  // scores: value 8 u + j of a lane is key 16 u + 8 h + j of the step
   f32x16 score;
 #pragma unroll
   for (int i = 0; i < 16; ++i) score[i] = 0.f;
-  const unsigned char* mine = keys + (h * TILE + sub * 32 + row) * 16;
 #pragma unroll
   for (int s = 0; s < D / 16; ++s) {
+    const float power = packed_power(now.key_powers[s / 4]);
+    const unsigned codes = now.keys[s / 4][s % 4];
     Eight key;
-    key.u = *(const u32x4*)(mine + 2 * s * TILE * 16);
-    score = __builtin_amdgcn_mfma_f32_32x32x16_bf16(key.v, columns.query[s].v, score, 0, 0, 0);
+    key.u = (u32x4){unpack_pair<0>(codes, power), unpack_pair<1>(codes, power), unpack_pair<2>(codes, power), unpack_pair<3>(codes, power)};
+    score = multiply(key, columns.query[s], score);
   }
-  if (edge) {
-    const int highest = columns.position - base - 8 * h, lowest = w.window > 0 ? highest - w.window + 1 : -(1 << 30);
+  const int highest = columns.position - base - 8 * h, lowest = w.window > 0 ? highest - w.window + 1 : -(1 << 30);
+  const auto sees = [&](int i) { return 16 * (i / 8) + i % 8 <= highest && 16 * (i / 8) + i % 8 >= lowest; };
+  float x[16];                                // log2 of the weights
 #pragma unroll
-    for (int i = 0; i < 16; ++i) {
-      const int key = 16 * (i / 8) + i % 8;
-      if (key > highest || key < lowest) score[i] = -INFINITY;
-    }
+  for (int i = 0; i < 16; ++i) {
+    const float y = __builtin_fmaf(score[i], w.scale, -columns.reference);
+    x[i] = !EDGE || sees(i) ? y : -INFINITY;
   }
-  float x[16];
-#pragma unroll
-  for (int i = 0; i < 16; ++i) x[i] = __builtin_fmaf(score[i], w.scale, -columns.reference);
-  if (__any(fmaxf(largest_of(x), largest_of(x + 8)) > AHEAD)) {
-#pragma unroll
-    for (int i = 0; i < 16; ++i) x[i] = score[i] * w.scale;
-    float largest = fmaxf(largest_of(x), largest_of(x + 8));
-    largest = fmaxf(fmaxf(largest, __shfl_xor(largest, 32)), columns.reference);
-    const float change = __builtin_amdgcn_exp2f(columns.reference - largest);
-    columns.reference = largest;
+  float largest = fmaxf(largest_of(x), largest_of(x + 8));
+  if (__any(largest > (columns.begun ? AHEAD : -INFINITY))) {
+    largest = fmaxf(largest, __shfl_xor(largest, 32));
+    // (a column's first reference is its first largest score, wherever that lies; later ones only rise)
+    const float rise = largest > (columns.begun ? 0.f : -INFINITY) ? largest : 0.f, change = columns.begun ? __builtin_amdgcn_exp2f(-rise) : 1.f;
+    columns.begun = columns.begun || largest > -INFINITY;
+    columns.reference += rise;
     columns.total *= change;
 #pragma unroll
     for (int t = 0; t < D / 32; ++t) columns.sum[t] *= change;
 #pragma unroll
-    for (int i = 0; i < 16; ++i) x[i] -= largest;
+    for (int i = 0; i < 16; ++i) x[i] -= rise;
   }
-  const unsigned char* first = values + ((sub * 4 + h) * D + n / 8 * 8) * 16;
 #pragma unroll
   for (int u = 0; u < 2; ++u) {
     Eight weight;
@@ -893,122 +829,146 @@ __device__ __forceinline__ void take_half(WideColumns& columns, const unsigned c
       columns.total = __builtin_amdgcn_fdot2_f32_bf16(pair.v, ones.v, columns.total, false);
     }
 #pragma unroll
-    for (int t = 0; t < D / 32; ++t) {
-      Eight value;
-      value.u = *(const u32x4*)(first + (2 * u * D + t * 32) * 16 + ((n & 7) ^ ((t * 2 + (n >> 4)) & 7)) * 16);
-      columns.sum[t] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(value.v, weight.v, columns.sum[t], 0, 0, 0);
+    for (int c = 0; c < CHUNKS; ++c) {
+      const int width = chunk_width(c), first = chunk_first(c) / 32;
+      u32x2 powers = now.value_powers[u][c];
+      bool poisoned = false;
+      Eight marks;
+      if (EDGE) {  // (as above: what no column sees is a small number; what is no number is taken out, and put back where it is seen)
+        marks.u = (u32x4){0u, 0u, 0u, 0u};
+        bool mine = false;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          const int key = base + 16 * u + 8 * h + j;
+          const unsigned shift = (j & 3) * 8, byte = (powers[j / 4] >> shift) & 255u;
+          const bool unseen = key > item.last_position || (w.window > 0 && key <= item.first_position - w.window), bad = byte == PACKED_NO_NUMBER;
+          if (unseen || bad) powers[j / 4] &= ~(255u << shift);
+          if (bad && !unseen) {
+            marks.u[j / 2] |= 0x3f80u << (j % 2 * 16);
+            mine = true;
+          }
+        }
+        poisoned = __any(mine);
+      }
+      Eight value[4];                         // the lane's elements (two at a width of 64), of eight keys
+#pragma unroll
+      for (int j = 0; j < 8; j += 2) {
+        const float power0 = __uint_as_float(powers[j / 4] << (23 - j % 4 * 8)), power1 = __uint_as_float(j % 4 == 2 ? powers[j / 4] >> 1 : powers[j / 4] << 15);
+        const unsigned a = now.values[u][c][j / 4][j % 4], b = now.values[u][c][j / 4][j % 4 + 1];
+        if (width == 128) {                   // two of a granule's four bytes, of two keys
+          const unsigned both = __builtin_amdgcn_perm(b, a, n & 1 ? 0x07060302u : 0x05040100u);
+          const unsigned a0 = unpack_pair<0>(both, power0), a1 = unpack_pair<1>(both, power0), b0 = unpack_pair<2>(both, power1), b1 = unpack_pair<3>(both, power1);
+          value[0].u[j / 2] = __builtin_amdgcn_perm(b0, a0, 0x05040100u);
+          value[1].u[j / 2] = __builtin_amdgcn_perm(b0, a0, 0x07060302u);
+          value[2].u[j / 2] = __builtin_amdgcn_perm(b1, a1, 0x05040100u);
+          value[3].u[j / 2] = __builtin_amdgcn_perm(b1, a1, 0x07060302u);
+        } else {                              // one of them
+          const unsigned both = __builtin_amdgcn_perm(b, a, (unsigned)((n & 3) | (4 + (n & 3)) << 8));
+          const unsigned a0 = unpack_pair<0>(both, power0), b0 = unpack_pair<1>(both, power1);
+          value[0].u[j / 2] = __builtin_amdgcn_perm(b0, a0, 0x05040100u);
+          value[1].u[j / 2] = __builtin_amdgcn_perm(b0, a0, 0x07060302u);
+        }
+      }
+#pragma unroll
+      for (int e = 0; e < width / 32; ++e) columns.sum[first + e] = multiply(value[e], weight, columns.sum[first + e]);
+      if (EDGE && poisoned) {
+        Eight seen;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) seen.v[j] = (bf16_t)(sees(8 * u + j) ? 1.f : 0.f);
+        f32x16 none;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) none[i] = 0.f;
+        const f32x16 hit = multiply(marks, seen, none);
+#pragma unroll
+        for (int e = 0; e < width / 32; ++e)
+#pragma unroll
+          for (int i = 0; i < 16; ++i)
+            if (hit[i] > 0.f) columns.sum[first + e][i] = __uint_as_float(0x7fc00000u);
+      }
     }
   }
 }
 
-__device__ __forceinline__ int wide_units(const Walk& w, const Item& item) { return (item.to - item.from / TILE * TILE + TILE - 1) / TILE; }
-
-__global__ void __launch_bounds__(SHARED_THREADS, D <= 128 ? 2 : 1)
-packed_shared_kernel(const bf16_t* q, int q_stride, bf16_t* out, int out_stride, const unsigned char* pages, Walk w, Streams streams, int items, int whole, int whole_out) {
-  constexpr int TILE_BYTES = TILE * D * 2;
-  __shared__ __attribute__((aligned(16))) unsigned char memory[2][2 * TILE_BYTES];
-  __shared__ unsigned long long bad[3][D / 32];
-  __shared__ int item_ends[SHARED_THREADS], ends[SHARED_THREADS], wave_sums[2][SHARED_THREADS / WAVE];
-  __shared__ Request held[SHARED_THREADS];
-  const int lane = threadIdx.x % WAVE, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / WAVE), n = lane & 31, h = lane >> 5, group = w.heads / w.kv_heads;
-
-  const auto take_walk = [&](const Item& item, int kv_head, int begin, int end, float* part) {
-    SharedTiles tiles;
-    tiles.page = {D, w.page_size};
-    tiles.from = pages + (size_t)kv_head * tiles.page.bytes();
-    tiles.table = w.tables + (size_t)item.request * w.table_width;
-    tiles.page_stride = (unsigned)w.kv_heads * tiles.page.bytes();
-    Entries entries[3];
+__device__ __forceinline__ void load_queries(WideColumns& columns, const bf16_t* q, int q_stride, const Item& item, int kv_head, bool whole) {
+  const int lane = threadIdx.x % WAVE, n = lane & 31, h = lane >> 5, flat = item.first + min(n, item.columns - 1), token = flat / item.group;
+  columns.position = item.first_position - item.first / item.group + token;
+  const bf16_t* row = q + (size_t)(item.first_row + token) * q_stride + (kv_head * item.group + flat - token * item.group) * D + h * (D / 2);
 #pragma unroll
-    for (int i = 0; i < 3; ++i) load_entries(entries[i], w, tiles, begin + i * TILE);
-    Codes now, next;
-    load_codes(now, entries[0], w, tiles, begin);
-    load_codes(next, entries[1], w, tiles, begin + TILE);
-    WideColumns columns;
-    const int first_column = wave * 32, column = min(first_column + n, item.columns - 1), flat = item.first + column, token = flat / group;
-    const int token_zero = item.first_position - item.first / group;  // the position that the request's first token of the step is at
-    columns.position = token_zero + token;
-    columns.first_position = token_zero + (item.first + min(first_column, item.columns - 1)) / group;
-    columns.last_position = first_column < item.columns ? token_zero + (item.first + min(first_column + 31, item.columns - 1)) / group : -1;
-    const bf16_t* row = q + (size_t)(item.first_row + token) * q_stride + (kv_head * group + flat - token * group) * D + h * 8;
-#pragma unroll
-    for (int s = 0; s < D / 16; ++s) {
-      if (whole) {
-        columns.query[s].u = *(const u32x4*)(row + s * 16);
-      } else {
-#pragma unroll
-        for (int e = 0; e < 8; ++e) columns.query[s].v[e] = row[s * 16 + e];
-      }
-    }
-    columns.reference = NO_SCORE;
-    columns.total = 0.f;
-#pragma unroll
-    for (int t = 0; t < D / 32; ++t)
-#pragma unroll
-      for (int i = 0; i < 16; ++i) columns.sum[t][i] = 0.f;
-    __syncthreads();                          // (a walk before this one has been read, and what it marked)
-    if (threadIdx.x < 3 * (D / 32)) (&bad[0][0])[threadIdx.x] = 0ull;
-    __syncthreads();
-    unpack_tile(now, memory[0], memory[0] + TILE_BYTES, bad[0], begin, item.last_position);
-    int turn = 0, third = 0;                  // of the tile that is multiplied: its place in LDS, that of its marks
-    for (int base = begin; base < end; base += TILE) {
-      __syncthreads();
-      now = next;
-      entries[1] = entries[2];
-      load_codes(next, entries[1], w, tiles, base + 2 * TILE);
-      load_entries(entries[2], w, tiles, base + 3 * TILE);
-      if (threadIdx.x < D / 32) bad[third == 0 ? 2 : third - 1][threadIdx.x] = 0ull;  // (those of the tile before, which are those of the next but one)
-      const unsigned char *keys = memory[turn], *values = memory[turn] + TILE_BYTES;
-#pragma unroll 1
-      for (int sub = 0; sub < 2; ++sub) {
-        const int from = base + sub * 32;
-        if (from < end && from <= columns.last_position && (w.window <= 0 || from + 31 > columns.first_position - w.window))
-          take_half(columns, keys, values, w, from, sub, from + 31 > columns.first_position || (w.window > 0 && from < columns.last_position - w.window + 1));
-      }
-#pragma unroll
-      for (int t = 0; t < D / 32; ++t) {
-        const unsigned long long marked = bad[third][t];
-        if (marked) {                         // hardly ever: values that are no number, for the columns that see them
-          const int lowest = w.window > 0 ? max(columns.position - w.window + 1 - base, 0) : 0, highest = min(columns.position - base, TILE - 1);
-          const unsigned long long seen = highest < lowest ? 0ull : ((2ull << highest) - 1ull) & ~((1ull << lowest) - 1ull);
-          if (marked & seen)
-#pragma unroll
-            for (int i = 0; i < 16; ++i) columns.sum[t][i] = __uint_as_float(0x7fc00000u);
-        }
-      }
-      turn ^= 1;
-      third = third == 2 ? 0 : third + 1;
-      if (base + TILE < end) unpack_tile(now, memory[turn], memory[turn] + TILE_BYTES, bad[third], base + TILE, item.last_position);
-    }
-    const float weights = columns.total + __shfl_xor(columns.total, 32);
-    if (first_column + n >= item.columns) return;
-    if (part) {
-      float* to = part + (first_column + n) * (D + 4);
-#pragma unroll
-      for (int t = 0; t < D / 32; ++t)
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-          *(f32x4*)(to + t * 32 + 8 * i + 4 * h) = (f32x4){columns.sum[t][4 * i], columns.sum[t][4 * i + 1], columns.sum[t][4 * i + 2], columns.sum[t][4 * i + 3]};
-      if (h == 0) *(f32x4*)(to + D) = (f32x4){columns.reference, weights, 0.f, 0.f};
+  for (int s = 0; s < D / 16; ++s) {
+    if (whole) {
+      columns.query[s].u = *(const u32x4*)(row + s * 8);
     } else {
-      const float over = 1.f / weights;
-      bf16_t* to = out + (size_t)(item.first_row + token) * out_stride + (kv_head * group + flat - token * group) * D;
 #pragma unroll
-      for (int t = 0; t < D / 32; ++t)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          union { bf16_t e[4]; u32x2 u; } four;
-#pragma unroll
-          for (int j = 0; j < 4; ++j) four.e[j] = (bf16_t)(columns.sum[t][4 * i + j] * over);
-          if (whole_out) {
-            *(u32x2*)(to + t * 32 + 8 * i + 4 * h) = four.u;
-          } else {
-#pragma unroll
-            for (int j = 0; j < 4; ++j) to[t * 32 + 8 * i + 4 * h + j] = four.e[j];
-          }
-        }
+      for (int e = 0; e < 8; ++e) columns.query[s].v[e] = row[s * 8 + e];
     }
-  };
+  }
+  columns.reference = columns.total = 0.f;
+  columns.begun = false;
+#pragma unroll
+  for (int t = 0; t < D / 32; ++t)
+#pragma unroll
+    for (int i = 0; i < 16; ++i) columns.sum[t][i] = 0.f;
+}
+
+__device__ __forceinline__ void settle(WideColumns& columns) {
+#pragma unroll
+  for (int s = 0; s < D / 16; ++s) asm volatile("" : "+v"(columns.query[s].u));
+}
+
+// (memory as above: 16 columns at a time)
+template <int W, typename Take>
+__device__ __forceinline__ void bring_together(const WideColumns& columns, int count, int wave, unsigned char* memory, Take take) {
+  float (*results)[16][D + 4] = (float (*)[16][D + 4])memory;
+  float (*sums)[16][2] = (float (*)[16][2])(memory + W * 16 * (D + 4) * 4);
+  const int lane = threadIdx.x % WAVE, n = lane & 31, h = lane >> 5, r = n & 15;
+  const float total = columns.total + __shfl_xor(columns.total, 32);
+#pragma unroll
+  for (int half = 0; half < 2; ++half) {
+    if (half * 16 >= count) break;
+    __syncthreads();
+    if (n / 16 == half) {
+      if (h == 0) {
+        sums[wave][r][0] = columns.begun ? columns.reference : -INFINITY;
+        sums[wave][r][1] = total;
+      }
+#pragma unroll
+      for (int c = 0; c < CHUNKS; ++c) {
+        const int each = chunk_width(c) / 32, first = chunk_first(c) / 32;  // neighbouring elements of a row of the tiles
+#pragma unroll
+        for (int i = 0; i < 16; ++i)
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            if (e < each) results[wave][r][chunk_first(c) + (8 * (i / 4) + 4 * h + i % 4) * each + e] = columns.sum[first + e][i];
+      }
+    }
+    __syncthreads();
+    join_waves<W>(results, sums, min(16, count - half * 16), [&](int column, int d, f32x4 result, float largest, float weights) { take(half * 16 + column, d, result, largest, weights); });
+  }
+}
+
+// Which columns a wave takes: 32 at heads of a multiple of 64 in bfloat16, 16 elsewhere.
+template <typename T> constexpr bool WIDE = sizeof(T) == 2 && D % 64 == 0;
+template <typename T> constexpr int PORTION_COLUMNS = WIDE<T> ? 32 : 16;
+template <typename T> constexpr int PORTION_PART = PORTION_COLUMNS<T> * (D + 4);
+template <typename T, bool> struct PortionOf {
+  typedef Columns<T, 1> Cols;
+  typedef Step Taken;
+};
+template <typename T> struct PortionOf<T, true> {
+  typedef WideColumns Cols;
+  typedef WideStep Taken;
+};
+
+__device__ __forceinline__ int portion_units(const Item& item) { return BEGINNING + (item.to - item.from + PORTION_UNIT - 1) / PORTION_UNIT; }
+
+template <typename T>
+__global__ void __launch_bounds__(PORTION_THREADS, D <= 128 ? 2 : 1) packed_portions_kernel(const T* q, int q_stride, T* out, int out_stride, const unsigned char* pages, Walk w, Streams streams, int items, int whole) {
+  constexpr int COLUMNS = PORTION_COLUMNS<T>;
+  __shared__ __attribute__((aligned(16))) unsigned char memory[memory_of<PORTION_WAVES>()];
+  __shared__ int item_ends[PORTION_THREADS], ends[PORTION_THREADS], wave_sums[2][PORTION_WAVES];
+  __shared__ Request held[PORTION_THREADS];
+  const int lane = threadIdx.x % WAVE, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / WAVE), group = w.heads / w.kv_heads;
+
   // where the requests' items end, then where the items' units end (no more requests than threads; a run of items a thread)
   const auto added_up = [&](int mine, int* sums) {
 #pragma unroll
@@ -1021,66 +981,78 @@ packed_shared_kernel(const bf16_t* q, int q_stride, bf16_t* out, int out_stride,
     for (int v = 0; v < wave; ++v) mine += sums[v];
     return mine;
   };
-  int all_items = 0, run = 0, share = 1, first = 0, last = 1;
+  int all_items = 0, run = 0, share = 1, first = 0, last = 1, total = 0;
   const auto item_at = [&](int index, Item& item) {
-    int low = 0, high = SHARED_THREADS - 1;
+    int low = 0, high = PORTION_THREADS - 1;
     while (low < high) {
       const int middle = (low + high) / 2;
       if (item_ends[middle] > index) high = middle;
       else low = middle + 1;
     }
-    return make_item(w, low, held[low], (index - (low > 0 ? item_ends[low - 1] : 0)) * WIDE, WIDE, item);
+    return make_item(w, low, held[low], (index - (low > 0 ? item_ends[low - 1] : 0)) * COLUMNS, COLUMNS, item);
+  };
+  // the walk that a unit lies in, and where in it: kv head, unit of it, units
+  const auto walk_at = [&](int at, Item& item, int& kv_head, int& unit, int& each) {
+    int low = 0, high = PORTION_THREADS - 1;
+    while (low < high) {
+      const int middle = (low + high) / 2;
+      if (ends[middle] > at) high = middle;
+      else low = middle + 1;
+    }
+    int index = __builtin_amdgcn_readfirstlane(low) * run, inside = __builtin_amdgcn_readfirstlane(at - (low > 0 ? ends[low - 1] : 0));
+    for (; index < all_items; ++index) {
+      each = __builtin_amdgcn_readfirstlane(item_at(index, item) ? portion_units(item) : 0);
+      if (inside < each * w.kv_heads) break;
+      inside -= each * w.kv_heads;
+    }
+    if (index >= all_items) return false;
+    kv_head = inside / each;
+    unit = inside - kv_head * each;
+    return true;
   };
   if (streams.least > 0) {
     int count = 0;
     if ((int)threadIdx.x < w.requests) {
       held[threadIdx.x] = load_request(w, threadIdx.x);
       const int tokens = held[threadIdx.x].count;
-      count = few_columns(tokens, group) ? 0 : (max(tokens, 0) * group + WIDE - 1) / WIDE;
+      count = few_columns(tokens, group) ? 0 : (max(tokens, 0) * group + COLUMNS - 1) / COLUMNS;
     }
     item_ends[threadIdx.x] = added_up(count, wave_sums[0]);
     __syncthreads();
-    all_items = __builtin_amdgcn_readfirstlane(item_ends[SHARED_THREADS - 1]);
-    run = (all_items + SHARED_THREADS - 1) / SHARED_THREADS;
+    all_items = __builtin_amdgcn_readfirstlane(item_ends[PORTION_THREADS - 1]);
+    run = (all_items + PORTION_THREADS - 1) / PORTION_THREADS;
     int units = 0;
     for (int i = threadIdx.x * run; i < min((int)(threadIdx.x + 1) * run, all_items); ++i) {
       Item item;
-      if (item_at(i, item)) units += wide_units(w, item) * w.kv_heads;
+      if (item_at(i, item)) units += portion_units(item) * w.kv_heads;
     }
     ends[threadIdx.x] = added_up(units, wave_sums[1]);
     __syncthreads();
-    const int total = __builtin_amdgcn_readfirstlane(ends[SHARED_THREADS - 1]);
-    share = max(streams.least, (total + (int)gridDim.x - 1) / (int)gridDim.x);
+    total = __builtin_amdgcn_readfirstlane(ends[PORTION_THREADS - 1]);
+    share = max(max(streams.least, BEGINNING + 1), (total + (int)gridDim.x - 1) / (int)gridDim.x);
     first = min(blockIdx.x * (long)share, (long)total);
     last = min(first + share, total);
     if (threadIdx.x == 0) streams.cuts[blockIdx.x].parts = 0;
+    // a walk is not cut within its beginning: a cut there is one before it (the next workgroup's `first` the same way)
+    if (first < last) {
+      Item item;
+      int kv_head, unit, each;
+      if (walk_at(first, item, kv_head, unit, each) && unit <= BEGINNING) first -= unit;
+      if (last < total && walk_at(last, item, kv_head, unit, each) && unit <= BEGINNING) last -= unit;
+    }
   }
   for (int at = first; at < last;) {
     Item item;
     int kv_head, begin, taken = 1, each = 1, unit = 0, place = 0;
     if (streams.least == 0) {                 // a walk whole; the longest begin first: a request's last columns walk most keys
-      if (!find_item(w, items - 1 - blockIdx.x / w.kv_heads, WIDE, item)) return;
+      if (!find_item(w, items - 1 - blockIdx.x / w.kv_heads, COLUMNS, item)) return;
       kv_head = blockIdx.x % w.kv_heads;
-      begin = item.from / TILE * TILE;
+      begin = item.from;
     } else {
-      int low = 0, high = SHARED_THREADS - 1;
-      while (low < high) {
-        const int middle = (low + high) / 2;
-        if (ends[middle] > at) high = middle;
-        else low = middle + 1;
-      }
-      int index = __builtin_amdgcn_readfirstlane(low) * run, inside = __builtin_amdgcn_readfirstlane(at - (low > 0 ? ends[low - 1] : 0));
-      for (; index < all_items; ++index) {
-        each = __builtin_amdgcn_readfirstlane(item_at(index, item) ? wide_units(w, item) : 0);
-        if (inside < each * w.kv_heads) break;
-        inside -= each * w.kv_heads;
-      }
-      if (index >= all_items) break;
-      kv_head = inside / each;
-      unit = inside - kv_head * each;
+      if (!walk_at(at, item, kv_head, unit, each)) break;
       taken = min(each - unit, last - at);
       place = at == first ? 0 : 1;
-      begin = __builtin_amdgcn_readfirstlane(item.from) / TILE * TILE + unit * TILE;
+      begin = item.from + max(unit - BEGINNING, 0) * PORTION_UNIT;
     }
     item.request = __builtin_amdgcn_readfirstlane(item.request);
     item.first_row = __builtin_amdgcn_readfirstlane(item.first_row);
@@ -1088,9 +1060,24 @@ packed_shared_kernel(const bf16_t* q, int q_stride, bf16_t* out, int out_stride,
     item.columns = __builtin_amdgcn_readfirstlane(item.columns);
     item.first_position = __builtin_amdgcn_readfirstlane(item.first_position);
     item.last_position = __builtin_amdgcn_readfirstlane(item.last_position);
+    item.from = __builtin_amdgcn_readfirstlane(item.from);
     item.to = __builtin_amdgcn_readfirstlane(item.to);
+    begin = __builtin_amdgcn_readfirstlane(begin);
     const bool cut = taken < each;
-    take_walk(item, kv_head, begin, streams.least == 0 || unit + taken == each ? item.to : begin + taken * TILE, cut ? streams.parts + ((size_t)blockIdx.x * 2 + place) * WIDE_PART : nullptr);
+    const int end = streams.least == 0 || unit + taken == each ? item.to : item.from + (unit + taken - BEGINNING) * PORTION_UNIT;
+    float* part = cut ? streams.parts + ((size_t)blockIdx.x * 2 + place) * PORTION_PART<T> : nullptr;
+    typename PortionOf<T, WIDE<T>>::Cols columns;
+    __syncthreads();                          // (what a walk before this one left in LDS has been read)
+    walk_keys<T, typename PortionOf<T, WIDE<T>>::Taken, PORTION_WAVES>(columns, q, q_stride, pages, w, item, kv_head, whole, begin, end, wave, memory + wave * (STAGES * STAGE));
+    bring_together<PORTION_WAVES>(columns, item.columns, wave, memory, [&](int column, int d, f32x4 result, float largest, float weights) {
+      if (part) {
+        *(f32x4*)(part + column * (D + 4) + d) = result;
+        if (d == 0) *(f32x4*)(part + column * (D + 4) + D) = (f32x4){largest, weights, 0.f, 0.f};
+      } else {
+        const int flat = item.first + column, token = flat / item.group, head = kv_head * item.group + flat - token * item.group;
+        write_four(out + (size_t)(item.first_row + token) * out_stride + head * D + d, result * (1.f / weights));
+      }
+    });
     if (cut && unit == 0 && threadIdx.x == 0)
       streams.cuts[blockIdx.x] = {item.first_row, group, item.first, item.columns, kv_head, (at + each - 1) / share - (int)blockIdx.x + 1, place, 0};
     at += taken;
@@ -1099,11 +1086,11 @@ packed_shared_kernel(const bf16_t* q, int q_stride, bf16_t* out, int out_stride,
 
 // ---------------------------------------------------------------------------------------------------------------- launches
 
-constexpr int WORKGROUPS = 512;               // two a CU, as many as its LDS holds (one where heads are wider than 128)
+constexpr int WORKGROUPS = 512, PORTION_WORKGROUPS = 512;  // two a CU, as many as its LDS or registers hold (at heads of up to 128)
 
 template <typename T>
 static int launch(const void* q, int q_stride, void* out, int out_stride, const void* pages, const Walk& w, const Streams& few, const Streams& many, int tokens, int kinds, hipStream_t stream) {
-  const int group = w.heads / w.kv_heads, piece = sizeof(T) == 4 ? 4 : 8, whole = (size_t)q % 16 == 0 && q_stride % piece == 0, whole_out = (size_t)out % 8 == 0 && out_stride % 4 == 0;
+  const int group = w.heads / w.kv_heads, piece = sizeof(T) == 4 ? 4 : 8, whole = (size_t)q % 16 == 0 && q_stride % piece == 0;
   if (kinds & 1) {
     const long blocks = few.least ? WORKGROUPS : (long)w.requests * ((group + 15) / 16) * w.kv_heads;
     if (blocks >= (1L << 31)) return ERR_BAD_ARGUMENT;
@@ -1113,26 +1100,22 @@ static int launch(const void* q, int q_stride, void* out, int out_stride, const 
     if (int status = LAUNCH_STATUS()) return status;
   }
   if (!(kinds & 2)) return 0;
-  if constexpr (sizeof(T) == 4) {
-    const long items = ((long)tokens * group + 15) / 16 + w.requests, blocks = items * w.kv_heads;
-    if (blocks >= (1L << 31)) return ERR_BAD_ARGUMENT;
-    packed_portions_kernel<T, 1><<<(unsigned)blocks, PORTION_WAVES * WAVE, 0, stream>>>((const T*)q, q_stride, (T*)out, out_stride, (const unsigned char*)pages, w, (int)items, whole);
-  } else {
-    const long items = ((long)tokens * group + WIDE - 1) / WIDE + w.requests, blocks = many.least ? WORKGROUPS : items * w.kv_heads;
-    if (blocks >= (1L << 31)) return ERR_BAD_ARGUMENT;
-    packed_shared_kernel<<<(unsigned)blocks, SHARED_THREADS, 0, stream>>>((const T*)q, q_stride, (T*)out, out_stride, (const unsigned char*)pages, w, many, (int)items, whole, whole_out);
-    if (int status = LAUNCH_STATUS()) return status;
-    if (many.least) packed_join_kernel<T><<<dim3(WORKGROUPS, 8), 4 * WAVE, 0, stream>>>((T*)out, out_stride, many, WIDE);
-  }
+  const long items = ((long)tokens * group + PORTION_COLUMNS<T> - 1) / PORTION_COLUMNS<T> + w.requests, blocks = many.least ? PORTION_WORKGROUPS : items * w.kv_heads;
+  if (blocks >= (1L << 31)) return ERR_BAD_ARGUMENT;
+  packed_portions_kernel<T><<<(unsigned)blocks, PORTION_THREADS, 0, stream>>>((const T*)q, q_stride, (T*)out, out_stride, (const unsigned char*)pages, w, many, (int)items, whole);
+  if (int status = LAUNCH_STATUS()) return status;
+  if (many.least) packed_join_kernel<T><<<dim3(PORTION_WORKGROUPS, PORTION_COLUMNS<T> / 4), 4 * WAVE, 0, stream>>>((T*)out, out_stride, many, PORTION_COLUMNS<T>);
   return LAUNCH_STATUS();
 }
 
-// Floats of workspace that requests of few columns, or of many (bfloat16), need where walks may be cut.
-extern "C" int llmserve_packed_attention_workspace(int many) { return WORKGROUPS * (2 * (many ? WIDE_PART : PART) + (int)(sizeof(Cut) / 4)); }
+// Floats of workspace that requests of few columns, or of many, need where walks may be cut.
+extern "C" int llmserve_packed_attention_workspace(int many) {
+  return many ? PORTION_WORKGROUPS * (2 * 32 * (D + 4) + (int)(sizeof(Cut) / 4)) : WORKGROUPS * (2 * PART + (int)(sizeof(Cut) / 4));
+}
 
 // q's heads are the first columns of rows of q_stride; tokens, requests: as many rows and requests as the arrays hold.  kinds: 1: some requests may have few columns (a
 // single token, or no more than 16 of them in all), 2: some may have more.  few_least, many_least: 0: a walk over the keys of few (many) columns is taken whole by one workgroup; else every
-// workgroup takes at least so many units of 256 (64) keys, walks are cut, and there is a workspace.  Those of many columns are cut in bfloat16 and for up to 256 requests alone.
+// workgroup takes at least so many units of 256 (128) keys, walks are cut, and there is a workspace.  Those of many columns are cut for up to 256 requests alone.
 extern "C" int llmserve_packed_attention(const void* q, int is_float, int q_stride, void* out, int out_stride, void* few_workspace, void* many_workspace, const void* pages, int num_pages, const int* tables,
                                          int table_width, const int* query_start, const int* contexts, int requests, int tokens, int heads, int kv_heads, int page_size, float scale, int window, int kinds,
                                          int few_least, int many_least, hipStream_t stream) {
@@ -1140,7 +1123,7 @@ extern "C" int llmserve_packed_attention(const void* q, int is_float, int q_stri
   if (!q || !out || !pages || !tables || !query_start || !contexts || requests < 0 || tokens < 0 || kv_heads <= 0 || heads <= 0 || heads % kv_heads || num_pages <= 0 || table_width <= 0 ||
       !packed_fits(D, page_size) || (long)page_size * D * kv_heads >= (1L << 30) || !(scale > 0.f) || (size_t)pages % 16 || q_stride < heads * D || out_stride < heads * D || window < 0 ||
       kinds < 1 || kinds > 3 || few_least < 0 || (few_least > 0 && (!few_workspace || (size_t)few_workspace % 16)) || many_least < 0 ||
-      (many_least > 0 && (!many_workspace || (size_t)many_workspace % 16 || is_float || requests > SHARED_THREADS)))
+      (many_least > 0 && (!many_workspace || (size_t)many_workspace % 16 || requests > PORTION_THREADS)))
     return ERR_BAD_ARGUMENT;
   const unsigned per_page = (unsigned)page_size / 8;
   const bool power_of_two = (per_page & (per_page - 1)) == 0;
@@ -1148,7 +1131,7 @@ extern "C" int llmserve_packed_attention(const void* q, int is_float, int q_stri
   if (!power_of_two && ((unsigned long)table_width * per_page + 64) * per_page >= (1UL << 32)) return ERR_BAD_ARGUMENT;
   const Walk w = {tables, table_width, num_pages, page_size, power_of_two ? 31 - __builtin_clz(per_page) : -1, (unsigned)(((1UL << 32) + per_page - 1) / per_page), query_start, contexts, requests, heads, kv_heads, window, scale * LOG2_E};
   const Streams few = {(float*)few_workspace, (Cut*)((float*)few_workspace + WORKGROUPS * 2 * PART), few_least};
-  const Streams many = {(float*)many_workspace, (Cut*)((float*)many_workspace + WORKGROUPS * 2 * WIDE_PART), many_least};
+  const Streams many = {(float*)many_workspace, (Cut*)((float*)many_workspace + PORTION_WORKGROUPS * 2 * 32 * (D + 4)), many_least};
   if (is_float) return launch<float>(q, q_stride, out, out_stride, pages, w, few, many, tokens, kinds, stream);
   return launch<bf16_t>(q, q_stride, out, out_stride, pages, w, few, many, tokens, kinds, stream);
 }

@@ -1771,15 +1771,15 @@ class HipKernels:
 
     @staticmethod
     def _packed_least(batch, dtype, tokens: int, requests: int, heads: int, kv_heads: int, window: int) -> tuple[int, int]:
-        """(units of 256 keys that a workgroup takes at least of walks over the keys of few columns, units of 64 keys of those of many): walks are cut anywhere.  0: every
+        """(units of 256 keys that a workgroup takes at least of walks over the keys of few columns, units of 128 keys of those of many): walks are cut anywhere.  0: every
         walk is taken whole."""
         group = heads // kv_heads
         walk = min(batch.max_context_length, window + 31) if window else batch.max_context_length
         pairs = requests * kv_heads * -(-group // 16)
         few = 0 if walk <= 1024 or 22 * walk <= 50000 + 3 * pairs * walk // 10 else 4
         most = batch.max_query_length
-        items = kv_heads * -(-tokens * group // 128)
-        many = 0 if most <= 1 or dtype == torch.float32 or requests > 256 or items >= 1024 or walk <= 512 else 8
+        items = kv_heads * -(-tokens * group // 32)
+        many = 0 if most <= 1 or requests > 256 or items >= 1024 or walk <= 512 else 8
         return few, many
 
     def _packed_attention(self, qkv, layout, batch, cell, scale: float, window: int | None, out):
