@@ -310,7 +310,8 @@ class HipKernels:
     def _stream(self) -> int:
         if self._pinned_stream is not None:
             return self._pinned_stream
-        return torch.cuda.current_stream(self.device).cuda_stream
+        # (the address of `torch.cuda.current_stream(self.device)` without the object around it, which takes the host 2 us a launch)
+        return torch._C._cuda_getCurrentRawStream(self.device.index if self.device.index is not None else torch.cuda.current_device())
 
     @contextlib.contextmanager
     def stream_scope(self):
@@ -372,8 +373,7 @@ class HipKernels:
 
     def _here(self, tensor: torch.Tensor) -> bool:
         """Whether the tensor lies in the memory of this library's device."""
-        index = self.device.index if self.device.index is not None else torch.cuda.current_device()
-        return tensor.device.type == "cuda" and tensor.device.index == index
+        return tensor.get_device() == (self.device.index if self.device.index is not None else torch.cuda.current_device())  # (-1: the host's)
 
     def _ahead(self, weights: Any, busy: int, up_to: int, rows_each: int = 16) -> tuple:
         """What a kernel of `busy` workgroups is told of the weight that the next product reads (csrc/common.h: Ahead), which takes
@@ -1722,16 +1722,20 @@ class HipKernels:
 
     def _packed_cell(self, cell, kv_heads: int, dim: int, page_size: int, what: str) -> torch.Tensor:
         """The cell's pages, which the kernels read and write by address, after a look at their shape."""
-        pages = _packed_pages(cell)
-        if pages is None or pages.dtype != torch.uint8 or pages.ndim != 3 or (cell.need.num_kv_heads, cell.need.head_dim) != (kv_heads, dim):
+        pages, need = _packed_pages(cell), cell.need
+        if pages is None or need.num_kv_heads != kv_heads or need.head_dim != dim:
             raise KernelError(f"{what}: the cell keeps no keys and values in 4 bits for {kv_heads} heads of {dim}")
-        if page_size % 8 or pages.shape[1] != kv_heads or pages.shape[2] != page_size * (dim + dim // 16) or not self._here(pages):
+        if page_size % 8 or pages.dtype is not torch.uint8 or pages.shape[1:] != (kv_heads, page_size * (dim + dim // 16)) or not self._here(pages):
             raise KernelError(f"{what}: the cell's pages do not hold {page_size} tokens of {kv_heads} heads of {dim} in 4 bits on {self.device}")
         return pages
 
     def _indices(self, tensor: torch.Tensor, shape: tuple, what: str) -> None:
-        if tensor.dtype != torch.int32 or tuple(tensor.shape) != shape or not self._here(tensor):
+        if tensor.dtype is not torch.int32 or tensor.shape != shape or not self._here(tensor):
             raise KernelError(f"{what}: int32 {list(shape)} on {self.device}")
+
+    def _packed_query_rows(self, qkv: torch.Tensor, layout, what: str) -> None:
+        if qkv.ndim != 2 or qkv.shape[1] != layout.stride or not self._here(qkv):
+            raise KernelError(f"{what}: rows of the layout's width on {self.device}")
 
     def store_packed(self, qkv, layout, batch, cell) -> None:
         """The keys and values of `qkv`'s rows (as `rotate_and_store` leaves them), rounded to 4 bits, into the cell's pages at the step's
@@ -1739,11 +1743,10 @@ class HipKernels:
         tokens, kv_heads, dim = qkv.shape[0], layout.num_kv_heads, layout.head_dim
         group = batch.groups[cell.group]
         pages = self._packed_cell(cell, kv_heads, dim, group.page_size, "store_packed")
-        if qkv.ndim != 2 or qkv.shape[1] != layout.stride or not self._here(qkv):
-            raise KernelError("store_packed: rows of the layout's width on the library's device")
+        self._packed_query_rows(qkv, layout, "store_packed")
         self._indices(group.slot_mapping, (tokens,), "store_packed: the step's slots")
         status = self._library_of("packed").llmserve_packed_store(
-            _pointer(qkv), _is_float(qkv), layout.stride, layout.num_heads * dim, tokens, kv_heads, dim, _pointer(pages), pages.shape[0], group.page_size,
+            _pointer(qkv), _is_float(qkv), qkv.shape[1], layout.num_heads * dim, tokens, kv_heads, dim, _pointer(pages), pages.shape[0], group.page_size,
             _pointer(group.slot_mapping), self._stream,
         )
         _check(status, "store_packed")
@@ -1751,14 +1754,12 @@ class HipKernels:
     def packed_rows(self, cell, slots: torch.Tensor, page_size: int) -> tuple[torch.Tensor, torch.Tensor]:
         """(keys, values) [n, kv_heads, dim] in the run dtype of what the cell's pages hold at `slots` int32 [n], exactly; zeros for a
         negative slot or one beyond the pages."""
-        need = cell.need
-        pages = self._packed_cell(cell, need.num_kv_heads, need.head_dim, page_size, "packed_rows")
-        self._indices(slots, (slots.numel(),), "packed_rows: slots")
-        both = self._empty((2, slots.shape[0], need.num_kv_heads, need.head_dim), self.dtype)
-        keys, values = both[0], both[1]
+        kv_heads, dim, rows = cell.need.num_kv_heads, cell.need.head_dim, slots.numel()
+        pages = self._packed_cell(cell, kv_heads, dim, page_size, "packed_rows")
+        self._indices(slots, (rows,), "packed_rows: slots")
+        keys, values = self._empty((2, rows, kv_heads, dim), self.dtype).unbind()
         status = self._library_of("packed").llmserve_packed_rows(
-            _pointer(pages), pages.shape[0], need.num_kv_heads, need.head_dim, page_size, _pointer(slots), slots.shape[0], _pointer(keys), _pointer(values),
-            _is_float(both), self._stream,
+            _pointer(pages), pages.shape[0], kv_heads, dim, page_size, _pointer(slots), rows, keys.data_ptr(), values.data_ptr(), _is_float(keys), self._stream,
         )
         _check(status, "packed_rows")
         return keys, values
@@ -1768,6 +1769,11 @@ class HipKernels:
         if key not in self._lazy:
             self._lazy[key] = _declared(load_module("packed_attention", {"HEAD_DIM": head_dim}))
         return self._lazy[key]
+
+    @staticmethod
+    def _all_portions(batch, group: int) -> bool:
+        """Whether no request of the step has few columns (a single token, or up to 16 query heads a kv head in all).  A captured step is replayed with others."""
+        return getattr(batch, "padded_to", None) is None and all(chunk.count > 1 and chunk.count * group > 16 for chunk in batch.chunks)
 
     @staticmethod
     def _packed_least(batch, dtype, tokens: int, requests: int, heads: int, kv_heads: int, window: int) -> tuple[int, int]:
@@ -1787,8 +1793,7 @@ class HipKernels:
         group = batch.groups[cell.group]
         pages = self._packed_cell(cell, kv_heads, dim, group.page_size, "paged_attention")
         requests = batch.context_lengths.shape[0]
-        if qkv.ndim != 2 or qkv.shape[1] != layout.stride or not self._here(qkv):
-            raise KernelError("paged_attention: rows of the layout's width on the library's device")
+        self._packed_query_rows(qkv, layout, "paged_attention")
         self._indices(group.block_tables, (requests, group.width), "paged_attention: block tables")
         self._indices(batch.query_start, (requests + 1,), "paged_attention: query starts")
         self._indices(batch.context_lengths, (requests,), "paged_attention: context lengths")
@@ -1800,7 +1805,7 @@ class HipKernels:
         status = library.llmserve_packed_attention(
             _pointer(qkv), _is_float(qkv), layout.stride, _pointer(out), out.shape[1], _pointer(spaces[0]), _pointer(spaces[1]), _pointer(pages), pages.shape[0],
             _pointer(group.block_tables), group.width, _pointer(batch.query_start), _pointer(batch.context_lengths), requests, tokens, heads, kv_heads, group.page_size, scale, window,
-            1 if most <= 1 else 3, few, many, self._stream,
+            1 if most <= 1 else 2 if self._all_portions(batch, heads // kv_heads) else 3, few, many, self._stream,
         )
         _check(status, "paged_attention over 4 bits")
         return out
@@ -1819,9 +1824,8 @@ class HipKernels:
         for name, tensor in (("slots", slots), ("starts", starts), ("counts", counts)):
             self._indices(tensor, (requests,), f"place_tokens: {name}")
         if out is None:
-            both = self._empty((2 * tokens + 2 * requests + 1 + groups * (tokens + requests * width),), torch.int32)
-            positions, sequence, query_start, contexts, mapping, compact = both.split(
-                (tokens, tokens, requests + 1, requests, groups * tokens, groups * requests * width))
+            sizes = (tokens, tokens, requests + 1, requests, groups * tokens, groups * requests * width)
+            positions, sequence, query_start, contexts, mapping, compact = self._empty((sum(sizes),), torch.int32).split_with_sizes(sizes)
             out = positions, sequence, query_start, contexts, mapping.view(groups, tokens), compact.view(groups, requests, width)
         else:
             shapes = ((tokens,), (tokens,), (requests + 1,), (requests,), (groups, tokens), (groups, requests, width))
@@ -1833,8 +1837,8 @@ class HipKernels:
                 raise KernelError("place_tokens: the tensors to fill are contiguous, a group's where there are several")
         positions, sequence, query_start, contexts, mapping, compact = out
         status = self._library_of("placing").llmserve_place_tokens(
-            _pointer(tables), groups, rows, blocks, _pointer(slots), _pointer(starts), _pointer(counts), requests, page_size, tokens, width, _pointer(positions),
-            _pointer(sequence), _pointer(query_start), _pointer(contexts), mapping.data_ptr(), mapping.stride(0), compact.data_ptr(), compact.stride(0), self._stream,
+            _pointer(tables), groups, rows, blocks, _pointer(slots), _pointer(starts), _pointer(counts), requests, page_size, tokens, width, positions.data_ptr(),
+            sequence.data_ptr(), query_start.data_ptr(), contexts.data_ptr(), mapping.data_ptr(), mapping.stride(0), compact.data_ptr(), compact.stride(0), self._stream,
         )
         _check(status, "place_tokens")
         return out
