@@ -84,6 +84,36 @@ def test_rows_packed_and_read_back(kernels, dtype, heads, kv_heads, dim, page, t
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("begins", [0, 3, 7])
+@pytest.mark.parametrize("tokens", [2600, 2601, 4093])
+def test_many_rows_packed_and_read_back(kernels, dtype, begins, tokens):
+    """Portions of two requests, from anywhere in a page, with rows that are stored nowhere among them, and slots in no order at the end."""
+    from llmserve_amd.cache import CacheCell
+    from llmserve_amd.parts import HeadLayout, PackedKeyValue
+
+    k, page, kv_heads, dim = kernels[dtype], 24, 3, 96
+    layout, need, generator = HeadLayout(5, kv_heads, dim, 11 * dim + 8), PackedKeyValue(kv_heads, dim), torch.Generator().manual_seed(tokens + begins)
+    pages = tokens // page + 40
+    cell = CacheCell(need, fields={"packed": torch.full((pages, kv_heads, need.page_bytes(page)), 255, dtype=torch.uint8, device="cuda")}, group=0)
+    order = torch.randperm(pages, generator=generator)
+    place = lambda first, positions: order[first + positions // page] * page + positions % page
+    one, other = begins + torch.arange(tokens // 2), 5 + torch.arange(tokens - tokens // 2 - 60)
+    given = torch.cat([place(0, one), place(tokens // 2 // page + 3, other), place(pages - 10, torch.randperm(200, generator=generator)[:60])])
+    given[[9, 10, 700, tokens - 1]] = torch.tensor([-1, pages * page, -5, -1])
+    rows = (torch.randn((tokens, layout.stride), generator=generator) * 3).to(dtype)
+    rows[33, 6 * dim] = math.inf
+    k.store_packed(rows.cuda(), layout, group_of(page, given.tolist()), cell)
+    keys, values = k.packed_rows(cell, given.int().cuda(), page)
+    want = kept(rows[:, 5 * dim:11 * dim].double().view(tokens, 2 * kv_heads, dim))
+    want[(given < 0) | (given >= pages * page)] = 0.0
+    same(keys, want[:, :kv_heads])
+    same(values, want[:, kv_heads:])
+    untouched = torch.ones(pages * page, dtype=torch.bool)
+    untouched[given[(given >= 0) & (given < pages * page)]] = False
+    assert all(torch.isnan(x).all() for x in k.packed_rows(cell, untouched.nonzero().flatten().int().cuda(), page))
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
 def test_blocks_that_are_no_numbers(kernels, dtype):
     """An infinity or a NaN makes its own block of 32 read as NaN and no other; the page's other tokens stay as they were."""
     from llmserve_amd.cache import CacheCell
