@@ -714,8 +714,8 @@ __global__ void __launch_bounds__(4 * WAVE) packed_join_kernel(T* out, int out_s
 // Many columns see the same keys: the matrix cores and the instructions that make codes bfloat16 bound these.  In bfloat16, at heads of a multiple of 64, a wave
 // takes 32 columns with v_mfma_f32_32x32x16_bf16, which does 1.8 PFLOP/s here where 16x16x32 does 1.1; a step's codes are made bfloat16 once for them.  Everything else is as
 // above: a lane takes D / 2 neighbouring elements of a key, keys are dealt to rows so that a lane ends with the weights of two pieces of eight neighbouring keys, and of the values it takes
-// D / 32 neighbouring elements of those keys.  (Tiles made bfloat16 once for four such waves, in LDS, take as many instructions a wave, the barriers and the way through LDS counted:
-// 2,048 tokens behind 30,000 keys at 12/2 heads took 480 us so.)
+// D / 32 neighbouring elements of those keys.  (Tiles made bfloat16 once for four such waves, in LDS, spare
+// a wave three quarters of that and cost barriers and the way through LDS: 2,048 tokens behind 30,000 keys at 12/2 heads took 480 us so, 564 as here, but a prompt of 2,047 59 and 42 here.)
 constexpr int PORTION_WAVES = 4, PORTION_THREADS = PORTION_WAVES * WAVE;
 constexpr int PORTION_UNIT = PORTION_WAVES * KEYS;  // keys
 constexpr int BEGINNING = 4;                  // units that a walk's beginning and end take as long as

@@ -1771,22 +1771,45 @@ class HipKernels:
         return self._lazy[key]
 
     @staticmethod
-    def _all_portions(batch, group: int) -> bool:
-        """Whether no request of the step has few columns (a single token, or up to 16 query heads a kv head in all).  A captured step is replayed with others."""
-        return getattr(batch, "padded_to", None) is None and all(chunk.count > 1 and chunk.count * group > 16 for chunk in batch.chunks)
+    def _packed_kinds(batch, group: int, tokens: int) -> tuple[int, int, int, int]:
+        """(1: no request has many columns, 2: none has few, 3; the longest context of those of few columns, of those of many; the latter's tokens).  Few are a
+        single token or up to 16 query heads a kv head in all.  A captured step is replayed with other requests: any of either kind."""
+        longest = batch.max_context_length
+        if batch.max_query_length <= 1:
+            return 1, longest, 0, 0
+        if getattr(batch, "padded_to", None) is not None:
+            return 3, longest, longest, tokens
+        known = batch.scratch.get(("packed kinds", group))
+        if known is not None:
+            return known
+        few = many = singles = 0
+        for chunk in batch.chunks:
+            end = chunk.start + chunk.count
+            if chunk.count > 1 and chunk.count * group > 16:
+                many = end if end > many else many
+            else:
+                few = end if end > few else few
+                singles += chunk.count
+        known = batch.scratch[("packed kinds", group)] = (1 if many == 0 else 2 if few == 0 else 3), few, many, tokens - singles
+        return known
 
     @staticmethod
-    def _packed_least(batch, dtype, tokens: int, requests: int, heads: int, kv_heads: int, window: int) -> tuple[int, int]:
+    def _packed_least(few: int, many: int, tokens: int, requests: int, heads: int, kv_heads: int, window: int) -> tuple[int, int]:
         """(units of 256 keys that a workgroup takes at least of walks over the keys of few columns, units of 128 keys of those of many): walks are cut anywhere.  0: every
-        walk is taken whole."""
+        walk is taken whole.  `few` and `many` are the longest contexts, `tokens` those of many columns."""
         group = heads // kv_heads
-        walk = min(batch.max_context_length, window + 31) if window else batch.max_context_length
+        if window:
+            few, many = min(few, window + 31), min(many, window + 31)
         pairs = requests * kv_heads * -(-group // 16)
-        few = 0 if walk <= 1024 or 22 * walk <= 50000 + 3 * pairs * walk // 10 else 4
-        most = batch.max_query_length
-        items = kv_heads * -(-tokens * group // 32)
-        many = 0 if most <= 1 or requests > 256 or items >= 1024 or walk <= 512 else 8
-        return few, many
+        few = 0 if few <= 1024 or 22 * few <= 50000 + 3 * pairs * few // 10 else 4
+        if many == 0 or requests > 256:
+            return few, 0
+        # Of many columns: whole, the 512 workgroups that the chip holds take 11.5 us for 1,000 keys of 32 columns each, 256 of them 8.25 (each alone on its unit);
+        # cut, the sum of all walks is what counts, 25 ns for 1,000 keys of a column's 32, and 18 us on top.  us, whole and cut: 12 heads on 2, 128 tokens
+        # behind 30,000 251 and 64, behind 2,000 27 and 30; 512 behind 10,000 93 and 75; 2,048 behind 30,000 562 and 573; 40 heads on 8, 512 behind 10,000 201 and 186.
+        whole, rest = divmod(kv_heads * -(-tokens * group // 32), 512)
+        spared = 11.5 * whole + (0.0 if rest == 0 else 8.25 if rest <= 256 else 11.5) - 0.025 * (512 * whole + rest)
+        return few, 8 if spared * many > 18000 else 0
 
     def _packed_attention(self, qkv, layout, batch, cell, scale: float, window: int | None, out):
         tokens, heads, kv_heads, dim = qkv.shape[0], layout.num_heads, layout.num_kv_heads, layout.head_dim
@@ -1799,13 +1822,14 @@ class HipKernels:
         self._indices(batch.context_lengths, (requests,), "paged_attention: context lengths")
         out = self._attention_out(qkv, layout, out)
         window = int(window or 0)
-        library, most = self._packed_library(dim), batch.max_query_length
-        few, many = self._packed_least(batch, qkv.dtype, tokens, requests, heads, kv_heads, window)
+        library = self._packed_library(dim)
+        kinds, few, many, of_many = self._packed_kinds(batch, heads // kv_heads, tokens)
+        few, many = self._packed_least(few, many, of_many, requests, heads, kv_heads, window)
         spaces = [self._empty((library.llmserve_packed_attention_workspace(kind),), torch.float32) if least else None for kind, least in ((0, few), (1, many))]
         status = library.llmserve_packed_attention(
             _pointer(qkv), _is_float(qkv), layout.stride, _pointer(out), out.shape[1], _pointer(spaces[0]), _pointer(spaces[1]), _pointer(pages), pages.shape[0],
             _pointer(group.block_tables), group.width, _pointer(batch.query_start), _pointer(batch.context_lengths), requests, tokens, heads, kv_heads, group.page_size, scale, window,
-            1 if most <= 1 else 2 if self._all_portions(batch, heads // kv_heads) else 3, few, many, self._stream,
+            kinds, few, many, self._stream,
         )
         _check(status, "paged_attention over 4 bits")
         return out
