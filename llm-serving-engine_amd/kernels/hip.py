@@ -1742,6 +1742,8 @@ class HipKernels:
         slots (a negative slot, or one beyond the pages: nowhere; every other slot once)."""
         tokens, kv_heads, dim = qkv.shape[0], layout.num_kv_heads, layout.head_dim
         group = batch.groups[cell.group]
+        if not cell.writable:
+            raise KernelError("store_packed: the cell is another run's to write")
         pages = self._packed_cell(cell, kv_heads, dim, group.page_size, "store_packed")
         self._packed_query_rows(qkv, layout, "store_packed")
         self._indices(group.slot_mapping, (tokens,), "store_packed: the step's slots")
@@ -1820,6 +1822,8 @@ class HipKernels:
         self._indices(group.block_tables, (requests, group.width), "paged_attention: block tables")
         self._indices(batch.query_start, (requests + 1,), "paged_attention: query starts")
         self._indices(batch.context_lengths, (requests,), "paged_attention: context lengths")
+        if out is not None and not self._here(out):
+            raise KernelError(f"paged_attention: the rows to write are on {self.device}")
         out = self._attention_out(qkv, layout, out)
         window = int(window or 0)
         library = self._packed_library(dim)
@@ -1841,7 +1845,9 @@ class HipKernels:
         width]), int32, or `out`, six such tensors, filled.  A token without a page is mapped to -1; a table row is -1 behind the request's last page.  A
         request whose slot is not a row of the tables pads the step: its tokens are at position 0 and stored nowhere, its context is one token, its table
         row 0.  Where the counts add up to less than `tokens`, the rows behind the last are such tokens of the last request; to more: what is too many is left out."""
-        requests = slots.shape[0]
+        requests = slots.numel()
+        if not 0 <= tokens < 1 << 30 or not 0 < width < 1 << 30:
+            raise KernelError("place_tokens: 0 to 2^30 tokens, tables of 1 to 2^30 pages")
         if tables.ndim != 3 or tables.dtype != torch.int32 or not self._here(tables):
             raise KernelError(f"place_tokens: tables are int32 [groups, rows, blocks] on {self.device}")
         groups, rows, blocks = tables.shape

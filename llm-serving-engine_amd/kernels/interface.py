@@ -307,6 +307,24 @@ class Kernels(Protocol):
         + shared where no gates are given), float32 [T, hidden]; `shared` may be partial sums [parts, T, hidden]; the inner rows are rounded to the run dtype between the
         two products."""
 
+    # ------------------------------------------------------------------ keys and values in 4 bits, index arrays on the device
+
+    # Over a cell of `PackedKeyValue` (`CacheConfig.packed`), `rotate_and_store` rounds the rows' keys and values to 4 bits and `paged_attention` reads those:
+    # softmax(q k^T scale) v over what the pages stand for, with or without a window, without changes of the scores.
+
+    def store_packed(self, qkv: torch.Tensor, layout: HeadLayout, batch: Any, cell: Any) -> None:
+        """Keys and values of `qkv`'s rows, as they are, rounded to 4 bits into the cell's pages at the step's slots."""
+
+    def packed_rows(self, cell: Any, slots: torch.Tensor, page_size: int) -> tuple[torch.Tensor, torch.Tensor]:
+        """(keys, values) [n, kv_heads, dim] in the run dtype: what the cell's pages stand for at `slots` int32 [n], exactly; zeros for a slot that is none."""
+
+    def place_tokens(
+        self, tables: torch.Tensor, slots: torch.Tensor, starts: torch.Tensor, counts: torch.Tensor, page_size: int, tokens: int, width: int,
+        out: tuple[torch.Tensor, ...] | None = None,
+    ) -> tuple[torch.Tensor, ...]:
+        """A step's (positions, token's request, query starts, context lengths, slot mapping [groups, tokens], block tables [groups, B, width]) from its requests'
+        rows in `tables` [groups, rows, blocks], cached lengths and token counts.  A library without it has the runner pack them on the host."""
+
     # ------------------------------------------------------------------ copies of the stream, a diagonal recurrence, weighted sums
 
     def stream_copies(self, hidden: torch.Tensor, copies: int, scale: float) -> torch.Tensor:
