@@ -183,9 +183,82 @@ __device__ __forceinline__ void ask_step(unsigned char* stage, const unsigned ch
   }
 }
 
+// Behind a step's last product: the compiler may begin the next block of instructions with moves of the sums (it did, from accumulator registers, at heads wider than 128), and
+// keeps the distance that a product's result needs (8 instructions, 12 of the 32 x 32 ones) within a block only.
+__device__ __forceinline__ void products_done() {
+  __builtin_amdgcn_sched_barrier(0);
+  asm volatile("s_nop 15" ::: "memory");
+  __builtin_amdgcn_sched_barrier(0);
+}
+
 template <int N> __device__ __forceinline__ void wait_for_asked() { asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory"); }
 
-// A step's codes and powers out of LDS.  The reads are written out, with the wait behind them: the compiler would have them wait for all that has been asked for.
+// A step's codes and powers out of LDS.  The reads are written out, with the wait behind them: the compiler would have them wait for all that has been asked for.  A block of them ends
+// with its wait, so that no register is moved, or given to something else, before what is read into it has come.
+#define WORDS_1 "ds_read_b32 %[w0], %[keys]\n\t"
+#define WORDS_2 WORDS_1 "ds_read_b32 %[w1], %[keys] offset:4\n\t"
+#define WORDS_3 WORDS_2 "ds_read_b32 %[w2], %[keys] offset:8\n\t"
+#define WORDS_4 WORDS_3 "ds_read_b32 %[w3], %[keys] offset:12\n\t"
+#define WORDS_5 WORDS_4 "ds_read_b32 %[w4], %[keys] offset:16\n\t"
+#define WORDS_6 WORDS_5 "ds_read_b32 %[w5], %[keys] offset:20\n\t"
+#define WORDS_7 WORDS_6 "ds_read_b32 %[w6], %[keys] offset:24\n\t"
+#define WORDS_8 WORDS_7 "ds_read_b32 %[w7], %[keys] offset:28\n\t"
+#define BYTES_1 "ds_read_u8 %[b0], %[a0]\n\t"
+#define BYTES_2 BYTES_1 "ds_read_u8 %[b1], %[a1]\n\t"
+#define BYTES_3 BYTES_2 "ds_read_u8 %[b2], %[a2]\n\t"
+#define BYTES_5 BYTES_3 "ds_read_u8 %[b3], %[a3]\n\tds_read_u8 %[b4], %[a4]\n\t"
+#define BYTES_6 BYTES_5 "ds_read_u8 %[b5], %[a5]\n\t"
+#define BYTES_7 BYTES_6 "ds_read_u8 %[b6], %[a6]\n\t"
+#define TO_WORDS_1 [w0] "=&v"(words[0])
+#define TO_WORDS_2 TO_WORDS_1, [w1] "=&v"(words[1])
+#define TO_WORDS_3 TO_WORDS_2, [w2] "=&v"(words[2])
+#define TO_WORDS_4 TO_WORDS_3, [w3] "=&v"(words[3])
+#define TO_WORDS_5 TO_WORDS_4, [w4] "=&v"(words[4])
+#define TO_WORDS_6 TO_WORDS_5, [w5] "=&v"(words[5])
+#define TO_WORDS_7 TO_WORDS_6, [w6] "=&v"(words[6])
+#define TO_WORDS_8 TO_WORDS_7, [w7] "=&v"(words[7])
+#define TO_BYTES_1 [b0] "=&v"(bytes[0])
+#define TO_BYTES_2 TO_BYTES_1, [b1] "=&v"(bytes[1])
+#define TO_BYTES_3 TO_BYTES_2, [b2] "=&v"(bytes[2])
+#define TO_BYTES_5 TO_BYTES_3, [b3] "=&v"(bytes[3]), [b4] "=&v"(bytes[4])
+#define TO_BYTES_6 TO_BYTES_5, [b5] "=&v"(bytes[5])
+#define TO_BYTES_7 TO_BYTES_6, [b6] "=&v"(bytes[6])
+#define AT_1 [a0] "v"(at[0])
+#define AT_2 AT_1, [a1] "v"(at[1])
+#define AT_3 AT_2, [a2] "v"(at[2])
+#define AT_5 AT_3, [a3] "v"(at[3]), [a4] "v"(at[4])
+#define AT_6 AT_5, [a5] "v"(at[5])
+#define AT_7 AT_6, [a6] "v"(at[6])
+#define READ_KEY(w, b) asm volatile(WORDS_##w BYTES_##b "s_waitcnt lgkmcnt(0)" : TO_WORDS_##w, TO_BYTES_##b : [keys] "v"(keys), AT_##b : "memory")
+template <int W, int B> __device__ __forceinline__ void read_key(unsigned (&words)[W], unsigned (&bytes)[B], unsigned keys, const unsigned (&at)[B]) {
+  if constexpr (W == 1 && B == 1) READ_KEY(1, 1);
+  else if constexpr (W == 2 && B == 1) READ_KEY(2, 1);
+  else if constexpr (W == 3 && B == 3) READ_KEY(3, 3);
+  else if constexpr (W == 5 && B == 5) READ_KEY(5, 5);
+  else if constexpr (W == 6 && B == 6) READ_KEY(6, 6);
+  else if constexpr (W == 7 && B == 7) READ_KEY(7, 7);
+  else {
+    static_assert(W == 8 && B == 2, "heads of 32 to 256 in steps of 32, but for 128");
+    READ_KEY(8, 2);
+  }
+}
+
+#define VALUE(i) "ds_read_b128 %[l" #i "], %[v" #i "]\n\tds_read_b128 %[h" #i "], %[v" #i "] offset:16\n\tds_read_b64 %[b" #i "], %[a" #i "]\n\t"
+#define TO_VALUE(i) [l##i] "=&v"(low[i]), [h##i] "=&v"(high[i]), [b##i] "=&v"(powers[i])
+#define VALUE_AT(i) [v##i] "v"(values[i]), [a##i] "v"(at[i])
+// N times eight keys' codes of a granule, and their powers
+template <int N> __device__ __forceinline__ void read_values(u32x4 (&low)[N], u32x4 (&high)[N], u32x2 (&powers)[N], const unsigned (&values)[N], const unsigned (&at)[N]) {
+  if constexpr (N == 1) asm volatile(VALUE(0) "s_waitcnt lgkmcnt(0)" : TO_VALUE(0) : VALUE_AT(0) : "memory");
+  else if constexpr (N == 2) asm volatile(VALUE(0) VALUE(1) "s_waitcnt lgkmcnt(0)" : TO_VALUE(0), TO_VALUE(1) : VALUE_AT(0), VALUE_AT(1) : "memory");
+  else if constexpr (N == 3)
+    asm volatile(VALUE(0) VALUE(1) VALUE(2) "s_waitcnt lgkmcnt(0)" : TO_VALUE(0), TO_VALUE(1), TO_VALUE(2) : VALUE_AT(0), VALUE_AT(1), VALUE_AT(2) : "memory");
+  else {
+    static_assert(N == 4, "three chunks, or two of two pieces");
+    asm volatile(VALUE(0) VALUE(1) VALUE(2) VALUE(3) "s_waitcnt lgkmcnt(0)"
+                 : TO_VALUE(0), TO_VALUE(1), TO_VALUE(2), TO_VALUE(3) : VALUE_AT(0), VALUE_AT(1), VALUE_AT(2), VALUE_AT(3) : "memory");
+  }
+}
+
 __device__ __forceinline__ void read_step(Step& s, const unsigned char* stage) {
   const unsigned lane = threadIdx.x % WAVE, r = lane & 15, g = lane >> 4;
   const unsigned at = (unsigned)(size_t)(const unsigned char __attribute__((address_space(3)))*)stage;
@@ -204,34 +277,27 @@ __device__ __forceinline__ void read_step(Step& s, const unsigned char* stage) {
       s.keys[1][i] = k1[i];
     }
   } else {
+    unsigned powers[KEY_POWERS];
 #pragma unroll
-    for (int t = 0; t < 2; ++t) {
+    for (int i = 0; i < KEY_POWERS; ++i) powers[i] = key_powers + (D % 128 == 0 ? g * KEY_POWERS + i : (g * SLICES + i) / 4);
+    read_key(s.keys[0], s.key_powers[0], keys, powers);
 #pragma unroll
-      for (int i = 0; i < SLICES; ++i) asm volatile("ds_read_b32 %0, %1 offset:%2" : "=v"(s.keys[t][i]) : "v"(keys), "n"(t * 2 * D + i * 4) : "memory");
-#pragma unroll
-      for (int i = 0; i < KEY_POWERS; ++i) {
-        const unsigned block = D % 128 == 0 ? g * KEY_POWERS + i : (g * SLICES + i) / 4;
-        asm volatile("ds_read_u8 %0, %1 offset:%2" : "=v"(s.key_powers[t][i]) : "v"(key_powers + block), "n"(t * (D / 8)) : "memory");
-      }
-    }
+    for (int i = 0; i < KEY_POWERS; ++i) powers[i] += D / 8;
+    read_key(s.keys[1], s.key_powers[1], keys + 2 * D, powers);
+    u32x4 low[CHUNKS], high[CHUNKS];
+    unsigned values[CHUNKS], value_powers[CHUNKS];
 #pragma unroll
     for (int c = 0; c < CHUNKS; ++c) {
-      const unsigned granule = chunk_first(c) / 8 + r * chunk_width(c) / 128, value = at + g * PIECE + 4 * D + granule * 32, power = at + 4 * PIECE + g * (D / 2) + D / 4 + granule / 4 * 8;
-      asm volatile("ds_read_b128 %0, %1" : "=v"(s.values[c][0]) : "v"(value) : "memory");
-      asm volatile("ds_read_b128 %0, %1 offset:16" : "=v"(s.values[c][1]) : "v"(value) : "memory");
-      asm volatile("ds_read_b64 %0, %1" : "=v"(s.value_powers[c]) : "v"(power) : "memory");
+      const unsigned granule = chunk_first(c) / 8 + r * chunk_width(c) / 128;
+      values[c] = at + g * PIECE + 4 * D + granule * 32;
+      value_powers[c] = at + 4 * PIECE + g * (D / 2) + D / 4 + granule / 4 * 8;
     }
-    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-    // used only after the wait
+    read_values(low, high, s.value_powers, values, value_powers);
 #pragma unroll
-    for (int t = 0; t < 2; ++t) {
-#pragma unroll
-      for (int i = 0; i < SLICES; ++i) asm volatile("" : "+v"(s.keys[t][i]));
-#pragma unroll
-      for (int i = 0; i < KEY_POWERS; ++i) asm volatile("" : "+v"(s.key_powers[t][i]));
+    for (int c = 0; c < CHUNKS; ++c) {
+      s.values[c][0] = low[c];
+      s.values[c][1] = high[c];
     }
-#pragma unroll
-    for (int c = 0; c < CHUNKS; ++c) asm volatile("" : "+v"(s.values[c][0]), "+v"(s.values[c][1]), "+v"(s.value_powers[c]));
   }
 }
 
@@ -482,11 +548,13 @@ __device__ __forceinline__ void walk_keys(Cols& columns, const T* q, int q_strid
       Taken now;
       next_step(now);
       take_step<false>(columns, now, w, item, base);
+      products_done();
     }
     if (base >= end) break;
     Taken now;
     next_step(now);
     take_step<true>(columns, now, w, item, base);
+    products_done();
   }
 }
 
@@ -714,8 +782,7 @@ __global__ void __launch_bounds__(4 * WAVE) packed_join_kernel(T* out, int out_s
 // Many columns see the same keys: the matrix cores and the instructions that make codes bfloat16 bound these.  In bfloat16, at heads of a multiple of 64, a wave
 // takes 32 columns with v_mfma_f32_32x32x16_bf16, which does 1.8 PFLOP/s here where 16x16x32 does 1.1; a step's codes are made bfloat16 once for them.  Everything else is as
 // above: a lane takes D / 2 neighbouring elements of a key, keys are dealt to rows so that a lane ends with the weights of two pieces of eight neighbouring keys, and of the values it takes
-// D / 32 neighbouring elements of those keys.  (Tiles made bfloat16 once for four such waves, in LDS, spare
-// a wave three quarters of that and cost barriers and the way through LDS: 2,048 tokens behind 30,000 keys at 12/2 heads took 480 us so, 564 as here, but a prompt of 2,047 59 and 42 here.)
+// D / 32 neighbouring elements of those keys.  (Where columns are many, tiles are shared: below.)
 constexpr int PORTION_WAVES = 4, PORTION_THREADS = PORTION_WAVES * WAVE;
 constexpr int PORTION_UNIT = PORTION_WAVES * KEYS;  // keys
 constexpr int BEGINNING = 4;                  // units that a walk's beginning and end take as long as
@@ -741,43 +808,52 @@ struct WideColumns {                          // a wave's 32
 
 __device__ __forceinline__ f32x16 multiply(const Eight& a, const Eight& b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a.v, b.v, c, 0, 0, 0); }
 
+// N blocks of a key, and their powers
+#define BLOCK(i, o, p) "ds_read_b128 %[k" #i "], %[keys] offset:" #o "\n\tds_read_u8 %[b" #i "], %[at] offset:" #p "\n\t"
+#define TO_BLOCK(i) [k##i] "=&v"(blocks[i]), [b##i] "=&v"(powers[i])
+template <int N> __device__ __forceinline__ void read_blocks(u32x4 (&blocks)[N], unsigned (&powers)[N], unsigned keys, unsigned at) {
+  if constexpr (N == 1) asm volatile(BLOCK(0, 0, 0) "s_waitcnt lgkmcnt(0)" : TO_BLOCK(0) : [keys] "v"(keys), [at] "v"(at) : "memory");
+  else if constexpr (N == 3)
+    asm volatile(BLOCK(0, 0, 0) BLOCK(1, 16, 1) BLOCK(2, 32, 2) "s_waitcnt lgkmcnt(0)" : TO_BLOCK(0), TO_BLOCK(1), TO_BLOCK(2) : [keys] "v"(keys), [at] "v"(at) : "memory");
+  else {
+    static_assert(N == 4, "heads of 64, 192 and 256");
+    asm volatile(BLOCK(0, 0, 0) BLOCK(1, 16, 1) BLOCK(2, 32, 2) BLOCK(3, 48, 3) "s_waitcnt lgkmcnt(0)"
+                 : TO_BLOCK(0), TO_BLOCK(1), TO_BLOCK(2), TO_BLOCK(3) : [keys] "v"(keys), [at] "v"(at) : "memory");
+  }
+}
+
 __device__ __forceinline__ void read_step(WideStep& s, const unsigned char* stage) {
   const unsigned lane = threadIdx.x % WAVE, n = lane & 31, h = lane >> 5, at = (unsigned)(size_t)(const unsigned char __attribute__((address_space(3)))*)stage;
   const unsigned row = (n & 0x13) | ((n & 4) << 1) | ((n & 8) >> 1);  // the key that row n of the first product is
   const unsigned keys = at + (row >> 3) * PIECE + (row & 7) * (D / 2) + h * (D / 4), key_powers = at + 4 * PIECE + (row >> 3) * (D / 2) + (row & 7) * (D / 32) + h * (D / 64);
-  if constexpr (D == 128) {
-    const unsigned values = at + h * PIECE + 4 * D + (n >> 1) * 32, value_powers = at + 4 * PIECE + h * (D / 2) + D / 4 + (n >> 3) * 8;
-    asm volatile(
-        "ds_read_b128 %0, %10\n\tds_read_b128 %1, %10 offset:16\n\tds_read_u8 %2, %11\n\tds_read_u8 %3, %11 offset:1\n\tds_read_b128 %4, %12\n\tds_read_b128 %5, %12 offset:16\n\t"
-        "ds_read_b64 %8, %13\n\tds_read_b128 %6, %12 offset:%14\n\tds_read_b128 %7, %12 offset:%15\n\tds_read_b64 %9, %13 offset:%16\n\ts_waitcnt lgkmcnt(0)"
-        : "=&v"(s.keys[0]), "=&v"(s.keys[1]), "=&v"(s.key_powers[0]), "=&v"(s.key_powers[1]), "=&v"(s.values[0][0][0]), "=&v"(s.values[0][0][1]), "=&v"(s.values[1][0][0]),
-          "=&v"(s.values[1][0][1]), "=&v"(s.value_powers[0][0]), "=&v"(s.value_powers[1][0])
-        : "v"(keys), "v"(key_powers), "v"(values), "v"(value_powers), "n"(2 * PIECE), "n"(2 * PIECE + 16), "n"(D)
-        : "memory");
-  } else {
+#if HEAD_DIM == 128
+  const unsigned values = at + h * PIECE + 4 * D + (n >> 1) * 32, value_powers = at + 4 * PIECE + h * (D / 2) + D / 4 + (n >> 3) * 8;
+  asm volatile(
+      "ds_read_b128 %0, %10\n\tds_read_b128 %1, %10 offset:16\n\tds_read_u8 %2, %11\n\tds_read_u8 %3, %11 offset:1\n\tds_read_b128 %4, %12\n\tds_read_b128 %5, %12 offset:16\n\t"
+      "ds_read_b64 %8, %13\n\tds_read_b128 %6, %12 offset:%14\n\tds_read_b128 %7, %12 offset:%15\n\tds_read_b64 %9, %13 offset:%16\n\ts_waitcnt lgkmcnt(0)"
+      : "=&v"(s.keys[0]), "=&v"(s.keys[1]), "=&v"(s.key_powers[0]), "=&v"(s.key_powers[1]), "=&v"(s.values[0][0][0]), "=&v"(s.values[0][0][1]), "=&v"(s.values[1][0][0]),
+        "=&v"(s.values[1][0][1]), "=&v"(s.value_powers[0][0]), "=&v"(s.value_powers[1][0])
+      : "v"(keys), "v"(key_powers), "v"(values), "v"(value_powers), "n"(2 * PIECE), "n"(2 * PIECE + 16), "n"(D)
+      : "memory");
+#elif HEAD_DIM % 64 == 0
+  read_blocks(s.keys, s.key_powers, keys, key_powers);
+  u32x4 low[2 * CHUNKS], high[2 * CHUNKS];
+  u32x2 powers[2 * CHUNKS];
+  unsigned values[2 * CHUNKS], value_powers[2 * CHUNKS];
 #pragma unroll
-    for (int i = 0; i < HALF_BLOCKS; ++i) {
-      asm volatile("ds_read_b128 %0, %1 offset:%2" : "=v"(s.keys[i]) : "v"(keys), "n"(i * 16) : "memory");
-      asm volatile("ds_read_u8 %0, %1 offset:%2" : "=v"(s.key_powers[i]) : "v"(key_powers), "n"(i) : "memory");
-    }
-#pragma unroll
-    for (int u = 0; u < 2; ++u)
-#pragma unroll
-      for (int c = 0; c < CHUNKS; ++c) {
-        const unsigned granule = chunk_first(c) / 8 + n * chunk_width(c) / 256, value = at + (2 * u + h) * PIECE + 4 * D + granule * 32;
-        asm volatile("ds_read_b128 %0, %1" : "=v"(s.values[u][c][0]) : "v"(value) : "memory");
-        asm volatile("ds_read_b128 %0, %1 offset:16" : "=v"(s.values[u][c][1]) : "v"(value) : "memory");
-        asm volatile("ds_read_b64 %0, %1" : "=v"(s.value_powers[u][c]) : "v"(at + 4 * PIECE + (2 * u + h) * (D / 2) + D / 4 + granule / 4 * 8) : "memory");
-      }
-    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-    // used only after the wait
-#pragma unroll
-    for (int i = 0; i < HALF_BLOCKS; ++i) asm volatile("" : "+v"(s.keys[i]), "+v"(s.key_powers[i]));
-#pragma unroll
-    for (int u = 0; u < 2; ++u)
-#pragma unroll
-      for (int c = 0; c < CHUNKS; ++c) asm volatile("" : "+v"(s.values[u][c][0]), "+v"(s.values[u][c][1]), "+v"(s.value_powers[u][c]));
+  for (int i = 0; i < 2 * CHUNKS; ++i) {
+    const unsigned c = i % CHUNKS, piece = 2 * (i / CHUNKS) + h, granule = chunk_first(c) / 8 + n * chunk_width(c) / 256;
+    values[i] = at + piece * PIECE + 4 * D + granule * 32;
+    value_powers[i] = at + 4 * PIECE + piece * (D / 2) + D / 4 + granule / 4 * 8;
   }
+  read_values(low, high, powers, values, value_powers);
+#pragma unroll
+  for (int i = 0; i < 2 * CHUNKS; ++i) {
+    s.values[i / CHUNKS][i % CHUNKS][0] = low[i];
+    s.values[i / CHUNKS][i % CHUNKS][1] = high[i];
+    s.value_powers[i / CHUNKS][i % CHUNKS] = powers[i];
+  }
+#endif
 }
 
 template <bool EDGE> __device__ __forceinline__ void take_step(WideColumns& columns, const WideStep& now, const Walk& w, const Item& item, int base) {
@@ -959,17 +1035,18 @@ template <typename T> struct PortionOf<T, true> {
   typedef WideStep Taken;
 };
 
-__device__ __forceinline__ int portion_units(const Item& item) { return BEGINNING + (item.to - item.from + PORTION_UNIT - 1) / PORTION_UNIT; }
+// The walks of a kernel of portions: whole ones, the workgroup's own, or runs of all walks' units, which lie behind each other (up to 256 requests, one a thread).  A unit is UNIT keys from a multiple
+// of ALIGN on, a walk's beginning and end take as long as BEGINS units.  take(item, kv head, the keys from, to, where to leave a part or null).
+struct Shares {
+  int item_ends[PORTION_THREADS], ends[PORTION_THREADS], wave_sums[2][PORTION_WAVES];
+  Request held[PORTION_THREADS];
+};
 
-template <typename T>
-__global__ void __launch_bounds__(PORTION_THREADS, D <= 128 ? 2 : 1) packed_portions_kernel(const T* q, int q_stride, T* out, int out_stride, const unsigned char* pages, Walk w, Streams streams, int items, int whole) {
-  constexpr int COLUMNS = PORTION_COLUMNS<T>;
-  __shared__ __attribute__((aligned(16))) unsigned char memory[memory_of<PORTION_WAVES>()];
-  __shared__ int item_ends[PORTION_THREADS], ends[PORTION_THREADS], wave_sums[2][PORTION_WAVES];
-  __shared__ Request held[PORTION_THREADS];
+template <int COLUMNS, int UNIT, int ALIGN, int BEGINS, typename Take>
+__device__ __forceinline__ void take_walks(const Walk& w, const Streams& streams, int items, Shares& shares, Take take) {
   const int lane = threadIdx.x % WAVE, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / WAVE), group = w.heads / w.kv_heads;
-
-  // where the requests' items end, then where the items' units end (no more requests than threads; a run of items a thread)
+  const auto units_of = [&](const Item& item) { return BEGINS + (item.to - item.from / ALIGN * ALIGN + UNIT - 1) / UNIT; };
+  // where the requests' items end, then where the items' units end (a run of items a thread)
   const auto added_up = [&](int mine, int* sums) {
 #pragma unroll
     for (int step = 1; step < WAVE; step <<= 1) {
@@ -986,22 +1063,22 @@ __global__ void __launch_bounds__(PORTION_THREADS, D <= 128 ? 2 : 1) packed_port
     int low = 0, high = PORTION_THREADS - 1;
     while (low < high) {
       const int middle = (low + high) / 2;
-      if (item_ends[middle] > index) high = middle;
+      if (shares.item_ends[middle] > index) high = middle;
       else low = middle + 1;
     }
-    return make_item(w, low, held[low], (index - (low > 0 ? item_ends[low - 1] : 0)) * COLUMNS, COLUMNS, item);
+    return make_item(w, low, shares.held[low], (index - (low > 0 ? shares.item_ends[low - 1] : 0)) * COLUMNS, COLUMNS, item);
   };
   // the walk that a unit lies in, and where in it: kv head, unit of it, units
   const auto walk_at = [&](int at, Item& item, int& kv_head, int& unit, int& each) {
     int low = 0, high = PORTION_THREADS - 1;
     while (low < high) {
       const int middle = (low + high) / 2;
-      if (ends[middle] > at) high = middle;
+      if (shares.ends[middle] > at) high = middle;
       else low = middle + 1;
     }
-    int index = __builtin_amdgcn_readfirstlane(low) * run, inside = __builtin_amdgcn_readfirstlane(at - (low > 0 ? ends[low - 1] : 0));
+    int index = __builtin_amdgcn_readfirstlane(low) * run, inside = __builtin_amdgcn_readfirstlane(at - (low > 0 ? shares.ends[low - 1] : 0));
     for (; index < all_items; ++index) {
-      each = __builtin_amdgcn_readfirstlane(item_at(index, item) ? portion_units(item) : 0);
+      each = __builtin_amdgcn_readfirstlane(item_at(index, item) ? units_of(item) : 0);
       if (inside < each * w.kv_heads) break;
       inside -= each * w.kv_heads;
     }
@@ -1013,23 +1090,23 @@ __global__ void __launch_bounds__(PORTION_THREADS, D <= 128 ? 2 : 1) packed_port
   if (streams.least > 0) {
     int count = 0;
     if ((int)threadIdx.x < w.requests) {
-      held[threadIdx.x] = load_request(w, threadIdx.x);
-      const int tokens = held[threadIdx.x].count;
+      shares.held[threadIdx.x] = load_request(w, threadIdx.x);
+      const int tokens = shares.held[threadIdx.x].count;
       count = few_columns(tokens, group) ? 0 : (max(tokens, 0) * group + COLUMNS - 1) / COLUMNS;
     }
-    item_ends[threadIdx.x] = added_up(count, wave_sums[0]);
+    shares.item_ends[threadIdx.x] = added_up(count, shares.wave_sums[0]);
     __syncthreads();
-    all_items = __builtin_amdgcn_readfirstlane(item_ends[PORTION_THREADS - 1]);
+    all_items = __builtin_amdgcn_readfirstlane(shares.item_ends[PORTION_THREADS - 1]);
     run = (all_items + PORTION_THREADS - 1) / PORTION_THREADS;
     int units = 0;
     for (int i = threadIdx.x * run; i < min((int)(threadIdx.x + 1) * run, all_items); ++i) {
       Item item;
-      if (item_at(i, item)) units += portion_units(item) * w.kv_heads;
+      if (item_at(i, item)) units += units_of(item) * w.kv_heads;
     }
-    ends[threadIdx.x] = added_up(units, wave_sums[1]);
+    shares.ends[threadIdx.x] = added_up(units, shares.wave_sums[1]);
     __syncthreads();
-    total = __builtin_amdgcn_readfirstlane(ends[PORTION_THREADS - 1]);
-    share = max(max(streams.least, BEGINNING + 1), (total + (int)gridDim.x - 1) / (int)gridDim.x);
+    total = __builtin_amdgcn_readfirstlane(shares.ends[PORTION_THREADS - 1]);
+    share = max(max(streams.least, BEGINS + 1), (total + (int)gridDim.x - 1) / (int)gridDim.x);
     first = min(blockIdx.x * (long)share, (long)total);
     last = min(first + share, total);
     if (threadIdx.x == 0) streams.cuts[blockIdx.x].parts = 0;
@@ -1037,8 +1114,8 @@ __global__ void __launch_bounds__(PORTION_THREADS, D <= 128 ? 2 : 1) packed_port
     if (first < last) {
       Item item;
       int kv_head, unit, each;
-      if (walk_at(first, item, kv_head, unit, each) && unit <= BEGINNING) first -= unit;
-      if (last < total && walk_at(last, item, kv_head, unit, each) && unit <= BEGINNING) last -= unit;
+      if (walk_at(first, item, kv_head, unit, each) && unit <= BEGINS) first -= unit;
+      if (last < total && walk_at(last, item, kv_head, unit, each) && unit <= BEGINS) last -= unit;
     }
   }
   for (int at = first; at < last;) {
@@ -1047,12 +1124,12 @@ __global__ void __launch_bounds__(PORTION_THREADS, D <= 128 ? 2 : 1) packed_port
     if (streams.least == 0) {                 // a walk whole; the longest begin first: a request's last columns walk most keys
       if (!find_item(w, items - 1 - blockIdx.x / w.kv_heads, COLUMNS, item)) return;
       kv_head = blockIdx.x % w.kv_heads;
-      begin = item.from;
+      begin = item.from / ALIGN * ALIGN;
     } else {
       if (!walk_at(at, item, kv_head, unit, each)) break;
       taken = min(each - unit, last - at);
       place = at == first ? 0 : 1;
-      begin = item.from + max(unit - BEGINNING, 0) * PORTION_UNIT;
+      begin = item.from / ALIGN * ALIGN + max(unit - BEGINS, 0) * UNIT;
     }
     item.request = __builtin_amdgcn_readfirstlane(item.request);
     item.first_row = __builtin_amdgcn_readfirstlane(item.first_row);
@@ -1062,10 +1139,22 @@ __global__ void __launch_bounds__(PORTION_THREADS, D <= 128 ? 2 : 1) packed_port
     item.last_position = __builtin_amdgcn_readfirstlane(item.last_position);
     item.from = __builtin_amdgcn_readfirstlane(item.from);
     item.to = __builtin_amdgcn_readfirstlane(item.to);
-    begin = __builtin_amdgcn_readfirstlane(begin);
     const bool cut = taken < each;
-    const int end = streams.least == 0 || unit + taken == each ? item.to : item.from + (unit + taken - BEGINNING) * PORTION_UNIT;
-    float* part = cut ? streams.parts + ((size_t)blockIdx.x * 2 + place) * PORTION_PART<T> : nullptr;
+    take(item, kv_head, __builtin_amdgcn_readfirstlane(begin), streams.least == 0 || unit + taken == each ? item.to : item.from / ALIGN * ALIGN + (unit + taken - BEGINS) * UNIT,
+         cut ? streams.parts + ((size_t)blockIdx.x * 2 + place) * (COLUMNS * (D + 4)) : nullptr);
+    if (cut && unit == 0 && threadIdx.x == 0)
+      streams.cuts[blockIdx.x] = {item.first_row, group, item.first, item.columns, kv_head, (at + each - 1) / share - (int)blockIdx.x + 1, place, 0};
+    at += taken;
+  }
+}
+
+template <typename T>
+__global__ void __launch_bounds__(PORTION_THREADS, D <= 128 ? 2 : 1) packed_portions_kernel(const T* q, int q_stride, T* out, int out_stride, const unsigned char* pages, Walk w, Streams streams, int items, int whole) {
+  constexpr int COLUMNS = PORTION_COLUMNS<T>;
+  __shared__ __attribute__((aligned(16))) unsigned char memory[memory_of<PORTION_WAVES>()];
+  __shared__ Shares shares;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / WAVE);
+  take_walks<COLUMNS, PORTION_UNIT, KEYS, BEGINNING>(w, streams, items, shares, [&](const Item& item, int kv_head, int begin, int end, float* part) {
     typename PortionOf<T, WIDE<T>>::Cols columns;
     __syncthreads();                          // (what a walk before this one left in LDS has been read)
     walk_keys<T, typename PortionOf<T, WIDE<T>>::Taken, PORTION_WAVES>(columns, q, q_stride, pages, w, item, kv_head, whole, begin, end, wave, memory + wave * (STAGES * STAGE));
@@ -1078,10 +1167,323 @@ __global__ void __launch_bounds__(PORTION_THREADS, D <= 128 ? 2 : 1) packed_port
         write_four(out + (size_t)(item.first_row + token) * out_stride + head * D + d, result * (1.f / weights));
       }
     });
-    if (cut && unit == 0 && threadIdx.x == 0)
-      streams.cuts[blockIdx.x] = {item.first_row, group, item.first, item.columns, kv_head, (at + each - 1) / share - (int)blockIdx.x + 1, place, 0};
-    at += taken;
+  });
+}
+
+// ---------------------------------------------------------------------------------------------------------------- bfloat16 portions
+//
+// The same for portions that have columns enough to fill the chip with 128 a workgroup, 32 a wave: the instructions that make a key bfloat16, which every wave above does for 32 columns, are shared.
+// Tiles of 64 keys and values are made bfloat16 in LDS once for the four waves, the next tile's while they multiply with this one's:
+//   S^T = K Q^T, O^T += V^T P^T with v_mfma_f32_32x32x16_bf16.
+// The keys of 32 are dealt to the rows of the first product so that a lane ends with the weights of two pieces of eight neighbouring keys, the slices that the
+// second product takes.  In LDS keys lie in pieces of eight elements, a piece of all 64 keys side by side, values in pieces of eight keys, a piece of all elements side by
+// side (eight neighbours exchanged by the number of their 16, so that the writers of one element write to different banks): all reads are whole lines.
+// us, as above and so: 2,048 tokens behind 30,000 keys at 12/2 heads 562 and 458, a prompt of 8,192 at 40/8 heads 1,007 and 780, of 2,048 101 and 71, but at 12/2 heads 41 and 59.
+constexpr int TILE = 64, SHARED_COLUMNS = 128;  // keys, columns
+constexpr int UNITS_ROUNDS = (2 * D + PORTION_THREADS - 1) / PORTION_THREADS;  // 16-byte units of codes a thread takes of a tile's keys, and of its values
+constexpr int SHARED_BEGINNING = 3;           // tiles that a walk's beginning and end take as long as
+
+struct Codes {                                // of a thread, of a tile
+  u32x4 keys[UNITS_ROUNDS], values[UNITS_ROUNDS];
+  unsigned key_power[UNITS_ROUNDS], value_powers[UNITS_ROUNDS];
+};
+struct Entries {                              // table entries of a thread's units
+  int key[UNITS_ROUNDS], value[UNITS_ROUNDS];
+};
+
+struct SharedTiles {
+  const unsigned char* from;                  // of the kv head
+  const int* table;
+  unsigned page_stride;
+  PackedPage page;
+};
+
+__device__ __forceinline__ unsigned page_of(const Walk& w, unsigned piece) { return w.page_shift >= 0 ? piece >> w.page_shift : __umulhi(piece, w.page_reciprocal); }
+
+// unit u of a tile's keys: key u % 64, block u / 64; of its values: half u % 2 of the eight keys of piece u / (D / 4), granule (u / 2) % (D / 8)
+__device__ __forceinline__ void load_entries(Entries& e, const Walk& w, const SharedTiles& tiles, int base) {
+#pragma unroll
+  for (int i = 0; i < UNITS_ROUNDS; ++i) {
+    const unsigned unit = i * PORTION_THREADS + threadIdx.x, key_at = page_of(w, (base + unit % TILE) / 8), value_at = page_of(w, base / 8 + unit / (D / 4));
+    e.key[i] = key_at < (unsigned)w.table_width ? tiles.table[key_at] : 0;
+    e.value[i] = value_at < (unsigned)w.table_width ? tiles.table[value_at] : 0;
   }
+}
+__device__ __forceinline__ void load_codes(Codes& c, const Entries& e, const Walk& w, const SharedTiles& tiles, int base) {
+  const unsigned per_page = (unsigned)w.page_size / 8;
+#pragma unroll
+  for (int i = 0; i < UNITS_ROUNDS; ++i) {
+    const unsigned unit = i * PORTION_THREADS + threadIdx.x;
+    if (2 * D % PORTION_THREADS && unit >= 2 * D) continue;
+    {
+      const unsigned key = base + unit % TILE, block = unit / TILE, offset = key - page_of(w, key / 8) * per_page * 8;
+      const unsigned char* mine = tiles.from + (size_t)((unsigned)e.key[i] < (unsigned)w.num_pages ? (unsigned)e.key[i] : 0u) * tiles.page_stride;
+      c.keys[i] = *(const u32x4*)(mine + tiles.page.key_codes(offset, block * 4));
+      c.key_power[i] = mine[tiles.page.key_power(offset, block)];
+    }
+    const unsigned piece = base / 8 + unit / (D / 4), half = unit % 2, granule = unit / 2 % (D / 8), offset = (piece - page_of(w, piece) * per_page) * 8;
+    const unsigned char* mine = tiles.from + (size_t)((unsigned)e.value[i] < (unsigned)w.num_pages ? (unsigned)e.value[i] : 0u) * tiles.page_stride;
+    c.values[i] = *(const u32x4*)(mine + tiles.page.value_codes(offset + half * 4, granule));
+    c.value_powers[i] = *(const unsigned*)(mine + tiles.page.value_power(offset + half * 4, granule / 4));
+  }
+}
+
+// Values that are no number count as zero, and as what they are where they are seen: `bad` gets, per block of 32 elements, the keys of the tile that have such.
+// Keys beyond `last`, which nobody sees, are made small numbers, whatever lies there.
+__device__ __forceinline__ void settle_powers(Codes& c, unsigned long long* bad, int base, int last) {
+#pragma unroll
+  for (int i = 0; i < UNITS_ROUNDS; ++i) {
+    const unsigned unit = i * PORTION_THREADS + threadIdx.x;
+    if (2 * D % PORTION_THREADS && unit >= 2 * D) continue;
+    const unsigned powers = c.value_powers[i], all = powers & (powers >> 4), granule = unit / 2 % (D / 8);
+    const int first = unit / (D / 4) * 8 + unit % 2 * 4;  // key of the tile
+    if (base + first + 3 > last || ((all & (all >> 2)) & 0x03030303u) != 0u) {  // (bytes of 255, and some others)
+      unsigned settled = powers;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const bool unseen = base + first + j > last, none = ((powers >> (8 * j)) & 255u) == PACKED_NO_NUMBER;
+        if (none && !unseen) atomicOr(&bad[granule / 4], 1ull << (first + j));
+        if (none || unseen) settled &= ~(255u << (8 * j));
+      }
+      c.value_powers[i] = settled;
+    }
+  }
+}
+
+// A thread's codes as bfloat16 into LDS, in eight parts: keys [D / 8][64][8] in the first four, values [8][D][8] in the others.
+constexpr int UNPACKS = 8;
+template <int PART_> __device__ __forceinline__ void unpack_part(const Codes& c, unsigned char* tile) {
+#pragma unroll
+  for (int i = 0; i < UNITS_ROUNDS; ++i) {
+    const unsigned unit = i * PORTION_THREADS + threadIdx.x;
+    if (2 * D % PORTION_THREADS && unit >= 2 * D) continue;
+    if constexpr (PART_ < 4) {
+      const unsigned key = unit % TILE, block = unit / TILE, codes = c.keys[i][PART_];
+      const float power = packed_power(c.key_power[i]);
+      *(u32x4*)(tile + ((block * 4 + PART_) * TILE + key) * 16) = (u32x4){unpack_pair<0>(codes, power), unpack_pair<1>(codes, power), unpack_pair<2>(codes, power), unpack_pair<3>(codes, power)};
+    } else {
+      constexpr int E = PART_ - 4;              // elements 2 E and 2 E + 1 of the eight
+      const unsigned piece = unit / (D / 4), half = unit % 2, granule = unit / 2 % (D / 8), exchange = (granule >> 1) & 7, powers = c.value_powers[i];
+      unsigned raw[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) raw[j] = unpack_pair<E>(c.values[i][j], __uint_as_float(j == 3 ? powers >> 1 : powers << (23 - j * 8)));
+      unsigned char* to = tile + TILE * D * 2 + (piece * D + granule * 8) * 16 + half * 8;
+      *(u32x2*)(to + ((2 * E) ^ exchange) * 16) = (u32x2){__builtin_amdgcn_perm(raw[1], raw[0], 0x05040100u), __builtin_amdgcn_perm(raw[3], raw[2], 0x05040100u)};
+      *(u32x2*)(to + ((2 * E + 1) ^ exchange) * 16) = (u32x2){__builtin_amdgcn_perm(raw[1], raw[0], 0x07060302u), __builtin_amdgcn_perm(raw[3], raw[2], 0x07060302u)};
+    }
+  }
+}
+template <int FIRST, int LAST> __device__ __forceinline__ void unpack_parts(const Codes& c, unsigned char* tile) {
+  if constexpr (FIRST < LAST) {
+    unpack_part<FIRST>(c, tile);
+    unpack_parts<FIRST + 1, LAST>(c, tile);
+  }
+}
+
+struct SharedColumns {                          // a wave's 32
+  Eight query[D / 16];
+  int position;                               // of the lane's column's token
+  int first_position, last_position;          // of the wave's
+  float reference, total;                     // total: of the lane's half of the keys
+  bool begun;                                 // some key has been seen; before, the reference is 0
+  f32x16 sum[D / 32];
+};
+
+// A tile of 64 keys from `base` on, with the next tile's codes made bfloat16 on the way (`next`: where to).  In a wave instructions begin in order, and one of these products keeps the
+// matrix core busy for eight others: so each is followed by what does not wait for it, a part of the next tile behind those of the scores, weights of later keys
+// behind those of the values.  edge: some column does not see some of the keys.
+constexpr int KEYS_AHEAD = 3;                 // slices of the keys that have been asked for
+template <int S> __device__ __forceinline__ void score_parts(f32x16 (&score)[2], Eight (&key)[KEYS_AHEAD][2], const SharedColumns& columns, const unsigned char* mine, const Codes& codes, unsigned char* next) {
+  if constexpr (S < D / 16) {
+#pragma unroll
+    for (int sub = 0; sub < 2; ++sub) {
+      score[sub] = multiply(key[S % KEYS_AHEAD][sub], columns.query[S], score[sub]);
+      if constexpr (S + KEYS_AHEAD < D / 16) key[S % KEYS_AHEAD][sub].u = *(const u32x4*)(mine + (2 * (S + KEYS_AHEAD) * TILE + sub * 32) * 16);
+    }
+    unpack_parts<S * UNPACKS / (D / 16), (S + 1) * UNPACKS / (D / 16)>(codes, next);
+    __builtin_amdgcn_sched_barrier(0);
+    score_parts<S + 1>(score, key, columns, mine, codes, next);
+  }
+}
+
+__device__ __forceinline__ void take_tile(SharedColumns& columns, const unsigned char* tile, const Walk& w, int base, bool edge, const Codes& codes, unsigned char* next) {
+  const int lane = threadIdx.x % WAVE, n = lane & 31, h = lane >> 5;
+  const int row = (n & 0x13) | ((n & 4) << 1) | ((n & 8) >> 1);  // the key that row n of the product is
+  f32x16 score[2];
+#pragma unroll
+  for (int i = 0; i < 16; ++i) score[0][i] = score[1][i] = 0.f;
+  const unsigned char* mine = tile + (h * TILE + row) * 16;
+  Eight key[KEYS_AHEAD][2];
+#pragma unroll
+  for (int s = 0; s < KEYS_AHEAD; ++s)
+#pragma unroll
+    for (int sub = 0; sub < 2; ++sub)
+      if (s < D / 16) key[s][sub].u = *(const u32x4*)(mine + (2 * s * TILE + sub * 32) * 16);
+  score_parts<0>(score, key, columns, mine, codes, next);
+  const unsigned char* values = tile + TILE * D * 2 + (h * D + n / 8 * 8) * 16;
+  const auto value_of = [&](int f, int t) { return *(const u32x4*)(values + (2 * f * D + t * 32) * 16 + ((n & 7) ^ ((t * 2 + (n >> 4)) & 7)) * 16); };
+  Eight value[D / 32];
+#pragma unroll
+  for (int t = 0; t < D / 32; ++t) value[t].u = value_of(0, t);
+  if (edge) {
+    const int highest = columns.position - base - 8 * h, lowest = w.window > 0 ? highest - w.window + 1 : -(1 << 30);
+#pragma unroll
+    for (int i = 0; i < 32; ++i) {
+      const int key = 16 * (i / 8) + i % 8;
+      if (key > highest || key < lowest) score[i / 16][i % 16] = -INFINITY;
+    }
+  }
+  float x[32];                                // log2 of the weights
+#pragma unroll
+  for (int i = 0; i < 32; ++i) x[i] = __builtin_fmaf(score[i / 16][i % 16], w.scale, -columns.reference);
+  float largest = fmaxf(fmaxf(largest_of(x), largest_of(x + 8)), fmaxf(largest_of(x + 16), largest_of(x + 24)));
+  if (__any(largest > (columns.begun ? AHEAD : -INFINITY))) {
+    largest = fmaxf(largest, __shfl_xor(largest, 32));
+    // (a column's first reference is its first tile's largest score, wherever that lies; later ones only rise)
+    const float rise = largest > (columns.begun ? 0.f : -INFINITY) ? largest : 0.f, change = columns.begun ? __builtin_amdgcn_exp2f(-rise) : 1.f;
+    columns.begun = columns.begun || largest > -INFINITY;
+    columns.reference += rise;
+    columns.total *= change;
+#pragma unroll
+    for (int t = 0; t < D / 32; ++t) columns.sum[t] *= change;
+#pragma unroll
+    for (int i = 0; i < 32; ++i) x[i] -= rise;
+  }
+  Eight weight;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) weight.v[j] = (bf16_t)__builtin_amdgcn_exp2f(x[j]);
+#pragma unroll
+  for (int f = 0; f < 4; ++f) {
+    Eight later;
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int t = 0; t < D / 32; ++t) {
+      columns.sum[t] = multiply(value[t], weight, columns.sum[t]);
+      if (f < 3) value[t].u = value_of(f + 1, t);
+    }
+    // the weights that are multiplied are the weights that are added up
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      union { unsigned u; packed_bf16x2 v; } pair, ones;
+      pair.u = weight.u[j];
+      ones.u = 0x3f803f80u;
+      columns.total = __builtin_amdgcn_fdot2_f32_bf16(pair.v, ones.v, columns.total, false);
+    }
+    if (f < 3) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) later.v[j] = (bf16_t)__builtin_amdgcn_exp2f(x[8 * (f + 1) + j]);
+      weight = later;
+    }
+#pragma unroll
+    for (int t = 0; t < D / 32; ++t) {          // a product, then the next value and a share of the rest
+      __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+      __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+      __builtin_amdgcn_sched_group_barrier(0x002, (16 + D / 32 - 1) / (D / 32), 0);
+    }
+  }
+}
+
+__global__ void __launch_bounds__(PORTION_THREADS, D <= 128 ? 2 : 1)
+packed_shared_kernel(const bf16_t* q, int q_stride, bf16_t* out, int out_stride, const unsigned char* pages, Walk w, Streams streams, int items, int whole, int whole_out) {
+  constexpr int TILE_BYTES = TILE * D * 2;
+  __shared__ __attribute__((aligned(16))) unsigned char memory[2][2 * TILE_BYTES];  // a tile's keys, then its values
+  __shared__ unsigned long long bad[3][D / 32];
+  __shared__ Shares shares;
+  const int lane = threadIdx.x % WAVE, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / WAVE), n = lane & 31, h = lane >> 5, group = w.heads / w.kv_heads;
+
+  take_walks<SHARED_COLUMNS, TILE, TILE, SHARED_BEGINNING>(w, streams, items, shares, [&](const Item& item, int kv_head, int begin, int end, float* part) {
+    SharedTiles tiles;
+    tiles.page = {D, w.page_size};
+    tiles.from = pages + (size_t)kv_head * tiles.page.bytes();
+    tiles.table = w.tables + (size_t)item.request * w.table_width;
+    tiles.page_stride = (unsigned)w.kv_heads * tiles.page.bytes();
+    Entries entries[3];
+#pragma unroll
+    for (int i = 0; i < 3; ++i) load_entries(entries[i], w, tiles, begin + i * TILE);
+    Codes now, next;
+    load_codes(now, entries[0], w, tiles, begin);
+    load_codes(next, entries[1], w, tiles, begin + TILE);
+    SharedColumns columns;
+    const int first_column = wave * 32, column = min(first_column + n, item.columns - 1), flat = item.first + column, token = flat / group;
+    const int token_zero = item.first_position - item.first / group;  // the position that the request's first token of the step is at
+    columns.position = token_zero + token;
+    columns.first_position = token_zero + (item.first + min(first_column, item.columns - 1)) / group;
+    columns.last_position = token_zero + (item.first + min(first_column + 31, item.columns - 1)) / group;
+    const bf16_t* row = q + (size_t)(item.first_row + token) * q_stride + (kv_head * group + flat - token * group) * D + h * 8;
+#pragma unroll
+    for (int s = 0; s < D / 16; ++s) {
+      if (whole) {
+        columns.query[s].u = *(const u32x4*)(row + s * 16);
+      } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) columns.query[s].v[e] = row[s * 16 + e];
+      }
+    }
+    columns.reference = columns.total = 0.f;
+    columns.begun = false;
+#pragma unroll
+    for (int t = 0; t < D / 32; ++t)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) columns.sum[t][i] = 0.f;
+    __syncthreads();                          // (a walk before this one has been read, and what it marked)
+    if (threadIdx.x < 3 * (D / 32)) (&bad[0][0])[threadIdx.x] = 0ull;
+    __syncthreads();
+    settle_powers(now, bad[0], begin, item.last_position);
+    unpack_parts<0, UNPACKS>(now, memory[0]);
+    int turn = 0, third = 0;                  // of the tile that is multiplied: its place in LDS, that of its marks
+    for (int base = begin; base < end; base += TILE) {
+      asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");  // (codes under way go on)
+      now = next;
+      entries[1] = entries[2];
+      load_codes(next, entries[1], w, tiles, base + 2 * TILE);
+      load_entries(entries[2], w, tiles, base + 3 * TILE);
+      if (threadIdx.x < D / 32) bad[third == 0 ? 2 : third - 1][threadIdx.x] = 0ull;  // (those of the tile before, which are those of the next but one)
+      const int following = third == 2 ? 0 : third + 1;
+      settle_powers(now, bad[following], base + TILE, item.last_position);
+      // (a tile behind the last one is made too, of whatever lies there: nobody looks at it)
+      take_tile(columns, memory[turn], w, base, base + TILE - 1 > columns.first_position || (w.window > 0 && base < columns.last_position - w.window + 1), now, memory[turn ^ 1]);
+      unsigned long long any = 0ull;
+#pragma unroll
+      for (int t = 0; t < D / 32; ++t) any |= bad[third][t];
+      if (any) {                              // hardly ever: values that are no number, for the columns that see them
+        const int lowest = w.window > 0 ? max(columns.position - w.window + 1 - base, 0) : 0, highest = min(columns.position - base, TILE - 1);
+        const unsigned long long seen = highest < lowest ? 0ull : ((2ull << highest) - 1ull) & ~((1ull << lowest) - 1ull);
+#pragma unroll
+        for (int t = 0; t < D / 32; ++t)
+          if (bad[third][t] & seen) columns.sum[t] += __uint_as_float(0x7fc00000u);
+      }
+      turn ^= 1;
+      third = following;
+    }
+    const float weights = columns.total + __shfl_xor(columns.total, 32);
+    if (first_column + n >= item.columns) return;
+    if (part) {
+      float* to = part + (first_column + n) * (D + 4);
+#pragma unroll
+      for (int t = 0; t < D / 32; ++t)
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          *(f32x4*)(to + t * 32 + 8 * i + 4 * h) = (f32x4){columns.sum[t][4 * i], columns.sum[t][4 * i + 1], columns.sum[t][4 * i + 2], columns.sum[t][4 * i + 3]};
+      if (h == 0) *(f32x4*)(to + D) = (f32x4){columns.begun ? columns.reference : -INFINITY, weights, 0.f, 0.f};
+    } else {
+      const float over = 1.f / weights;
+      bf16_t* to = out + (size_t)(item.first_row + token) * out_stride + (kv_head * group + flat - token * group) * D;
+#pragma unroll
+      for (int t = 0; t < D / 32; ++t)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          union { bf16_t e[4]; u32x2 u; } four;
+#pragma unroll
+          for (int j = 0; j < 4; ++j) four.e[j] = (bf16_t)(columns.sum[t][4 * i + j] * over);
+          if (whole_out) {
+            *(u32x2*)(to + t * 32 + 8 * i + 4 * h) = four.u;
+          } else {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) to[t * 32 + 8 * i + 4 * h + j] = four.e[j];
+          }
+        }
+    }
+  });
 }
 
 // ---------------------------------------------------------------------------------------------------------------- launches
@@ -1089,7 +1491,7 @@ __global__ void __launch_bounds__(PORTION_THREADS, D <= 128 ? 2 : 1) packed_port
 constexpr int WORKGROUPS = 512, PORTION_WORKGROUPS = 512;  // two a CU, as many as its LDS or registers hold (at heads of up to 128)
 
 template <typename T>
-static int launch(const void* q, int q_stride, void* out, int out_stride, const void* pages, const Walk& w, const Streams& few, const Streams& many, int tokens, int kinds, hipStream_t stream) {
+static int launch(const void* q, int q_stride, void* out, int out_stride, const void* pages, const Walk& w, const Streams& few, const Streams& many, int tokens, int kinds, bool shared, hipStream_t stream) {
   const int group = w.heads / w.kv_heads, piece = sizeof(T) == 4 ? 4 : 8, whole = (size_t)q % 16 == 0 && q_stride % piece == 0;
   if (kinds & 1) {
     const long blocks = few.least ? WORKGROUPS : (long)w.requests * ((group + 15) / 16) * w.kv_heads;
@@ -1100,6 +1502,17 @@ static int launch(const void* q, int q_stride, void* out, int out_stride, const 
     if (int status = LAUNCH_STATUS()) return status;
   }
   if (!(kinds & 2)) return 0;
+  if constexpr (sizeof(T) == 2) {
+    if (shared) {
+      const long items = ((long)tokens * group + SHARED_COLUMNS - 1) / SHARED_COLUMNS + w.requests, blocks = many.least ? PORTION_WORKGROUPS : items * w.kv_heads;
+      if (blocks >= (1L << 31)) return ERR_BAD_ARGUMENT;
+      const int whole_out = (size_t)out % 8 == 0 && out_stride % 4 == 0;
+      packed_shared_kernel<<<(unsigned)blocks, PORTION_THREADS, 0, stream>>>((const T*)q, q_stride, (T*)out, out_stride, (const unsigned char*)pages, w, many, (int)items, whole, whole_out);
+      if (int status = LAUNCH_STATUS()) return status;
+      if (many.least) packed_join_kernel<T><<<dim3(PORTION_WORKGROUPS, 8), 4 * WAVE, 0, stream>>>((T*)out, out_stride, many, SHARED_COLUMNS);
+      return LAUNCH_STATUS();
+    }
+  }
   const long items = ((long)tokens * group + PORTION_COLUMNS<T> - 1) / PORTION_COLUMNS<T> + w.requests, blocks = many.least ? PORTION_WORKGROUPS : items * w.kv_heads;
   if (blocks >= (1L << 31)) return ERR_BAD_ARGUMENT;
   packed_portions_kernel<T><<<(unsigned)blocks, PORTION_THREADS, 0, stream>>>((const T*)q, q_stride, (T*)out, out_stride, (const unsigned char*)pages, w, many, (int)items, whole);
@@ -1108,21 +1521,22 @@ static int launch(const void* q, int q_stride, void* out, int out_stride, const 
   return LAUNCH_STATUS();
 }
 
-// Floats of workspace that requests of few columns, or of many, need where walks may be cut.
-extern "C" int llmserve_packed_attention_workspace(int many) {
-  return many ? PORTION_WORKGROUPS * (2 * 32 * (D + 4) + (int)(sizeof(Cut) / 4)) : WORKGROUPS * (2 * PART + (int)(sizeof(Cut) / 4));
+// Floats of workspace that requests of few columns (kind 0), of many (1), of many that share tiles (2), need where walks may be cut.
+extern "C" int llmserve_packed_attention_workspace(int kind) {
+  return kind == 0 ? WORKGROUPS * (2 * PART + (int)(sizeof(Cut) / 4)) : PORTION_WORKGROUPS * (2 * (kind == 1 ? 32 : SHARED_COLUMNS) * (D + 4) + (int)(sizeof(Cut) / 4));
 }
 
 // q's heads are the first columns of rows of q_stride; tokens, requests: as many rows and requests as the arrays hold.  kinds: 1: some requests may have few columns (a
-// single token, or no more than 16 of them in all), 2: some may have more.  few_least, many_least: 0: a walk over the keys of few (many) columns is taken whole by one workgroup; else every
-// workgroup takes at least so many units of 256 (128) keys, walks are cut, and there is a workspace.  Those of many columns are cut for up to 256 requests alone.
+// single token, or no more than 16 of them in all), 2: some may have more, 4: those share tiles of keys
+// (bfloat16).  few_least, many_least: 0: a walk over the keys of few (many) columns is taken whole by one workgroup; else every
+// workgroup takes at least so many units of 256 (128; that share, 64) keys, walks are cut, and there is a workspace.  Those of many columns are cut for up to 256 requests alone.
 extern "C" int llmserve_packed_attention(const void* q, int is_float, int q_stride, void* out, int out_stride, void* few_workspace, void* many_workspace, const void* pages, int num_pages, const int* tables,
                                          int table_width, const int* query_start, const int* contexts, int requests, int tokens, int heads, int kv_heads, int page_size, float scale, int window, int kinds,
                                          int few_least, int many_least, hipStream_t stream) {
   if (tokens == 0 || requests == 0) return 0;
   if (!q || !out || !pages || !tables || !query_start || !contexts || requests < 0 || tokens < 0 || kv_heads <= 0 || heads <= 0 || heads % kv_heads || num_pages <= 0 || table_width <= 0 ||
       !packed_fits(D, page_size) || (long)page_size * D * kv_heads >= (1L << 30) || !(scale > 0.f) || (size_t)pages % 16 || q_stride < heads * D || out_stride < heads * D || window < 0 ||
-      kinds < 1 || kinds > 3 || few_least < 0 || (few_least > 0 && (!few_workspace || (size_t)few_workspace % 16)) || many_least < 0 ||
+      kinds < 1 || kinds > 7 || kinds == 4 || (is_float && (kinds & 4)) || few_least < 0 || (few_least > 0 && (!few_workspace || (size_t)few_workspace % 16)) || many_least < 0 ||
       (many_least > 0 && (!many_workspace || (size_t)many_workspace % 16 || requests > PORTION_THREADS)))
     return ERR_BAD_ARGUMENT;
   const unsigned per_page = (unsigned)page_size / 8;
@@ -1131,7 +1545,8 @@ extern "C" int llmserve_packed_attention(const void* q, int is_float, int q_stri
   if (!power_of_two && ((unsigned long)table_width * per_page + 64) * per_page >= (1UL << 32)) return ERR_BAD_ARGUMENT;
   const Walk w = {tables, table_width, num_pages, page_size, power_of_two ? 31 - __builtin_clz(per_page) : -1, (unsigned)(((1UL << 32) + per_page - 1) / per_page), query_start, contexts, requests, heads, kv_heads, window, scale * LOG2_E};
   const Streams few = {(float*)few_workspace, (Cut*)((float*)few_workspace + WORKGROUPS * 2 * PART), few_least};
-  const Streams many = {(float*)many_workspace, (Cut*)((float*)many_workspace + PORTION_WORKGROUPS * 2 * 32 * (D + 4)), many_least};
-  if (is_float) return launch<float>(q, q_stride, out, out_stride, pages, w, few, many, tokens, kinds, stream);
-  return launch<bf16_t>(q, q_stride, out, out_stride, pages, w, few, many, tokens, kinds, stream);
+  const bool shared = kinds & 4;
+  const Streams many = {(float*)many_workspace, (Cut*)((float*)many_workspace + PORTION_WORKGROUPS * 2 * (shared ? SHARED_COLUMNS : 32) * (D + 4)), many_least};
+  if (is_float) return launch<float>(q, q_stride, out, out_stride, pages, w, few, many, tokens, kinds, shared, stream);
+  return launch<bf16_t>(q, q_stride, out, out_stride, pages, w, few, many, tokens, kinds, shared, stream);
 }

@@ -1773,45 +1773,63 @@ class HipKernels:
         return self._lazy[key]
 
     @staticmethod
-    def _packed_kinds(batch, group: int, tokens: int) -> tuple[int, int, int, int]:
-        """(1: no request has many columns, 2: none has few, 3; the longest context of those of few columns, of those of many; the latter's tokens).  Few are a
-        single token or up to 16 query heads a kv head in all.  A captured step is replayed with other requests: any of either kind."""
-        longest = batch.max_context_length
+    def _packed_walks(batch, group: int, window: int) -> tuple:
+        """(1: no request has many columns, 2: none has few, 3; the longest walk over the keys of few columns; of many: their tokens, the longest walk, sums over the
+        requests' tokens of the shortest walk and of the mean one).  Few columns are those of a single token or of up to 16 query heads a kv head in all.  A captured step is replayed with
+        other requests: any of either kind, the longest."""
+        longest = min(batch.max_context_length, window + 31) if window else batch.max_context_length
         if batch.max_query_length <= 1:
-            return 1, longest, 0, 0
+            return 1, longest, 0, 0, 0, 0
         if getattr(batch, "padded_to", None) is not None:
-            return 3, longest, longest, tokens
-        known = batch.scratch.get(("packed kinds", group))
+            tokens = batch.padded_to[0]
+            return 3, longest, tokens, longest, tokens * longest, tokens * longest
+        known = batch.scratch.get(("packed walks", group, window))
         if known is not None:
             return known
-        few = many = singles = 0
+        few = many = tokens = shortest = mean = 0
         for chunk in batch.chunks:
-            end = chunk.start + chunk.count
-            if chunk.count > 1 and chunk.count * group > 16:
-                many = end if end > many else many
+            count, end = chunk.count, chunk.start + chunk.count
+            if count > 1 and count * group > 16:
+                first, last = (min(chunk.start, window), min(end, window + 31)) if window else (chunk.start, end)
+                tokens += count
+                many = max(many, last)
+                shortest += count * first
+                mean += count * (first + last) // 2
             else:
-                few = end if end > few else few
-                singles += chunk.count
-        known = batch.scratch[("packed kinds", group)] = (1 if many == 0 else 2 if few == 0 else 3), few, many, tokens - singles
+                few = max(few, min(end, window + 31) if window else end)
+        known = batch.scratch[("packed walks", group, window)] = (1 if tokens == 0 else 2 if few == 0 else 3), few, tokens, many, shortest, mean
         return known
 
     @staticmethod
-    def _packed_least(few: int, many: int, tokens: int, requests: int, heads: int, kv_heads: int, window: int) -> tuple[int, int]:
-        """(units of 256 keys that a workgroup takes at least of walks over the keys of few columns, units of 128 keys of those of many): walks are cut anywhere.  0: every
-        walk is taken whole.  `few` and `many` are the longest contexts, `tokens` those of many columns."""
-        group = heads // kv_heads
-        if window:
-            few, many = min(few, window + 31), min(many, window + 31)
+    def _packed_way(walks: tuple, requests: int, group: int, kv_heads: int, shares: bool) -> tuple[int, int, bool]:
+        """(units of 256 keys that a workgroup takes at least of walks over the keys of few columns, units of 128 or 64 of those of many, whether the latter share tiles
+        of keys, which `shares` allows): walks are cut anywhere; 0: every walk is taken whole."""
+        _, few, tokens, many, shortest, mean = walks
         pairs = requests * kv_heads * -(-group // 16)
         few = 0 if few <= 1024 or 22 * few <= 50000 + 3 * pairs * few // 10 else 4
-        if many == 0 or requests > 256:
-            return few, 0
-        # Of many columns: whole, the 512 workgroups that the chip holds take 11.5 us for 1,000 keys of 32 columns each, 256 of them 8.25 (each alone on its unit);
-        # cut, the sum of all walks is what counts, 25 ns for 1,000 keys of a column's 32, and 18 us on top.  us, whole and cut: 12 heads on 2, 128 tokens
-        # behind 30,000 251 and 64, behind 2,000 27 and 30; 512 behind 10,000 93 and 75; 2,048 behind 30,000 562 and 573; 40 heads on 8, 512 behind 10,000 201 and 186.
-        whole, rest = divmod(kv_heads * -(-tokens * group // 32), 512)
-        spared = 11.5 * whole + (0.0 if rest == 0 else 8.25 if rest <= 256 else 11.5) - 0.025 * (512 * whole + rest)
-        return few, 8 if spared * many > 18000 else 0
+        if tokens == 0:
+            return few, 0, False
+        # Of many columns.  Whole, a workgroup of 32 columns takes 8.25 us for 1,000 keys where it is alone on its unit (up to 256 of them), 11.5 beside another,
+        # one of 128 that share tiles 27.4 and 34.7; a walk's beginning and end take as long as 700 (420) keys, and 512 fit.  So it is the longest walk, or rounds of the keys that all walks have in
+        # common and the sum of the rest, the longest first.  Cut, it is the sum of all walks, and what the joining takes.  us, measured (and estimated), whole, cut, shared whole, shared and cut:
+        # 12 heads on 2, a prompt of 2,047 40 (38), 59, 60, 59; 128 tokens behind 30,000 251, 64 (53), 830, 130; 2,048 behind 30,000 562, 573, 879, 490 (500); 8,192 317, -, 248 (241), 293.
+        # 28 heads on 4, 2,048 76, 98, 68 (62), 87; behind 10,000 455, 515, 399 (398), 418.  40 heads on 8, 512 24 (22), 36, 22 (20), 43; 2,048 behind 10,000 634, 720, 636, 591 (590).
+        columns, common, rest = tokens * group * kv_heads, shortest / tokens / 1000, (mean - shortest) / tokens / 1000
+
+        def whole(width: int, alone: float, beside: float, extra: float) -> float:
+            items = -(-columns // width)
+            full, left = divmod(items, 512)
+            rounds = beside * full + (0.0 if left == 0 else alone if left <= 256 else beside)
+            return max(alone * many / 1000, common * rounds + beside / 512 * items * (rest + extra))
+
+        ways = [(8.0 + whole(32, 8.25, 11.5, 0.7), 0, False)]
+        if requests <= 256:
+            ways.append((21.0 + 0.0235 * columns / 32 * (common + rest + 0.5), 8, False))
+        if shares:
+            ways.append((6.0 + whole(128, 27.4, 34.7, 0.42), 0, True))
+            if requests <= 256:
+                ways.append((44.0 + 0.077 * columns / 128 * (common + rest), 8, True))
+        return few, *min(ways)[1:]
 
     def _packed_attention(self, qkv, layout, batch, cell, scale: float, window: int | None, out):
         tokens, heads, kv_heads, dim = qkv.shape[0], layout.num_heads, layout.num_kv_heads, layout.head_dim
@@ -1827,13 +1845,16 @@ class HipKernels:
         out = self._attention_out(qkv, layout, out)
         window = int(window or 0)
         library = self._packed_library(dim)
-        kinds, few, many, of_many = self._packed_kinds(batch, heads // kv_heads, tokens)
-        few, many = self._packed_least(few, many, of_many, requests, heads, kv_heads, window)
-        spaces = [self._empty((library.llmserve_packed_attention_workspace(kind),), torch.float32) if least else None for kind, least in ((0, few), (1, many))]
+        walks = self._packed_walks(batch, heads // kv_heads, window)
+        # (tiles of heads of 160 and 192 keep five and six of eight threads busy: 2,048 tokens behind 10,000 keys at 12/2 heads of 160 441 us apart, 476 shared, at 16/4 of 192 593 and 667,
+        # but at 16/2 of 224 1,182 and 700, of 256 697 and 606)
+        shares = qkv.dtype == torch.bfloat16 and not 128 < dim < 224
+        few, many, shared = self._packed_way(walks, requests, heads // kv_heads, kv_heads, shares)
+        spaces = [self._empty((library.llmserve_packed_attention_workspace(kind),), torch.float32) if least else None for kind, least in ((0, few), (2 if shared else 1, many))]
         status = library.llmserve_packed_attention(
             _pointer(qkv), _is_float(qkv), layout.stride, _pointer(out), out.shape[1], _pointer(spaces[0]), _pointer(spaces[1]), _pointer(pages), pages.shape[0],
             _pointer(group.block_tables), group.width, _pointer(batch.query_start), _pointer(batch.context_lengths), requests, tokens, heads, kv_heads, group.page_size, scale, window,
-            kinds, few, many, self._stream,
+            walks[0] + (4 if shared else 0), few, many, self._stream,
         )
         _check(status, "paged_attention over 4 bits")
         return out

@@ -119,13 +119,18 @@ def test_refusals_of_index_arrays(kernels):
 # ---------------------------------------------------------------------------- whole and cut
 
 
+def force(monkeypatch, k, least):
+    """Walks in the given way, tiles shared where they can be."""
+    monkeypatch.setattr(type(k), "_packed_way", staticmethod(lambda *given: (*least[:2], least[2] and k.dtype == torch.bfloat16)))
+
+
 @pytest.mark.parametrize("dtype", DTYPES)
-@pytest.mark.parametrize("least", [(0, 0), (1, 0), (0, 1), (1, 1), (4, 8), (3, 40)])
-@pytest.mark.parametrize("heads,kv_heads,dim,page,window", [(12, 2, 128, 16, None), (6, 2, 96, 24, 300), (7, 1, 64, 8, None), (34, 2, 32, 16, None)])
+@pytest.mark.parametrize("least", [(0, 0, False), (1, 0, False), (0, 1, False), (1, 1, False), (4, 8, False), (3, 40, False), (0, 0, True), (1, 1, True), (0, 8, True), (4, 33, True)])
+@pytest.mark.parametrize("heads,kv_heads,dim,page,window", [(12, 2, 128, 16, None), (6, 2, 96, 24, 300), (7, 1, 64, 8, None), (34, 2, 32, 16, None), (3, 1, 192, 40, 65), (4, 2, 256, 16, None)])
 def test_walks_whole_and_cut_anywhere(kernels, dtype, least, heads, kv_heads, dim, page, window, monkeypatch):
     k = kernels[dtype]
     lengths, counts = [1300, 1, 530, 777, 40, 0, 260, 1025], [1, 1, 1, 45, 40, 0, 2, 70]
-    monkeypatch.setattr(type(k), "_packed_least", staticmethod(lambda *given: least))
+    force(monkeypatch, k, least)
     batch, cell, layout, qkv, found = packed_case(k, lengths, counts, heads, kv_heads, dim, page, seed=dim)
     got = k.paged_attention(qkv, layout, batch, cell, dim ** -0.5, window)
     assert_near(got, expected_of(found, lengths, counts, dim ** -0.5, window), largest_of(found, counts), dtype)
@@ -133,27 +138,42 @@ def test_walks_whole_and_cut_anywhere(kernels, dtype, least, heads, kv_heads, di
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
-@pytest.mark.parametrize("least", [None, (1, 0), (0, 0)])
+@pytest.mark.parametrize("least", [None, (1, 0, False), (0, 0, True)])
 def test_many_requests(kernels, dtype, least, monkeypatch):
     """More requests than a workgroup has threads for, portions among them (which are then never cut)."""
     k = kernels[dtype]
     lengths = [1 + (index * 37) % 90 for index in range(300)]
     counts = [1 if index % 50 else min(length, 30) for index, length in enumerate(lengths)]
     if least is not None:
-        monkeypatch.setattr(type(k), "_packed_least", staticmethod(lambda *given: least))
+        force(monkeypatch, k, least)
     batch, cell, layout, qkv, found = packed_case(k, lengths, counts, 4, 2, 64, 8)
     got = k.paged_attention(qkv, layout, batch, cell, 0.125, None)
     assert_near(got, expected_of(found, lengths, counts, 0.125, None), largest_of(found, counts), dtype)
 
 
-def test_which_walks_are_cut():
-    """Both sides of the rule: few workgroups and long walks are cut, walks enough to fill the chip are not."""
+def test_which_way_walks_go():
+    """Few workgroups and long walks are cut, walks enough to fill the chip are not; tiles are shared where columns are many."""
+    from types import SimpleNamespace
+
+    from llmserve_amd.engine.batch import SequenceChunk
     from llmserve_amd.kernels import HipKernels
 
-    least = HipKernels._packed_least
-    assert least(640, 0, 0, 1, 12, 2, 0) == (0, 0) and least(30000, 0, 0, 8, 40, 8, 0) == (4, 0) and least(30000, 0, 0, 8, 40, 8, 512) == (0, 0)
-    assert least(0, 2047, 2047, 1, 12, 2, 0) == (0, 0) and least(0, 30128, 128, 1, 12, 2, 0) == (0, 8) and least(0, 32048, 2048, 1, 12, 2, 0) == (0, 0)
-    assert least(0, 30128, 128, 257, 12, 2, 0)[1] == 0 and least(0, 30128, 128, 1, 12, 2, 512) == (0, 0)
+    def way(chunks, heads, kv_heads, window=0, shares=True, padded_to=None):
+        batch = SimpleNamespace(max_context_length=max(start + count for start, count in chunks), max_query_length=max(count for _, count in chunks), padded_to=padded_to, scratch={},
+                                chunks=[SequenceChunk(str(i), i, start, count) for i, (start, count) in enumerate(chunks)])
+        walks = HipKernels._packed_walks(batch, heads // kv_heads, window)
+        assert walks == HipKernels._packed_walks(batch, heads // kv_heads, window)
+        return walks[0], *HipKernels._packed_way(walks, len(chunks), heads // kv_heads, kv_heads, shares)
+
+    assert way([(639, 1)], 12, 2) == (1, 0, 0, False)
+    assert way([(29999, 1)] * 8, 40, 8) == (1, 4, 0, False) and way([(29999, 1)] * 8, 40, 8, 512) == (1, 0, 0, False)
+    assert way([(0, 2047)], 12, 2) == (2, 0, 0, False)
+    assert way([(30000, 128)], 12, 2) == (2, 0, 8, False) and way([(30000, 128)], 12, 2, 512) == (2, 0, 0, False)
+    assert way([(30000, 2048)], 12, 2) == (2, 0, 8, True) and not way([(30000, 2048)], 12, 2, shares=False)[3]
+    assert way([(0, 8192)], 40, 8) == (2, 0, 0, True)
+    assert way([(600, 1)] * 31 + [(300, 256)], 28, 4) == (3, 0, 0, False)  # the long context is not of the single tokens
+    assert way([(40, 2)] * 256 + [(30000, 128)], 12, 2)[:3] == (3, 0, 0)  # more requests than are cut for
+    assert way([(600, 1)] * 3 + [(300, 256)], 28, 4, padded_to=(300, 5))[0] == 3 and way([(300, 256)], 28, 4, padded_to=(300, 5))[0] == 3
 
 
 # ---------------------------------------------------------------------------- streams, graphs
@@ -179,12 +199,12 @@ def test_another_stream(kernels, dtype):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
-@pytest.mark.parametrize("least", [(1, 1), (0, 0)])
+@pytest.mark.parametrize("least", [(1, 1, False), (0, 0, False), (1, 1, True), (0, 0, True)])
 def test_captured_and_replayed(kernels, dtype, least, monkeypatch):
     """Two captured steps of different cells, replayed in turn with eager calls between them and with lengths, queries and pages changed under them: index arrays,
     store and attention in one graph."""
     k, page, kv_heads, heads, dim, tokens = kernels[dtype], 16, 2, 6, 64, 24
-    monkeypatch.setattr(type(k), "_packed_least", staticmethod(lambda *given: least))
+    force(monkeypatch, k, least)
     rng = torch.Generator().manual_seed(1)
     cases = []
     for index in range(2):
