@@ -35,9 +35,27 @@ __device__ __forceinline__ bool whole_piece(const int (&slot)[8]) {
   return whole;
 }
 
-// A thread packs eight elements of its rows, four neighbours a block.  The exponent of the block's largest magnitude a decides the power: 2^(exponent - 2), one more
+// Eight elements of a block's granule as codes, four bits each, of the block's power.  The exponent of the block's largest magnitude a decides the power: 2^(exponent - 2), one more
 // where a's significand is 1.75 or larger (a would be rounded to 8, which the elements do not have), so that a lands on 4 to 6.  Division by the
 // power is exact, and what is rounded is rounded once, to the nearest element (ties to the even code), so the bits depend on nothing but the row.
+__device__ __forceinline__ unsigned largest_bits(const float* x) {
+  unsigned largest = 0;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) largest = max(largest, __float_as_uint(x[e]) & 0x7fffffffu);
+  return largest;
+}
+__device__ __forceinline__ unsigned pack_eight(const float* x, unsigned largest, unsigned& power) {
+  const bool number = largest < 0x7f800000u;
+  power = number ? (unsigned)min(max((int)((largest + 0x200000u) >> 23) - 2, 2), 252) : PACKED_NO_NUMBER;
+  const float unit = packed_power(power);
+  unsigned codes = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(0u, x[0], x[1], unit, 0);
+  codes = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(codes, x[2], x[3], unit, 1);
+  codes = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(codes, x[4], x[5], unit, 2);
+  codes = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(codes, x[6], x[7], unit, 3);
+  return number ? codes : 0u;
+}
+
+// A thread packs eight elements of its rows, four neighbours a block.
 template <typename T, int ROWS>
 __global__ void __launch_bounds__(256) packed_store_kernel(const T* x, int stride, int first, int kv_heads, int tokens, unsigned char* pages, int slots_held, const int* slots, PackedPage page, bool whole) {
   const int granules = page.dim / 8;
@@ -58,19 +76,10 @@ __global__ void __launch_bounds__(256) packed_store_kernel(const T* x, int strid
   unsigned codes[ROWS], power[ROWS];
 #pragma unroll
   for (int i = 0; i < ROWS; ++i) {
-    unsigned largest = 0;
-#pragma unroll
-    for (int e = 0; e < 8; ++e) largest = max(largest, __float_as_uint(v[i][e]) & 0x7fffffffu);
+    unsigned largest = largest_bits(v[i]);
     largest = max(largest, (unsigned)__shfl_xor((int)largest, 1));
     largest = max(largest, (unsigned)__shfl_xor((int)largest, 2));
-    const bool number = largest < 0x7f800000u;
-    power[i] = number ? (unsigned)min(max((int)((largest + 0x200000u) >> 23) - 2, 2), 252) : PACKED_NO_NUMBER;
-    const float unit = packed_power(power[i]);
-    codes[i] = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(0u, v[i][0], v[i][1], unit, 0);
-    codes[i] = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(codes[i], v[i][2], v[i][3], unit, 1);
-    codes[i] = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(codes[i], v[i][4], v[i][5], unit, 2);
-    codes[i] = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(codes[i], v[i][6], v[i][7], unit, 3);
-    if (!number) codes[i] = 0;
+    codes[i] = pack_eight(v[i], largest, power[i]);
   }
   if constexpr (ROWS == 8) {
     if (value && whole_piece(slot) && slot[7] < slots_held) {
@@ -94,6 +103,74 @@ __global__ void __launch_bounds__(256) packed_store_kernel(const T* x, int strid
     unsigned char* mine = pages + ((size_t)at * kv_heads + head) * page.bytes();
     *(unsigned*)(mine + (value ? page.value_codes(offset, granule) : page.key_codes(offset, granule))) = codes[i];
     if (granule % 4 == 0) mine[value ? page.value_power(offset, granule / 4) : page.key_power(offset, granule / 4)] = (unsigned char)power[i];
+  }
+}
+
+// Few rows, rotated as they are packed (one launch of a layer's decode step less): a thread takes 16 elements of a head of a row, which hold eight pairs.  Neighbouring pairs: granules 2 p and 2 p + 1, half a
+// block; half pairs: granules p and p + D / 16, of two blocks (heads of a multiple of 64, so that four threads have a block each).  q and k are written back rotated, k is packed as it was
+// written back.
+template <typename T, bool HALF>
+__global__ void __launch_bounds__(256) packed_rotate_store_kernel(T* qkv, int stride, const float2* table, int heads, int kv_heads, int tokens, unsigned char* pages, int slots_held, const int* slots, PackedPage page,
+                                                                   bool whole) {
+  const int per_head = page.dim / 16, per_row = (heads + 2 * kv_heads) * per_head;
+  const int flat = blockIdx.x * blockDim.x + threadIdx.x, token = flat / per_row, inside = flat - token * per_row, head = inside / per_head, p = inside - head * per_head;
+  if (token >= tokens) return;                // (whole blocks of 32 leave together: a row has a multiple of four threads with half pairs, of two without)
+  T* row = qkv + (size_t)token * stride + (size_t)head * page.dim;
+  const bool value = head >= heads + kv_heads;
+  const int granule[2] = {HALF && !value ? p : 2 * p, HALF && !value ? p + per_head : 2 * p + 1};
+  float x[2][8];
+#pragma unroll
+  for (int g = 0; g < 2; ++g) load_eight(row + granule[g] * 8, whole, x[g]);
+  if (!value) {
+    const float2* angles = table + (size_t)token * (page.dim / 2) + 8 * p;
+    float2 turn[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) turn[i] = angles[i];
+    union { u32x4 v[2 * sizeof(T) / 2]; T e[2][8]; } out;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const int g0 = HALF ? 0 : i / 4, e0 = HALF ? i : i % 4 * 2, g1 = HALF ? 1 : i / 4, e1 = HALF ? i : i % 4 * 2 + 1;
+      float first, second;
+      const float a = x[g0][e0], b = x[g1][e1];
+      // (the bits of the kernels that only rotate)
+      if (sizeof(T) == 4 || stride % 8 != 0) first = __builtin_fmaf(a, turn[i].x, -(b * turn[i].y)), second = __builtin_fmaf(a, turn[i].y, b * turn[i].x);
+      else turn_pair(a, b, turn[i].x, turn[i].y, i == 0, &first, &second);
+      out.e[g0][e0] = from_float<T>(first);
+      out.e[g1][e1] = from_float<T>(second);
+    }
+#pragma unroll
+    for (int g = 0; g < 2; ++g) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) x[g][e] = to_float(out.e[g][e]);
+      if (whole) {
+#pragma unroll
+        for (unsigned i = 0; i < sizeof(T) / 2; ++i) ((u32x4*)(row + granule[g] * 8))[i] = out.v[g * (sizeof(T) / 2) + i];
+      } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) row[granule[g] * 8 + e] = out.e[g][e];
+      }
+    }
+  }
+  unsigned largest[2] = {largest_bits(x[0]), largest_bits(x[1])};
+  if (HALF && !value) {
+#pragma unroll
+    for (int g = 0; g < 2; ++g) {
+      largest[g] = max(largest[g], (unsigned)__shfl_xor((int)largest[g], 1));
+      largest[g] = max(largest[g], (unsigned)__shfl_xor((int)largest[g], 2));
+    }
+  } else {
+    largest[0] = max(largest[0], largest[1]);
+    largest[0] = largest[1] = max(largest[0], (unsigned)__shfl_xor((int)largest[0], 1));
+  }
+  const int slot = slots[token];
+  if (head < heads || slot < 0 || slot >= slots_held) return;
+  const int at = slot / page.page_size, offset = slot - at * page.page_size;
+  unsigned char* mine = pages + ((size_t)at * kv_heads + (value ? head - heads - kv_heads : head - heads)) * page.bytes();
+#pragma unroll
+  for (int g = 0; g < 2; ++g) {
+    unsigned power;
+    *(unsigned*)(mine + (value ? page.value_codes(offset, granule[g]) : page.key_codes(offset, granule[g]))) = pack_eight(x[g], largest[g], power);
+    if (granule[g] % 4 == 0) mine[value ? page.value_power(offset, granule[g] / 4) : page.key_power(offset, granule[g] / 4)] = (unsigned char)power;
   }
 }
 
@@ -187,6 +264,29 @@ extern "C" int llmserve_packed_store(const void* x, int is_float, int stride, in
   else if (is_float) launch(packed_store_kernel<float, 1>, (const float*)x);
   else if (each == 8) launch(packed_store_kernel<bf16_t, 8>, (const bf16_t*)x);
   else launch(packed_store_kernel<bf16_t, 1>, (const bf16_t*)x);
+  return LAUNCH_STATUS();
+}
+
+// Whether rows are rotated as they are packed: those that a thread takes one of, and with half pairs heads of a multiple of 64.
+extern "C" int llmserve_packed_rotates(int tokens, int kv_heads, int dim, int pairing) { return rows_a_thread(tokens, kv_heads, dim) == 1 && (pairing == 1 || (pairing == 2 && dim % 64 == 0)); }
+
+// The first heads + kv_heads heads of `tokens` rows rotated in place by the table's angles (pairing 1: neighbours, 2: halves), then as above.
+extern "C" int llmserve_packed_rotate_store(void* qkv, int is_float, int stride, const float* table, int pairing, int tokens, int heads, int kv_heads, int dim, void* pages, int num_pages, int page_size,
+                                            const int* slots, hipStream_t stream) {
+  if (tokens == 0) return 0;
+  const long held = (long)num_pages * page_size;
+  if (!qkv || !table || !pages || !slots || tokens < 0 || heads <= 0 || kv_heads <= 0 || num_pages <= 0 || !packed_fits(dim, page_size) || held >= (1L << 31) || (heads + 2L * kv_heads) * dim > stride ||
+      (size_t)pages % 16 || !llmserve_packed_rotates(tokens, kv_heads, dim, pairing))
+    return ERR_BAD_ARGUMENT;
+  const long blocks = ((long)tokens * (heads + 2 * kv_heads) * (dim / 16) + 255) / 256;
+  if (blocks * 256 >= (1L << 31)) return ERR_BAD_ARGUMENT;
+  const PackedPage page = {dim, page_size};
+  const bool whole = (size_t)qkv % 16 == 0 && stride % (is_float ? 4 : 8) == 0;
+  const auto launch = [&](auto kernel, auto rows) { kernel<<<(unsigned)blocks, 256, 0, stream>>>(rows, stride, (const float2*)table, heads, kv_heads, tokens, (unsigned char*)pages, (int)held, slots, page, whole); };
+  if (is_float && pairing == 2) launch(packed_rotate_store_kernel<float, true>, (float*)qkv);
+  else if (is_float) launch(packed_rotate_store_kernel<float, false>, (float*)qkv);
+  else if (pairing == 2) launch(packed_rotate_store_kernel<bf16_t, true>, (bf16_t*)qkv);
+  else launch(packed_rotate_store_kernel<bf16_t, false>, (bf16_t*)qkv);
   return LAUNCH_STATUS();
 }
 

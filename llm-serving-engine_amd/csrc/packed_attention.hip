@@ -1442,6 +1442,7 @@ packed_shared_kernel(const bf16_t* q, int q_stride, bf16_t* out, int out_stride,
       settle_powers(now, bad[following], base + TILE, item.last_position);
       // (a tile behind the last one is made too, of whatever lies there: nobody looks at it)
       take_tile(columns, memory[turn], w, base, base + TILE - 1 > columns.first_position || (w.window > 0 && base < columns.last_position - w.window + 1), now, memory[turn ^ 1]);
+      products_done();
       unsigned long long any = 0ull;
 #pragma unroll
       for (int t = 0; t < D / 32; ++t) any |= bad[third][t];

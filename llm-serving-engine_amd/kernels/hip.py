@@ -149,6 +149,8 @@ _SIGNATURES = {
     "llmserve_difference_heads": "pipiiiifffp",
     "llmserve_gate_columns": "piipiiiiipiip",
     "llmserve_packed_store": "piiiiiipiipp",
+    "llmserve_packed_rotates": "iiii",
+    "llmserve_packed_rotate_store": "piipiiiiipiipp",
     "llmserve_packed_rows": "piiiipippip",
     "llmserve_packed_attention_workspace": "i",
     "llmserve_packed_attention": "piipipppipippiiiiifiiiip",
@@ -465,6 +467,9 @@ class HipKernels:
         if qkv.shape[1] != layout.stride:
             raise KernelError("rotate_and_store: qkv does not have the layout's width")
         if cell is not None and _packed_pages(cell) is not None:
+            if pairing != "none" and cell.writable and self._library_of("packed").llmserve_packed_rotates(tokens, layout.num_kv_heads, layout.head_dim, _PAIRINGS[pairing]):
+                self._rotate_store_packed(qkv, layout, batch, cell, self.rotary_table(batch, inverse_frequencies), pairing)
+                return
             if pairing != "none":
                 self.rotate_and_store(qkv, layout, batch, None, inverse_frequencies, pairing)
             if cell.writable:
@@ -1740,18 +1745,29 @@ class HipKernels:
     def store_packed(self, qkv, layout, batch, cell) -> None:
         """The keys and values of `qkv`'s rows (as `rotate_and_store` leaves them), rounded to 4 bits, into the cell's pages at the step's
         slots (a negative slot, or one beyond the pages: nowhere; every other slot once)."""
-        tokens, kv_heads, dim = qkv.shape[0], layout.num_kv_heads, layout.head_dim
-        group = batch.groups[cell.group]
-        if not cell.writable:
-            raise KernelError("store_packed: the cell is another run's to write")
-        pages = self._packed_cell(cell, kv_heads, dim, group.page_size, "store_packed")
-        self._packed_query_rows(qkv, layout, "store_packed")
-        self._indices(group.slot_mapping, (tokens,), "store_packed: the step's slots")
+        pages, group = self._packed_rows_to_store(qkv, layout, batch, cell, "store_packed")
         status = self._library_of("packed").llmserve_packed_store(
-            _pointer(qkv), _is_float(qkv), qkv.shape[1], layout.num_heads * dim, tokens, kv_heads, dim, _pointer(pages), pages.shape[0], group.page_size,
-            _pointer(group.slot_mapping), self._stream,
+            _pointer(qkv), _is_float(qkv), qkv.shape[1], layout.num_heads * layout.head_dim, qkv.shape[0], layout.num_kv_heads, layout.head_dim, _pointer(pages), pages.shape[0],
+            group.page_size, _pointer(group.slot_mapping), self._stream,
         )
         _check(status, "store_packed")
+
+    def _rotate_store_packed(self, qkv, layout, batch, cell, table, pairing: str) -> None:
+        pages, group = self._packed_rows_to_store(qkv, layout, batch, cell, "rotate_and_store")
+        status = self._library_of("packed").llmserve_packed_rotate_store(
+            _pointer(qkv), _is_float(qkv), qkv.shape[1], _pointer(table), _PAIRINGS[pairing], qkv.shape[0], layout.num_heads, layout.num_kv_heads, layout.head_dim, _pointer(pages),
+            pages.shape[0], group.page_size, _pointer(group.slot_mapping), self._stream,
+        )
+        _check(status, "rotate_and_store into 4 bits")
+
+    def _packed_rows_to_store(self, qkv, layout, batch, cell, what: str) -> tuple:
+        group = batch.groups[cell.group]
+        if not cell.writable:
+            raise KernelError(f"{what}: the cell is another run's to write")
+        pages = self._packed_cell(cell, layout.num_kv_heads, layout.head_dim, group.page_size, what)
+        self._packed_query_rows(qkv, layout, what)
+        self._indices(group.slot_mapping, (qkv.shape[0],), f"{what}: the step's slots")
+        return pages, group
 
     def packed_rows(self, cell, slots: torch.Tensor, page_size: int) -> tuple[torch.Tensor, torch.Tensor]:
         """(keys, values) [n, kv_heads, dim] in the run dtype of what the cell's pages hold at `slots` int32 [n], exactly; zeros for a

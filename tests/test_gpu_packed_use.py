@@ -294,6 +294,32 @@ def test_steps_of_growing_requests(kernels, dtype):
         assert torch.equal(torch.cat((keys, values), 1).double().cpu(), torch.cat(seen[index]))
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("pairing", ["adjacent", "half"])
+@pytest.mark.parametrize("heads,kv_heads,dim,tokens,spare", [(4, 2, 64, 7, 0), (12, 2, 128, 33, 0), (5, 1, 96, 9, 0), (3, 3, 32, 5, 0), (6, 2, 192, 65, 0), (2, 1, 256, 3, 0), (4, 2, 64, 7, 3), (7, 1, 224, 2, 5)])
+def test_rows_rotated_as_they_are_packed(kernels, dtype, pairing, heads, kv_heads, dim, tokens, spare):
+    """The rows and the pages are those of rotating first and packing then, bit by bit."""
+    k, page = kernels[dtype], 16
+    batch = packed_case(k, [tokens], [tokens], heads, kv_heads, dim, page, seed=dim + tokens)[0]
+    layout = HeadLayout(heads, kv_heads, dim, (heads + 2 * kv_heads) * dim + spare)
+    need, generator = PackedKeyValue(kv_heads, dim), torch.Generator().manual_seed(dim)
+    pages = -(-tokens // page) + 4
+    slots = torch.randperm((pages - 1) * page, generator=generator)[:tokens]
+    slots[tokens // 2] = -1 if dim % 128 else pages * page
+    batch.groups[0].slot_mapping.copy_(slots.int())
+    batch.positions.add_(11)
+    frequencies = 1.0 / (1000.0 ** (torch.arange(0, dim, 2, device="cuda").float() / dim))
+    rows = torch.randn((tokens, layout.stride), generator=generator).to(dtype).cuda()
+    rows[1, heads * dim + 3] = float("inf")
+    make = lambda: CacheCell(need, fields={"packed": torch.full((pages, kv_heads, need.page_bytes(page)), 255, dtype=torch.uint8, device="cuda")}, group=0)
+    apart, cell, other = rows.clone(), make(), make()
+    k.rotate_and_store(apart, layout, batch, None, frequencies, pairing)
+    k.store_packed(apart, layout, batch, other)
+    k.rotate_and_store(rows, layout, batch, cell, frequencies, pairing)
+    torch.testing.assert_close(rows, apart, atol=0, rtol=0, equal_nan=True)
+    assert torch.equal(cell.packed, other.packed)
+
+
 # ---------------------------------------------------------------------------- whole models
 
 
