@@ -126,7 +126,7 @@ def force(monkeypatch, k, least):
 
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("least", [(0, 0, False), (1, 0, False), (0, 1, False), (1, 1, False), (4, 8, False), (3, 40, False), (0, 0, True), (1, 1, True), (0, 8, True), (4, 33, True)])
-@pytest.mark.parametrize("heads,kv_heads,dim,page,window", [(12, 2, 128, 16, None), (6, 2, 96, 24, 300), (7, 1, 64, 8, None), (34, 2, 32, 16, None), (3, 1, 192, 40, 65), (4, 2, 256, 16, None)])
+@pytest.mark.parametrize("heads,kv_heads,dim,page,window", [(12, 2, 128, 16, None), (6, 2, 96, 24, 300), (7, 1, 64, 8, None), (34, 2, 32, 16, None), (3, 1, 192, 40, 65), (4, 2, 256, 16, None), (5, 1, 160, 16, None), (2, 1, 224, 8, None)])
 def test_walks_whole_and_cut_anywhere(kernels, dtype, least, heads, kv_heads, dim, page, window, monkeypatch):
     k = kernels[dtype]
     lengths, counts = [1300, 1, 530, 777, 40, 0, 260, 1025], [1, 1, 1, 45, 40, 0, 2, 70]
@@ -135,6 +135,97 @@ def test_walks_whole_and_cut_anywhere(kernels, dtype, least, heads, kv_heads, di
     got = k.paged_attention(qkv, layout, batch, cell, dim ** -0.5, window)
     assert_near(got, expected_of(found, lengths, counts, dim ** -0.5, window), largest_of(found, counts), dtype)
     assert torch.equal(got, k.paged_attention(qkv, layout, batch, cell, dim ** -0.5, window))  # sums in one order
+
+
+WAYS = [(0, 0, False), (1, 1, False), (0, 0, True), (1, 1, True)]
+
+
+def check(k, lengths, counts, heads, kv_heads, dim, page, scale, window=None, **more):
+    batch, cell, layout, qkv, found = packed_case(k, lengths, counts, heads, kv_heads, dim, page, window=window, **more)
+    got = k.paged_attention(qkv, layout, batch, cell, scale, window)
+    assert_near(got, expected_of(found, lengths, counts, scale, window), largest_of(found, counts), k.dtype)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("way", WAYS)
+@pytest.mark.parametrize("counts", [[1, 1], [40, 1], [3, 70]])
+def test_no_numbers_each_way(kernels, dtype, way, counts, monkeypatch):
+    def change(index, rows):  # [length, 4 q heads | 2 k heads | 2 v heads of 64]
+        if index == 0:
+            rows[90, 4 * 64 + 5] = float("nan")  # a key of kv head 0, seen by queries from 90 on
+            rows[80, 6 * 64 + 64 + 40] = float("inf")  # a value of kv head 1, second block
+        else:
+            rows[3, 6 * 64 + 1] = float("nan")  # before the window of most
+
+    force(monkeypatch, kernels[dtype], way)
+    check(kernels[dtype], [100, 75], counts, 4, 2, 64, 8, 0.125, 60, change=change, seed=3)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("way", WAYS)
+@pytest.mark.parametrize("window", [1, 31, 33, 64, 65, 200])
+def test_windows_each_way(kernels, dtype, way, window, monkeypatch):
+    force(monkeypatch, kernels[dtype], way)
+    check(kernels[dtype], [1, 40, 70, 341, 600, 290], [1, 1, 30, 141, 1, 200], 6, 2, 64, 8, 0.125, window, seed=window)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("way", WAYS)
+@pytest.mark.parametrize("place", [0, 37, 130, 199])
+def test_scores_far_apart_each_way(kernels, dtype, way, place, monkeypatch):
+    def change(index, rows):
+        rows[:, :64] *= 0.2
+        rows[place, 64:128] = 100.0 * torch.sign(rows[199, :64])
+
+    force(monkeypatch, kernels[dtype], way)
+    check(kernels[dtype], [200, 200], [1, 30], 1, 1, 64, 16, 1.0, change=change, seed=place)
+
+
+@pytest.mark.parametrize("way", WAYS)
+def test_rows_of_nobody_and_rows_anywhere_each_way(kernels, way, monkeypatch):
+    """Requests without tokens, rows behind the last request's, rows of an odd width from an odd element on, results into rows of an odd width."""
+    k = kernels[torch.bfloat16]
+    force(monkeypatch, k, way)
+    lengths, counts = [0, 20, 5, 260, 7], [0, 1, 0, 133, 0]
+    batch, cell, layout, qkv, found = packed_case(k, lengths, counts, 4, 2, 64, 8, row_stride=8 * 64 + 5)
+    rows = torch.zeros(137 * layout.stride + 8, dtype=qkv.dtype, device="cuda")[3:3 + 137 * layout.stride].view(137, layout.stride)
+    rows[:134].copy_(qkv)
+    out = torch.full((137 * 263 + 8,), 7.0, dtype=qkv.dtype, device="cuda")[1:1 + 137 * 263].view(137, 263)
+    assert k.paged_attention(rows, layout, batch, cell, 0.125, None, out=out) is out
+    assert bool((out[134:] == 7).all()) and bool((out[:, 256:] == 7).all())
+    assert_near(out[:134, :256], expected_of(found, lengths, counts, 0.125, None), max(v.abs().max() for _, _, v in found if v.numel()), k.dtype)
+
+
+@pytest.mark.parametrize("way", WAYS)
+def test_a_cache_beyond_32_bits(kernels, way, monkeypatch):
+    """Pages that begin behind the first 4 GiB."""
+    k, page, heads, kv_heads, dim = kernels[torch.bfloat16], 64, 4, 2, 128
+    force(monkeypatch, k, way)
+    lengths, counts = [700, 40, 300], [1, 1, 150]
+    batch, cell, layout, qkv, found = packed_case(k, lengths, counts, heads, kv_heads, dim, page, spare=0)
+    first = (1 << 32) // cell.packed[0].numel() + 1
+    wide = torch.empty((first + cell.packed.shape[0], *cell.packed.shape[1:]), dtype=torch.uint8, device="cuda")
+    wide[0] = 255
+    far = CacheCell(cell.need, fields={"packed": wide}, group=0)
+    tables = batch.groups[0].block_tables
+    step = dataclasses.replace(batch, groups=[dataclasses.replace(batch.groups[0], block_tables=torch.where(tables >= 0, tables + first, tables),
+                                                                  slot_mapping=batch.groups[0].slot_mapping + first * page)], scratch={})
+    wide[first:] = cell.packed
+    every = torch.arange(first * page, (first + 3) * page, dtype=torch.int32, device="cuda")
+    for mine, theirs in zip(k.packed_rows(far, every, page), k.packed_rows(cell, every - first * page, page)):
+        torch.testing.assert_close(mine, theirs, atol=0, rtol=0, equal_nan=True)
+    k.store_packed(qkv, layout, step, far)
+    assert torch.equal(wide[first:], cell.packed)  # (the step's rows were there already)
+    got = k.paged_attention(qkv, layout, step, far, dim ** -0.5, None)
+    assert torch.equal(got, k.paged_attention(qkv, layout, batch, cell, dim ** -0.5, None))
+    assert_near(got, expected_of(found, lengths, counts, dim ** -0.5, None), largest_of(found, counts), k.dtype)
+
+
+@pytest.mark.parametrize("page", [128, 1024, 1000])
+@pytest.mark.parametrize("way", WAYS)
+def test_large_pages(kernels, page, way, monkeypatch):
+    force(monkeypatch, kernels[torch.bfloat16], way)
+    check(kernels[torch.bfloat16], [page + 1, 2 * page - 1, 70], [1, 100, 70], 4, 2, 64, page, 0.125)
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
