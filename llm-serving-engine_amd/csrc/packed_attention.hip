@@ -1510,7 +1510,7 @@ static int launch(const void* q, int q_stride, void* out, int out_stride, const 
       const int whole_out = (size_t)out % 8 == 0 && out_stride % 4 == 0;
       packed_shared_kernel<<<(unsigned)blocks, PORTION_THREADS, 0, stream>>>((const T*)q, q_stride, (T*)out, out_stride, (const unsigned char*)pages, w, many, (int)items, whole, whole_out);
       if (int status = LAUNCH_STATUS()) return status;
-      if (many.least) packed_join_kernel<T><<<dim3(PORTION_WORKGROUPS, 8), 4 * WAVE, 0, stream>>>((T*)out, out_stride, many, SHARED_COLUMNS);
+      if (many.least) packed_join_kernel<T><<<dim3(PORTION_WORKGROUPS, SHARED_COLUMNS / 4), 4 * WAVE, 0, stream>>>((T*)out, out_stride, many, SHARED_COLUMNS);
       return LAUNCH_STATUS();
     }
   }
