@@ -1,6 +1,6 @@
 // Grouped-query attention over pages in 4 bits (packed.h), softmax in float32.  Compiled once per head size.
 //
-// A workgroup takes a run of up to 16 CT columns, the (token, query head) pairs of one request that share a kv head, and its four waves take steps
+// A workgroup takes a run of columns, the (token, query head) pairs of one request that share a kv head: 16 of them where they are few, and its waves take steps
 // of 32 keys in turn.  A step of a wave, with v_mfma_f32_16x16x32_bf16:
 //   S^T[key][column] = K[key][:] . Q[column][:]           A = rows of keys, two tiles of 16
 //   P = exp2(S * scale - the column's reference), masked to the keys that the column's token sees
@@ -314,13 +314,13 @@ template <typename T, int TERMS> __device__ __forceinline__ void split_eight(con
 }
 
 // What a wave keeps of its columns.
-template <typename T, int CT> struct Columns {
+template <typename T> struct Columns {
   static constexpr int TERMS = sizeof(T) == 4 ? 3 : 1;
-  Eight query[CT][TERMS][SLICES];
-  int position[CT];                           // of the lane's column's token
-  float reference[CT];                        // log2 of what weights are divided by
-  f32x4 total[CT];                            // sums of weights, the same number four times
-  f32x4 sum[CT][TILES];
+  Eight query[TERMS][SLICES];
+  int position;                               // of the lane's column's token
+  float reference;                            // log2 of what weights are divided by
+  f32x4 total;                                // sums of weights, the same number four times
+  f32x4 sum[TILES];
 };
 
 __device__ __forceinline__ f32x4 multiply(const Eight& a, const Eight& b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a.v, b.v, c, 0, 0, 0); }
@@ -328,69 +328,63 @@ __device__ __forceinline__ f32x4 multiply(const Eight& a, const Eight& b, f32x4 
 __device__ __forceinline__ float largest_of(const float* x) { return fmaxf(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])), fmaxf(fmaxf(x[4], x[5]), fmaxf(x[6], x[7]))); }
 
 // One step of 32 keys from `base` on.  EDGE: some column does not see some of them.
-template <bool EDGE, typename T, int CT>
-__device__ __forceinline__ void take_step(Columns<T, CT>& columns, const Step& now, const Walk& w, const Item& item, int base) {
-  constexpr int TERMS = Columns<T, CT>::TERMS;
+template <bool EDGE, typename T>
+__device__ __forceinline__ void take_step(Columns<T>& columns, const Step& now, const Walk& w, const Item& item, int base) {
+  constexpr int TERMS = Columns<T>::TERMS;
   const int lane = threadIdx.x % WAVE, r = lane & 15, g = lane >> 4;
   // scores: row 4 g + i of tile t is key 8 g + 4 t + i of the step
-  f32x4 score[CT][2];
+  f32x4 score[2];
 #pragma unroll
   for (int t = 0; t < 2; ++t) {
-#pragma unroll
-    for (int ct = 0; ct < CT; ++ct) score[ct][t] = (f32x4){0.f, 0.f, 0.f, 0.f};
+    score[t] = (f32x4){0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int s = 0; s < SLICES; ++s) {
       const float power = packed_power(now.key_powers[t][D % 128 == 0 ? s / 4 : D <= 64 ? 0 : s]);
       Eight key;
       key.u = (u32x4){unpack_pair<0>(now.keys[t][s], power), unpack_pair<1>(now.keys[t][s], power), unpack_pair<2>(now.keys[t][s], power), unpack_pair<3>(now.keys[t][s], power)};
 #pragma unroll
-      for (int ct = 0; ct < CT; ++ct)
-#pragma unroll
-        for (int k = TERMS - 1; k >= 0; --k) score[ct][t] = multiply(key, columns.query[ct][k][s], score[ct][t]);
+      for (int k = TERMS - 1; k >= 0; --k) score[t] = multiply(key, columns.query[k][s], score[t]);
     }
   }
-  const auto sees = [&](int ct, int i) {
+  const auto sees = [&](int i) {
     const int key = base + 8 * g + i;
-    return key <= columns.position[ct] && (w.window <= 0 || key > columns.position[ct] - w.window);
+    return key <= columns.position && (w.window <= 0 || key > columns.position - w.window);
   };
-  Eight weight[CT][TERMS];
-#pragma unroll
-  for (int ct = 0; ct < CT; ++ct) {
-    float x[8];  // log2 of the weights
-    const auto relative = [&]() {
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const float y = __builtin_fmaf(score[ct][i / 4][i % 4], w.scale, -columns.reference[ct]);
-        x[i] = !EDGE || sees(ct, i) ? y : -INFINITY;
-      }
-    };
-    relative();
-    if (__any(largest_of(x) > AHEAD)) {
-#pragma unroll
-      for (int i = 0; i < 8; ++i) x[i] = !EDGE || sees(ct, i) ? score[ct][i / 4][i % 4] * w.scale : -INFINITY;
-      float largest = largest_of(x);
-      largest = fmaxf(largest, __shfl_xor(largest, 16));
-      largest = fmaxf(largest, __shfl_xor(largest, 32));
-      largest = fmaxf(largest, columns.reference[ct]);
-      const float change = columns.reference[ct] == largest ? 1.f : __builtin_amdgcn_exp2f(columns.reference[ct] - largest);
-      columns.reference[ct] = largest;
-      columns.total[ct] *= change;
-#pragma unroll
-      for (int t = 0; t < TILES; ++t) columns.sum[ct][t] *= change;
-      relative();
-    }
+  Eight weight[TERMS];
+  float x[8];  // log2 of the weights
+  const auto relative = [&]() {
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      const float y = __builtin_amdgcn_exp2f(x[i]);
-      x[i] = !EDGE || sees(ct, i) ? y : 0.f;
+      const float y = __builtin_fmaf(score[i / 4][i % 4], w.scale, -columns.reference);
+      x[i] = !EDGE || sees(i) ? y : -INFINITY;
     }
-    split_eight<T, TERMS>(x, weight[ct]);
-    // the weights that are multiplied are the weights that are added up: by a product with ones, over all 32 keys at once
-    Eight ones;
-    ones.u = (u32x4){0x3f803f80u, 0x3f803f80u, 0x3f803f80u, 0x3f803f80u};
+  };
+  relative();
+  if (__any(largest_of(x) > AHEAD)) {
 #pragma unroll
-    for (int k = TERMS - 1; k >= 0; --k) columns.total[ct] = multiply(ones, weight[ct][k], columns.total[ct]);
+    for (int i = 0; i < 8; ++i) x[i] = !EDGE || sees(i) ? score[i / 4][i % 4] * w.scale : -INFINITY;
+    float largest = largest_of(x);
+    largest = fmaxf(largest, __shfl_xor(largest, 16));
+    largest = fmaxf(largest, __shfl_xor(largest, 32));
+    largest = fmaxf(largest, columns.reference);
+    const float change = columns.reference == largest ? 1.f : __builtin_amdgcn_exp2f(columns.reference - largest);
+    columns.reference = largest;
+    columns.total *= change;
+#pragma unroll
+    for (int t = 0; t < TILES; ++t) columns.sum[t] *= change;
+    relative();
   }
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const float y = __builtin_amdgcn_exp2f(x[i]);
+    x[i] = !EDGE || sees(i) ? y : 0.f;
+  }
+  split_eight<T, TERMS>(x, weight);
+  // the weights that are multiplied are the weights that are added up: by a product with ones, over all 32 keys at once
+  Eight ones;
+  ones.u = (u32x4){0x3f803f80u, 0x3f803f80u, 0x3f803f80u, 0x3f803f80u};
+#pragma unroll
+  for (int k = TERMS - 1; k >= 0; --k) columns.total = multiply(ones, weight[k], columns.total);
 #pragma unroll
   for (int c = 0; c < CHUNKS; ++c) {
     const int width = chunk_width(c), pairs = width / 32;  // pairs of elements that a lane takes of a key
@@ -439,75 +433,65 @@ __device__ __forceinline__ void take_step(Columns<T, CT>& columns, const Step& n
       }
       const int t = chunk_first(c) / 16 + 2 * e;
 #pragma unroll
-      for (int ct = 0; ct < CT; ++ct)
-#pragma unroll
-        for (int k = TERMS - 1; k >= 0; --k) {
-          columns.sum[ct][t] = multiply(even, weight[ct][k], columns.sum[ct][t]);
-          columns.sum[ct][t + 1] = multiply(odd, weight[ct][k], columns.sum[ct][t + 1]);
-        }
+      for (int k = TERMS - 1; k >= 0; --k) {
+        columns.sum[t] = multiply(even, weight[k], columns.sum[t]);
+        columns.sum[t + 1] = multiply(odd, weight[k], columns.sum[t + 1]);
+      }
     }
     if (EDGE && poisoned) {
+      Eight seen;
 #pragma unroll
-      for (int ct = 0; ct < CT; ++ct) {
-        Eight seen;
+      for (int i = 0; i < 8; ++i) seen.v[i] = (bf16_t)(sees(i) ? 1.f : 0.f);
+      const f32x4 hit = multiply(marks, seen, (f32x4){0.f, 0.f, 0.f, 0.f});
 #pragma unroll
-        for (int i = 0; i < 8; ++i) seen.v[i] = (bf16_t)(sees(ct, i) ? 1.f : 0.f);
-        const f32x4 hit = multiply(marks, seen, (f32x4){0.f, 0.f, 0.f, 0.f});
+      for (int e = 0; e < 8; ++e) {
+        if (e >= 2 * pairs) continue;
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          if (e >= 2 * pairs) continue;
-#pragma unroll
-          for (int i = 0; i < 4; ++i)
-            if (hit[i] > 0.f) columns.sum[ct][chunk_first(c) / 16 + e][i] = __uint_as_float(0x7fc00000u);
-        }
+        for (int i = 0; i < 4; ++i)
+          if (hit[i] > 0.f) columns.sum[chunk_first(c) / 16 + e][i] = __uint_as_float(0x7fc00000u);
       }
     }
   }
 }
 
 // Rows in memory as a wave's queries.
-template <typename T, int CT>
-__device__ __forceinline__ void load_queries(Columns<T, CT>& columns, const T* q, int q_stride, const Item& item, int kv_head, bool whole) {
-  constexpr int TERMS = Columns<T, CT>::TERMS;
+template <typename T>
+__device__ __forceinline__ void load_queries(Columns<T>& columns, const T* q, int q_stride, const Item& item, int kv_head, bool whole) {
+  constexpr int TERMS = Columns<T>::TERMS;
   const int lane = threadIdx.x % WAVE, r = lane & 15, g = lane >> 4;
+  const int column = min(r, item.columns - 1), flat = item.first + column, token = flat / item.group;
+  columns.position = item.first_position - item.first / item.group + token;
+  const T* row = q + (size_t)(item.first_row + token) * q_stride + (kv_head * item.group + flat - token * item.group) * D + g * (D / 4);
 #pragma unroll
-  for (int ct = 0; ct < CT; ++ct) {
-    const int column = min(ct * 16 + r, item.columns - 1), flat = item.first + column, token = flat / item.group;
-    columns.position[ct] = item.first_position - item.first / item.group + token;
-    const T* row = q + (size_t)(item.first_row + token) * q_stride + (kv_head * item.group + flat - token * item.group) * D + g * (D / 4);
+  for (int s = 0; s < SLICES; ++s) {
+    float x[8];
+    union { u32x4 v[sizeof(T) / 2]; T e[8]; } piece;
+    if (whole) {
 #pragma unroll
-    for (int s = 0; s < SLICES; ++s) {
-      float x[8];
-      union { u32x4 v[sizeof(T) / 2]; T e[8]; } piece;
-      if (whole) {
+      for (unsigned i = 0; i < sizeof(T) / 2; ++i) piece.v[i] = ((const u32x4*)(row + s * 8))[i];
+    } else {
 #pragma unroll
-        for (unsigned i = 0; i < sizeof(T) / 2; ++i) piece.v[i] = ((const u32x4*)(row + s * 8))[i];
-      } else {
-#pragma unroll
-        for (int e = 0; e < 8; ++e) piece.e[e] = row[s * 8 + e];
-      }
-#pragma unroll
-      for (int e = 0; e < 8; ++e) x[e] = to_float(piece.e[e]);
-      Eight terms[TERMS];
-      split_eight<T, TERMS>(x, terms);
-#pragma unroll
-      for (int k = 0; k < TERMS; ++k) columns.query[ct][k][s] = terms[k];
+      for (int e = 0; e < 8; ++e) piece.e[e] = row[s * 8 + e];
     }
-    columns.reference[ct] = -INFINITY;
-    columns.total[ct] = (f32x4){0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-    for (int t = 0; t < TILES; ++t) columns.sum[ct][t] = (f32x4){0.f, 0.f, 0.f, 0.f};
+    for (int e = 0; e < 8; ++e) x[e] = to_float(piece.e[e]);
+    Eight terms[TERMS];
+    split_eight<T, TERMS>(x, terms);
+#pragma unroll
+    for (int k = 0; k < TERMS; ++k) columns.query[k][s] = terms[k];
   }
+  columns.reference = -INFINITY;
+  columns.total = (f32x4){0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+  for (int t = 0; t < TILES; ++t) columns.sum[t] = (f32x4){0.f, 0.f, 0.f, 0.f};
 }
 
 // What a wave holds of its queries stays in registers from here on.
-template <typename T, int CT> __device__ __forceinline__ void settle(Columns<T, CT>& columns) {
+template <typename T> __device__ __forceinline__ void settle(Columns<T>& columns) {
 #pragma unroll
-  for (int ct = 0; ct < CT; ++ct)
+  for (int k = 0; k < Columns<T>::TERMS; ++k)
 #pragma unroll
-    for (int k = 0; k < Columns<T, CT>::TERMS; ++k)
-#pragma unroll
-      for (int s = 0; s < SLICES; ++s) asm volatile("" : "+v"(columns.query[ct][k][s].u));
+    for (int s = 0; s < SLICES; ++s) asm volatile("" : "+v"(columns.query[k][s].u));
 }
 
 // A wave's steps of the keys begin .. end (begin a multiple of 32): every W-th from its own on.  ring: STAGES stages of LDS that are its own.
@@ -580,14 +564,14 @@ __device__ __forceinline__ void join_waves(const float (*results)[16][D + 4], co
 
 // The sums of W waves, brought together through LDS.  memory: W * 16 * (D + 6) floats, free when all waves have come here.
 template <int W, typename T, typename Take>
-__device__ __forceinline__ void bring_together(const Columns<T, 1>& columns, int count, int wave, unsigned char* memory, Take take) {
+__device__ __forceinline__ void bring_together(const Columns<T>& columns, int count, int wave, unsigned char* memory, Take take) {
   float (*results)[16][D + 4] = (float (*)[16][D + 4])memory;
   float (*sums)[16][2] = (float (*)[16][2])(memory + W * 16 * (D + 4) * 4);
   const int lane = threadIdx.x % WAVE, r = lane & 15, g = lane >> 4;
   __syncthreads();
   if (g == 0) {
-    sums[wave][r][0] = columns.reference[0];
-    sums[wave][r][1] = columns.total[0][0];
+    sums[wave][r][0] = columns.reference;
+    sums[wave][r][1] = columns.total[0];
   }
 #pragma unroll
   for (int c = 0; c < CHUNKS; ++c) {
@@ -596,7 +580,7 @@ __device__ __forceinline__ void bring_together(const Columns<T, 1>& columns, int
     for (int i = 0; i < 4; ++i)
 #pragma unroll
       for (int e = 0; e < 8; ++e)
-        if (e < each) results[wave][r][chunk_first(c) + (4 * g + i) * each + e] = columns.sum[0][chunk_first(c) / 16 + e][i];
+        if (e < each) results[wave][r][chunk_first(c) + (4 * g + i) * each + e] = columns.sum[chunk_first(c) / 16 + e][i];
   }
   __syncthreads();
   join_waves<W>(results, sums, count, take);
@@ -646,7 +630,7 @@ __global__ void __launch_bounds__(WAVES * WAVE, 2) packed_streams_kernel(const T
   const int lane = threadIdx.x % WAVE, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / WAVE), group = w.heads / w.kv_heads;
   unsigned char* ring = memory + wave * (STAGES * STAGE);
   const auto take_walk = [&](const Item& item, int kv_head, int begin, int end, float* part) {
-    Columns<T, 1> columns;
+    Columns<T> columns;
     walk_keys<T, Step, WAVES>(columns, q, q_stride, pages, w, item, kv_head, whole, begin, end, wave, ring);
     bring_together<WAVES>(columns, item.columns, wave, memory, [&](int column, int d, f32x4 result, float largest, float weights) {
       if (part) {
@@ -1027,7 +1011,7 @@ template <typename T> constexpr bool WIDE = sizeof(T) == 2 && D % 64 == 0;
 template <typename T> constexpr int PORTION_COLUMNS = WIDE<T> ? 32 : 16;
 template <typename T> constexpr int PORTION_PART = PORTION_COLUMNS<T> * (D + 4);
 template <typename T, bool> struct PortionOf {
-  typedef Columns<T, 1> Cols;
+  typedef Columns<T> Cols;
   typedef Step Taken;
 };
 template <typename T> struct PortionOf<T, true> {

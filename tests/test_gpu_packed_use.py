@@ -230,10 +230,11 @@ def test_large_pages(kernels, page, way, monkeypatch):
 
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("least", [None, (1, 0, False), (0, 0, True)])
-def test_many_requests(kernels, dtype, least, monkeypatch):
-    """More requests than a workgroup has threads for, portions among them (which are then never cut)."""
+@pytest.mark.parametrize("requests", [300, 700])
+def test_many_requests(kernels, dtype, least, requests, monkeypatch):
+    """More requests than a workgroup has threads for (256 over many columns, 512 over few), portions among them (which are then never cut)."""
     k = kernels[dtype]
-    lengths = [1 + (index * 37) % 90 for index in range(300)]
+    lengths = [1 + (index * 37) % 90 for index in range(requests)]
     counts = [1 if index % 50 else min(length, 30) for index, length in enumerate(lengths)]
     if least is not None:
         force(monkeypatch, k, least)
