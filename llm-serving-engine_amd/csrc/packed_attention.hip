@@ -62,6 +62,7 @@ struct Walk {
   const int *query_start, *contexts;
   int requests, heads, kv_heads, window;
   float scale;                                // times log2 e
+  bool together;                              // those of few columns go with the others
 };
 
 struct Item {                                 // a run of columns
@@ -69,7 +70,7 @@ struct Item {                                 // a run of columns
 };
 
 // Few columns: those of a single token, or of some that fit one tile of 16.
-__device__ __forceinline__ bool few_columns(int count, int group) { return count == 1 || count * group <= 16; }
+__device__ __forceinline__ bool few_columns(const Walk& w, int count, int group) { return !w.together && (count == 1 || count * group <= 16); }
 
 struct Request {
   int start, count, context;                  // rows in the step, keys behind it
@@ -101,7 +102,7 @@ __device__ __forceinline__ bool find_item(const Walk& w, int index, int most, It
   int before = 0;
   for (int base = 0; base < w.requests; base += WAVE) {
     const int b = base + lane, count = b < w.requests ? w.query_start[b + 1] - w.query_start[b] : 0;
-    const int items = few_columns(count, group) ? 0 : (count * group + most - 1) / most;
+    const int items = few_columns(w, count, group) ? 0 : (count * group + most - 1) / most;
     int sum = items;
 #pragma unroll
     for (int step = 1; step < WAVE; step <<= 1) {
@@ -617,7 +618,7 @@ struct Streams {
 __device__ __forceinline__ int units_of(const Walk& w, const Request& request) {  // of all its columns and kv heads
   const int group = w.heads / w.kv_heads;
   Item item;
-  if (!few_columns(request.count, group) || !make_item(w, 0, request, 0, 1 << 20, item)) return 0;
+  if (!few_columns(w, request.count, group) || !make_item(w, 0, request, 0, 1 << 20, item)) return 0;
   return (item.to - item.from + UNIT - 1) / UNIT * ((request.count * group + 15) / 16) * w.kv_heads;
 }
 
@@ -646,7 +647,7 @@ __global__ void __launch_bounds__(WAVES * WAVE, 2) packed_streams_kernel(const T
     const int tiles = (group + 15) / 16, request = blockIdx.x / (tiles * w.kv_heads), inside = blockIdx.x - request * (tiles * w.kv_heads);
     const Request mine = load_request(w, request);
     Item item;
-    if (!few_columns(mine.count, group) || !make_item(w, request, mine, inside / w.kv_heads * 16, 16, item)) return;
+    if (!few_columns(w, mine.count, group) || !make_item(w, request, mine, inside / w.kv_heads * 16, 16, item)) return;
     take_walk(item, inside % w.kv_heads, item.from, item.to, nullptr);
     return;
   }
@@ -1076,7 +1077,7 @@ __device__ __forceinline__ void take_walks(const Walk& w, const Streams& streams
     if ((int)threadIdx.x < w.requests) {
       shares.held[threadIdx.x] = load_request(w, threadIdx.x);
       const int tokens = shares.held[threadIdx.x].count;
-      count = few_columns(tokens, group) ? 0 : (max(tokens, 0) * group + COLUMNS - 1) / COLUMNS;
+      count = few_columns(w, tokens, group) ? 0 : (max(tokens, 0) * group + COLUMNS - 1) / COLUMNS;
     }
     shares.item_ends[threadIdx.x] = added_up(count, shares.wave_sums[0]);
     __syncthreads();
@@ -1513,7 +1514,7 @@ extern "C" int llmserve_packed_attention_workspace(int kind) {
 
 // q's heads are the first columns of rows of q_stride; tokens, requests: as many rows and requests as the arrays hold.  kinds: 1: some requests may have few columns (a
 // single token, or no more than 16 of them in all), 2: some may have more, 4: those share tiles of keys
-// (bfloat16).  few_least, many_least: 0: a walk over the keys of few (many) columns is taken whole by one workgroup; else every
+// (bfloat16), 8 (and not 1): all go as those of many.  few_least, many_least: 0: a walk over the keys of few (many) columns is taken whole by one workgroup; else every
 // workgroup takes at least so many units of 256 (128; that share, 64) keys, walks are cut, and there is a workspace.  Those of many columns are cut for up to 256 requests alone.
 extern "C" int llmserve_packed_attention(const void* q, int is_float, int q_stride, void* out, int out_stride, void* few_workspace, void* many_workspace, const void* pages, int num_pages, const int* tables,
                                          int table_width, const int* query_start, const int* contexts, int requests, int tokens, int heads, int kv_heads, int page_size, float scale, int window, int kinds,
@@ -1521,14 +1522,14 @@ extern "C" int llmserve_packed_attention(const void* q, int is_float, int q_stri
   if (tokens == 0 || requests == 0) return 0;
   if (!q || !out || !pages || !tables || !query_start || !contexts || requests < 0 || tokens < 0 || kv_heads <= 0 || heads <= 0 || heads % kv_heads || num_pages <= 0 || table_width <= 0 ||
       !packed_fits(D, page_size) || (long)page_size * D * kv_heads >= (1L << 30) || !(scale > 0.f) || (size_t)pages % 16 || q_stride < heads * D || out_stride < heads * D || window < 0 ||
-      kinds < 1 || kinds > 7 || kinds == 4 || (is_float && (kinds & 4)) || few_least < 0 || (few_least > 0 && (!few_workspace || (size_t)few_workspace % 16)) || many_least < 0 ||
+      (kinds & 3) == 0 || kinds < 1 || kinds > 15 || (is_float && (kinds & 4)) || ((kinds & 8) && (kinds & 3) != 2) || few_least < 0 || (few_least > 0 && (!few_workspace || (size_t)few_workspace % 16)) || many_least < 0 ||
       (many_least > 0 && (!many_workspace || (size_t)many_workspace % 16 || requests > PORTION_THREADS)))
     return ERR_BAD_ARGUMENT;
   const unsigned per_page = (unsigned)page_size / 8;
   const bool power_of_two = (per_page & (per_page - 1)) == 0;
   // (a quotient by the reciprocal is exact below 2^32 over the divisor; pieces up to a few tiles beyond the tables are asked for)
   if (!power_of_two && ((unsigned long)table_width * per_page + 64) * per_page >= (1UL << 32)) return ERR_BAD_ARGUMENT;
-  const Walk w = {tables, table_width, num_pages, page_size, power_of_two ? 31 - __builtin_clz(per_page) : -1, (unsigned)(((1UL << 32) + per_page - 1) / per_page), query_start, contexts, requests, heads, kv_heads, window, scale * LOG2_E};
+  const Walk w = {tables, table_width, num_pages, page_size, power_of_two ? 31 - __builtin_clz(per_page) : -1, (unsigned)(((1UL << 32) + per_page - 1) / per_page), query_start, contexts, requests, heads, kv_heads, window, scale * LOG2_E, (kinds & 8) != 0};
   const Streams few = {(float*)few_workspace, (Cut*)((float*)few_workspace + WORKGROUPS * 2 * PART), few_least};
   const bool shared = kinds & 4;
   const Streams many = {(float*)many_workspace, (Cut*)((float*)many_workspace + PORTION_WORKGROUPS * 2 * (shared ? SHARED_COLUMNS : 32) * (D + 4)), many_least};

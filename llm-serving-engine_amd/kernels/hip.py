@@ -1790,19 +1790,19 @@ class HipKernels:
 
     @staticmethod
     def _packed_walks(batch, group: int, window: int) -> tuple:
-        """(1: no request has many columns, 2: none has few, 3; the longest walk over the keys of few columns; of many: their tokens, the longest walk, sums over the
-        requests' tokens of the shortest walk and of the mean one).  Few columns are those of a single token or of up to 16 query heads a kv head in all.  A captured step is replayed with
+        """(1: no request has many columns, 2: none has few, 3; of requests of few columns: the longest walk, the sum of all, how many; of many: their tokens, the longest walk, sums
+        over the requests' tokens of the shortest walk and of the mean one).  Few columns are those of a single token or of up to 16 query heads a kv head in all.  A captured step is replayed with
         other requests: any of either kind, the longest."""
         longest = min(batch.max_context_length, window + 31) if window else batch.max_context_length
         if batch.max_query_length <= 1:
-            return 1, longest, 0, 0, 0, 0
+            return 1, longest, 0, 0, 0, 0, 0, 0
         if getattr(batch, "padded_to", None) is not None:
             tokens = batch.padded_to[0]
-            return 3, longest, tokens, longest, tokens * longest, tokens * longest
+            return 3, longest, batch.padded_to[1] * longest, batch.padded_to[1], tokens, longest, tokens * longest, tokens * longest
         known = batch.scratch.get(("packed walks", group, window))
         if known is not None:
             return known
-        few = many = tokens = shortest = mean = 0
+        few = fews = few_keys = many = tokens = shortest = mean = 0
         for chunk in batch.chunks:
             count, end = chunk.count, chunk.start + chunk.count
             if count > 1 and count * group > 16:
@@ -1812,19 +1812,22 @@ class HipKernels:
                 shortest += count * first
                 mean += count * (first + last) // 2
             else:
-                few = max(few, min(end, window + 31) if window else end)
-        known = batch.scratch[("packed walks", group, window)] = (1 if tokens == 0 else 2 if few == 0 else 3), few, tokens, many, shortest, mean
+                last = min(end, window + 31) if window else end
+                few = max(few, last)
+                few_keys += last
+                fews += 1
+        known = batch.scratch[("packed walks", group, window)] = (1 if tokens == 0 else 2 if few == 0 else 3), few, few_keys, fews, tokens, many, shortest, mean
         return known
 
     @staticmethod
-    def _packed_way(walks: tuple, requests: int, group: int, kv_heads: int, shares: bool) -> tuple[int, int, bool]:
-        """(units of 256 keys that a workgroup takes at least of walks over the keys of few columns, units of 128 or 64 of those of many, whether the latter share tiles
-        of keys, which `shares` allows): walks are cut anywhere; 0: every walk is taken whole."""
-        _, few, tokens, many, shortest, mean = walks
-        pairs = requests * kv_heads * -(-group // 16)
+    def _packed_way(walks: tuple, requests: int, group: int, kv_heads: int, shares: bool) -> tuple[int, int, int]:
+        """(units of 256 keys that a workgroup takes at least of walks over the keys of few columns, units of 128 or 64 of those of many, 4: the latter share tiles
+        of keys, which `shares` allows, 8: those of few go with those of many, else 0): walks are cut anywhere; 0 units: every walk is taken whole."""
+        kinds, longest, few_keys, fews, tokens, many, shortest, mean = walks
+        few, pairs = longest, requests * kv_heads * -(-group // 16)
         few = 0 if few <= 1024 or 22 * few <= 50000 + 3 * pairs * few // 10 else 4
         if tokens == 0:
-            return few, 0, False
+            return few, 0, 0
         # Of many columns.  Whole, a workgroup of 32 columns takes 8.25 us for 1,000 keys where it is alone on its unit (up to 256 of them), 11.5 beside another,
         # one of 128 that share tiles 27.4 and 34.7; a walk's beginning and end take as long as 700 (420) keys, and 512 fit.  So it is the longest walk, or rounds of the keys that all walks have in
         # common and the sum of the rest, the longest first.  Cut, it is the sum of all walks, and what the joining takes.  us, measured (and estimated), whole, cut, shared whole, shared and cut:
@@ -1832,20 +1835,27 @@ class HipKernels:
         # 28 heads on 4, 2,048 76, 98, 68 (62), 87; behind 10,000 455, 515, 399 (398), 418.  40 heads on 8, 512 24 (22), 36, 22 (20), 43; 2,048 behind 10,000 634, 720, 636, 591 (590).
         columns, common, rest = tokens * group * kv_heads, shortest / tokens / 1000, (mean - shortest) / tokens / 1000
 
-        def whole(width: int, alone: float, beside: float, extra: float) -> float:
+        def whole(width: int, alone: float, beside: float, extra: float, others: int = 0, keys: int = 0) -> float:
             items = -(-columns // width)
             full, left = divmod(items, 512)
-            rounds = beside * full + (0.0 if left == 0 else alone if left <= 256 else beside)
-            return max(alone * many / 1000, common * rounds + beside / 512 * items * (rest + extra))
+            rounds = beside * full + (0.0 if left == 0 else alone if left + others <= 256 else beside)
+            return max(alone * max(many, longest if others else 0) / 1000, common * rounds + beside / 512 * (items * (rest + extra) + others * extra + keys / 1000))
 
-        ways = [(8.0 + whole(32, 8.25, 11.5, 0.7), 0, False)]
+        ways = [(8.0 + whole(32, 8.25, 11.5, 0.7), 0, 0)]
         if requests <= 256:
-            ways.append((21.0 + 0.0235 * columns / 32 * (common + rest + 0.5), 8, False))
+            ways.append((21.0 + 0.0235 * columns / 32 * (common + rest + 0.5), 8, 0))
         if shares:
-            ways.append((6.0 + whole(128, 27.4, 34.7, 0.42), 0, True))
+            ways.append((6.0 + whole(128, 27.4, 34.7, 0.42), 0, 4))
             if requests <= 256:
-                ways.append((44.0 + 0.077 * columns / 128 * (common + rest), 8, True))
-        return few, *min(ways)[1:]
+                ways.append((44.0 + 0.077 * columns / 128 * (common + rest), 8, 4))
+        best = min(ways)
+        if kinds == 3 and few == 0:
+            # A kernel of their own, behind the other, takes 5 us and 5.5 for 1,000 keys of the longest; with the others they are more walks of that kernel, slower ones.  us, apart and together:
+            # 28 heads on 4, 31 tokens at 640 beside 256 behind 300 25 and 19.5, 63 at 1,500 36 and 31, 32 at 4,000 49 and 63; 12 on 2, 8 at 600 beside 1,024 29 and 20.
+            walked = kv_heads * -(-group // 32)
+            if 8.0 + whole(32, 8.25, 11.5, 0.7, walked * fews, walked * few_keys) < best[0] + 5.0 + 5.5 * longest / 1000:
+                return 0, 0, 8
+        return few, *best[1:]
 
     def _packed_attention(self, qkv, layout, batch, cell, scale: float, window: int | None, out):
         tokens, heads, kv_heads, dim = qkv.shape[0], layout.num_heads, layout.num_kv_heads, layout.head_dim
@@ -1865,12 +1875,12 @@ class HipKernels:
         # (tiles of heads of 160 and 192 keep five and six of eight threads busy: 2,048 tokens behind 10,000 keys at 12/2 heads of 160 441 us apart, 476 shared, at 16/4 of 192 593 and 667,
         # but at 16/2 of 224 1,182 and 700, of 256 697 and 606)
         shares = qkv.dtype == torch.bfloat16 and not 128 < dim < 224
-        few, many, shared = self._packed_way(walks, requests, heads // kv_heads, kv_heads, shares)
-        spaces = [self._empty((library.llmserve_packed_attention_workspace(kind),), torch.float32) if least else None for kind, least in ((0, few), (2 if shared else 1, many))]
+        few, many, how = self._packed_way(walks, requests, heads // kv_heads, kv_heads, shares)
+        spaces = [self._empty((library.llmserve_packed_attention_workspace(kind),), torch.float32) if least else None for kind, least in ((0, few), (2 if how == 4 else 1, many))]
         status = library.llmserve_packed_attention(
             _pointer(qkv), _is_float(qkv), layout.stride, _pointer(out), out.shape[1], _pointer(spaces[0]), _pointer(spaces[1]), _pointer(pages), pages.shape[0],
             _pointer(group.block_tables), group.width, _pointer(batch.query_start), _pointer(batch.context_lengths), requests, tokens, heads, kv_heads, group.page_size, scale, window,
-            walks[0] + (4 if shared else 0), few, many, self._stream,
+            2 + how if how == 8 else walks[0] + how, few, many, self._stream,
         )
         _check(status, "paged_attention over 4 bits")
         return out

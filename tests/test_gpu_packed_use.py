@@ -120,12 +120,12 @@ def test_refusals_of_index_arrays(kernels):
 
 
 def force(monkeypatch, k, least):
-    """Walks in the given way, tiles shared where they can be."""
-    monkeypatch.setattr(type(k), "_packed_way", staticmethod(lambda *given: (*least[:2], least[2] and k.dtype == torch.bfloat16)))
+    """Walks in the given way (4: tiles shared where they can be, 8: few columns with many where a step has both, or many)."""
+    monkeypatch.setattr(type(k), "_packed_way", staticmethod(lambda *given: (*least[:2], least[2] if least[2] == 8 or k.dtype == torch.bfloat16 else 0)))
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
-@pytest.mark.parametrize("least", [(0, 0, False), (1, 0, False), (0, 1, False), (1, 1, False), (4, 8, False), (3, 40, False), (0, 0, True), (1, 1, True), (0, 8, True), (4, 33, True)])
+@pytest.mark.parametrize("least", [(0, 0, 0), (1, 0, 0), (0, 1, 0), (1, 1, 0), (4, 8, 0), (3, 40, 0), (0, 0, 4), (1, 1, 4), (0, 8, 4), (4, 33, 4), (0, 0, 8), (1, 1, 8)])
 @pytest.mark.parametrize("heads,kv_heads,dim,page,window", [(12, 2, 128, 16, None), (6, 2, 96, 24, 300), (7, 1, 64, 8, None), (34, 2, 32, 16, None), (3, 1, 192, 40, 65), (4, 2, 256, 16, None), (5, 1, 160, 16, None), (2, 1, 224, 8, None)])
 def test_walks_whole_and_cut_anywhere(kernels, dtype, least, heads, kv_heads, dim, page, window, monkeypatch):
     k = kernels[dtype]
@@ -137,7 +137,7 @@ def test_walks_whole_and_cut_anywhere(kernels, dtype, least, heads, kv_heads, di
     assert torch.equal(got, k.paged_attention(qkv, layout, batch, cell, dim ** -0.5, window))  # sums in one order
 
 
-WAYS = [(0, 0, False), (1, 1, False), (0, 0, True), (1, 1, True)]
+WAYS = [(0, 0, 0), (1, 1, 0), (0, 0, 4), (1, 1, 4), (0, 0, 8)]
 
 
 def check(k, lengths, counts, heads, kv_heads, dim, page, scale, window=None, **more):
@@ -229,7 +229,7 @@ def test_large_pages(kernels, page, way, monkeypatch):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
-@pytest.mark.parametrize("least", [None, (1, 0, False), (0, 0, True)])
+@pytest.mark.parametrize("least", [None, (1, 0, 0), (0, 0, 4), (0, 0, 8)])
 @pytest.mark.parametrize("requests", [300, 700])
 def test_many_requests(kernels, dtype, least, requests, monkeypatch):
     """More requests than a workgroup has threads for (256 over many columns, 512 over few), portions among them (which are then never cut)."""
@@ -257,13 +257,14 @@ def test_which_way_walks_go():
         assert walks == HipKernels._packed_walks(batch, heads // kv_heads, window)
         return walks[0], *HipKernels._packed_way(walks, len(chunks), heads // kv_heads, kv_heads, shares)
 
-    assert way([(639, 1)], 12, 2) == (1, 0, 0, False)
-    assert way([(29999, 1)] * 8, 40, 8) == (1, 4, 0, False) and way([(29999, 1)] * 8, 40, 8, 512) == (1, 0, 0, False)
-    assert way([(0, 2047)], 12, 2) == (2, 0, 0, False)
-    assert way([(30000, 128)], 12, 2) == (2, 0, 8, False) and way([(30000, 128)], 12, 2, 512) == (2, 0, 0, False)
-    assert way([(30000, 2048)], 12, 2) == (2, 0, 8, True) and not way([(30000, 2048)], 12, 2, shares=False)[3]
-    assert way([(0, 8192)], 40, 8) == (2, 0, 0, True)
-    assert way([(600, 1)] * 31 + [(300, 256)], 28, 4) == (3, 0, 0, False)  # the long context is not of the single tokens
+    assert way([(639, 1)], 12, 2) == (1, 0, 0, 0)
+    assert way([(29999, 1)] * 8, 40, 8) == (1, 4, 0, 0) and way([(29999, 1)] * 8, 40, 8, 512) == (1, 0, 0, 0)
+    assert way([(0, 2047)], 12, 2) == (2, 0, 0, 0)
+    assert way([(30000, 128)], 12, 2) == (2, 0, 8, 0) and way([(30000, 128)], 12, 2, 512) == (2, 0, 0, 0)
+    assert way([(30000, 2048)], 12, 2) == (2, 0, 8, 4) and not way([(30000, 2048)], 12, 2, shares=False)[3]
+    assert way([(0, 8192)], 40, 8) == (2, 0, 0, 4)
+    assert way([(600, 1)] * 31 + [(300, 256)], 28, 4) == (3, 0, 0, 8)  # the single tokens go with the portion
+    assert way([(20000, 1)] * 31 + [(300, 256)], 28, 4)[3] == 0 and way([(600, 1)] * 31 + [(30000, 256)], 28, 4)[1:3] == (0, 8)
     assert way([(40, 2)] * 256 + [(30000, 128)], 12, 2)[:3] == (3, 0, 0)  # more requests than are cut for
     assert way([(600, 1)] * 3 + [(300, 256)], 28, 4, padded_to=(300, 5))[0] == 3 and way([(300, 256)], 28, 4, padded_to=(300, 5))[0] == 3
 
@@ -291,7 +292,7 @@ def test_another_stream(kernels, dtype):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
-@pytest.mark.parametrize("least", [(1, 1, False), (0, 0, False), (1, 1, True), (0, 0, True)])
+@pytest.mark.parametrize("least", [(1, 1, 0), (0, 0, 0), (1, 1, 4), (0, 0, 4), (0, 0, 8)])
 def test_captured_and_replayed(kernels, dtype, least, monkeypatch):
     """Two captured steps of different cells, replayed in turn with eager calls between them and with lengths, queries and pages changed under them: index arrays,
     store and attention in one graph."""
