@@ -1794,13 +1794,20 @@ class HipKernels:
         over the requests' tokens of the shortest walk and of the mean one).  Few columns are those of a single token or of up to 16 query heads a kv head in all.  A captured step is replayed with
         other requests: any of either kind, the longest."""
         longest = min(batch.max_context_length, window + 31) if window else batch.max_context_length
-        if batch.max_query_length <= 1:
-            return 1, longest, 0, 0, 0, 0, 0, 0
-        if getattr(batch, "padded_to", None) is not None:
-            tokens = batch.padded_to[0]
-            return 3, longest, batch.padded_to[1] * longest, batch.padded_to[1], tokens, longest, tokens * longest, tokens * longest
+        if getattr(batch, "padded_to", None) is not None and batch.max_query_length > 1:
+            tokens, requests = batch.padded_to
+            return 3, longest, requests * longest, requests, tokens, longest, tokens * longest, tokens * longest
         known = batch.scratch.get(("packed walks", group, window))
         if known is not None:
+            return known
+        if batch.max_query_length <= 1:
+            ends = [chunk.start + chunk.count for chunk in batch.chunks]
+            requests = batch.context_lengths.shape[0]
+            if max(ends, default=0) == batch.max_context_length:
+                keys = sum(min(end, window + 31) if window else end for end in ends)
+            else:  # (a captured step: the contexts that its tables have room for)
+                keys = requests * longest
+            known = batch.scratch[("packed walks", group, window)] = 1, longest, keys, requests, 0, 0, 0, 0
             return known
         few = fews = few_keys = many = tokens = shortest = mean = 0
         for chunk in batch.chunks:
@@ -1824,8 +1831,13 @@ class HipKernels:
         """(units of 256 keys that a workgroup takes at least of walks over the keys of few columns, units of 128 or 64 of those of many, 4: the latter share tiles
         of keys, which `shares` allows, 8: those of few go with those of many, else 0): walks are cut anywhere; 0 units: every walk is taken whole."""
         kinds, longest, few_keys, fews, tokens, many, shortest, mean = walks
-        few, pairs = longest, requests * kv_heads * -(-group // 16)
-        few = 0 if few <= 1024 or 22 * few <= 50000 + 3 * pairs * few // 10 else 4
+        # Of few columns.  Whole, a workgroup takes 4.7 us for 1,000 keys where it has a unit to itself (up to 256 of them) and 7.2 beside another, and all of them
+        # 26 ns for 1,000 keys; cut, that, and 13 us for the joining, 20 in all at least.  us, whole and cut (measured, contexts from half the mean to one and a half): 12 heads on 2, 1 token at
+        # 1,000 keys 11 and 15, at 4,000 25 and 16, 64 at 2,000 21 and 25, at 8,000 61 and 39; 28 on 4, 64 at 4,000 37 and 40; 40 on 8, 16 at 20,000 144 and 73, 160 at 4,000 131 and 144.
+        each = kv_heads * -(-group // 16)
+        walked = 0.0262 * few_keys * each / 1000
+        few_whole, few_cut = max(6.5 + (4.7 if fews * each <= 256 else 7.2) * longest / 1000, 6.0 + walked), max(16.0 if fews == 1 else 20.0, 13.0 + walked)
+        few = 0 if few_whole <= few_cut else 4
         if tokens == 0:
             return few, 0, 0
         # Of many columns.  Whole, a workgroup of 32 columns takes 8.25 us for 1,000 keys where it is alone on its unit (up to 256 of them), 11.5 beside another,
@@ -1839,7 +1851,10 @@ class HipKernels:
             items = -(-columns // width)
             full, left = divmod(items, 512)
             rounds = beside * full + (0.0 if left == 0 else alone if left + others <= 256 else beside)
-            return max(alone * max(many, longest if others else 0) / 1000, common * rounds + beside / 512 * (items * (rest + extra) + others * extra + keys / 1000))
+            # (the others' walks begin behind the portions' where not all fit)
+            late = beside * (common + rest + extra) if others and items + others > 512 else 0.0
+            most = max(alone * many / 1000, alone * longest / 1000 + late if others else 0.0)
+            return max(most, common * rounds + beside / 512 * (items * (rest + extra) + others * extra + keys / 1000))
 
         ways = [(8.0 + whole(32, 8.25, 11.5, 0.7), 0, 0)]
         if requests <= 256:
@@ -1849,11 +1864,11 @@ class HipKernels:
             if requests <= 256:
                 ways.append((44.0 + 0.077 * columns / 128 * (common + rest), 8, 4))
         best = min(ways)
-        if kinds == 3 and few == 0:
-            # A kernel of their own, behind the other, takes 5 us and 5.5 for 1,000 keys of the longest; with the others they are more walks of that kernel, slower ones.  us, apart and together:
-            # 28 heads on 4, 31 tokens at 640 beside 256 behind 300 25 and 19.5, 63 at 1,500 36 and 31, 32 at 4,000 49 and 63; 12 on 2, 8 at 600 beside 1,024 29 and 20.
-            walked = kv_heads * -(-group // 32)
-            if 8.0 + whole(32, 8.25, 11.5, 0.7, walked * fews, walked * few_keys) < best[0] + 5.0 + 5.5 * longest / 1000:
+        if kinds == 3:
+            # With the others they are more walks of that kernel, slower ones.  us, apart and together: 28 heads on 4, 31 tokens at 640 beside 256 behind 300 25 and 19.5, 63 at 1,500 36
+            # and 31, 32 at 4,000 49 and 63; 12 on 2, 8 at 600 beside 1,024 29 and 20.
+            each = kv_heads * -(-group // 32)
+            if 8.0 + whole(32, 8.25, 11.5, 0.7, each * fews, each * few_keys) < best[0] + min(few_whole, few_cut):
                 return 0, 0, 8
         return few, *best[1:]
 

@@ -251,7 +251,7 @@ def test_which_way_walks_go():
     from llmserve_amd.kernels import HipKernels
 
     def way(chunks, heads, kv_heads, window=0, shares=True, padded_to=None):
-        batch = SimpleNamespace(max_context_length=max(start + count for start, count in chunks), max_query_length=max(count for _, count in chunks), padded_to=padded_to, scratch={},
+        batch = SimpleNamespace(max_context_length=max(start + count for start, count in chunks), max_query_length=max(count for _, count in chunks), padded_to=padded_to, scratch={}, context_lengths=torch.zeros(len(chunks)),
                                 chunks=[SequenceChunk(str(i), i, start, count) for i, (start, count) in enumerate(chunks)])
         walks = HipKernels._packed_walks(batch, heads // kv_heads, window)
         assert walks == HipKernels._packed_walks(batch, heads // kv_heads, window)
