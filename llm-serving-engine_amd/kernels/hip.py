@@ -1797,9 +1797,6 @@ class HipKernels:
         if getattr(batch, "padded_to", None) is not None and batch.max_query_length > 1:
             tokens, requests = batch.padded_to
             return 3, longest, requests * longest, requests, tokens, longest, tokens * longest, tokens * longest
-        known = batch.scratch.get(("packed walks", group, window))
-        if known is not None:
-            return known
         if batch.max_query_length <= 1:
             ends = [chunk.start + chunk.count for chunk in batch.chunks]
             requests = batch.context_lengths.shape[0]
@@ -1807,8 +1804,7 @@ class HipKernels:
                 keys = sum(min(end, window + 31) if window else end for end in ends)
             else:  # (a captured step: the contexts that its tables have room for)
                 keys = requests * longest
-            known = batch.scratch[("packed walks", group, window)] = 1, longest, keys, requests, 0, 0, 0, 0
-            return known
+            return 1, longest, keys, requests, 0, 0, 0, 0
         few = fews = few_keys = many = tokens = shortest = mean = 0
         for chunk in batch.chunks:
             count, end = chunk.count, chunk.start + chunk.count
@@ -1823,8 +1819,7 @@ class HipKernels:
                 few = max(few, last)
                 few_keys += last
                 fews += 1
-        known = batch.scratch[("packed walks", group, window)] = (1 if tokens == 0 else 2 if few == 0 else 3), few, few_keys, fews, tokens, many, shortest, mean
-        return known
+        return (1 if tokens == 0 else 2 if few == 0 else 3), few, few_keys, fews, tokens, many, shortest, mean
 
     @staticmethod
     def _packed_way(walks: tuple, requests: int, group: int, kv_heads: int, shares: bool) -> tuple[int, int, int]:
@@ -1886,16 +1881,20 @@ class HipKernels:
         out = self._attention_out(qkv, layout, out)
         window = int(window or 0)
         library = self._packed_library(dim)
-        walks = self._packed_walks(batch, heads // kv_heads, window)
-        # (tiles of heads of 160 and 192 keep five and six of eight threads busy: 2,048 tokens behind 10,000 keys at 12/2 heads of 160 441 us apart, 476 shared, at 16/4 of 192 593 and 667,
-        # but at 16/2 of 224 1,182 and 700, of 256 697 and 606)
-        shares = qkv.dtype == torch.bfloat16 and not 128 < dim < 224
-        few, many, how = self._packed_way(walks, requests, heads // kv_heads, kv_heads, shares)
+        known = ("packed way", heads, kv_heads, dim, window, qkv.dtype)
+        way = batch.scratch.get(known)
+        if way is None:
+            walks = self._packed_walks(batch, heads // kv_heads, window)
+            # (tiles of heads of 160 and 192 keep five and six of eight threads busy: 2,048 tokens behind 10,000 keys at 12/2 heads of 160 441 us apart, 476 shared, at 16/4 of 192 593 and
+            # 667, but at 16/2 of 224 1,182 and 700, of 256 697 and 606)
+            shares = qkv.dtype == torch.bfloat16 and not 128 < dim < 224
+            way = batch.scratch[known] = (walks[0], *self._packed_way(walks, requests, heads // kv_heads, kv_heads, shares))
+        kinds, few, many, how = way
         spaces = [self._empty((library.llmserve_packed_attention_workspace(kind),), torch.float32) if least else None for kind, least in ((0, few), (2 if how == 4 else 1, many))]
         status = library.llmserve_packed_attention(
             _pointer(qkv), _is_float(qkv), layout.stride, _pointer(out), out.shape[1], _pointer(spaces[0]), _pointer(spaces[1]), _pointer(pages), pages.shape[0],
             _pointer(group.block_tables), group.width, _pointer(batch.query_start), _pointer(batch.context_lengths), requests, tokens, heads, kv_heads, group.page_size, scale, window,
-            2 + how if how == 8 else walks[0] + how, few, many, self._stream,
+            2 + how if how == 8 else kinds + how, few, many, self._stream,
         )
         _check(status, "paged_attention over 4 bits")
         return out
