@@ -1754,6 +1754,8 @@ class HipKernels:
 
     def _rotate_store_packed(self, qkv, layout, batch, cell, table, pairing: str) -> None:
         pages, group = self._packed_rows_to_store(qkv, layout, batch, cell, "rotate_and_store")
+        if table.numel() != qkv.shape[0] * layout.head_dim:
+            raise KernelError("rotate_and_store: angles for every pair of a head, for every row")
         status = self._library_of("packed").llmserve_packed_rotate_store(
             _pointer(qkv), _is_float(qkv), qkv.shape[1], _pointer(table), _PAIRINGS[pairing], qkv.shape[0], layout.num_heads, layout.num_kv_heads, layout.head_dim, _pointer(pages),
             pages.shape[0], group.page_size, _pointer(group.slot_mapping), self._stream,

@@ -72,6 +72,8 @@ def test_refusals(kernels):
         lambda: attend(step=dataclasses.replace(batch, query_start=batch.query_start[:-1], scratch={})),
         lambda: attend(step=dataclasses.replace(batch, context_lengths=batch.context_lengths.long(), scratch={})),
         *[lambda scale=scale: attend(scale=scale) for scale in (0.0, -1.0, float("nan"))],
+        lambda: k.rotate_and_store(qkv, layout, dataclasses.replace(batch, scratch={}, computed={}), cell, torch.ones(16, device="cuda"), "half"),  # angles of half the pairs
+        lambda: k.rotate_and_store(qkv, layout, dataclasses.replace(batch, positions=batch.positions[:2], scratch={}, computed={}), cell, torch.ones(32, device="cuda"), "half"),
         lambda: attend(window=-3),
         lambda: attend(out=torch.empty((4, 256), dtype=torch.bfloat16)),
         lambda: attend(out=torch.empty((4, 256), device="cuda")),
