@@ -1231,7 +1231,11 @@ class HipKernels:
         gated; elsewhere a kernel of its own brings them together behind the attention.  `maps` (of the kernels that are
         not for bfloat16 on the matrix cores): a query row holds so many maps side by side, and the result is one head a map."""
         if _packed_pages(cell) is not None:
-            if any(given is not None for given in (score_slopes, soft_cap, sinks, vdim, distance_bias, gates)) or keep_first or chunk or maps != 1:
+            # (a chain: a generator costs the host as much as a fifth of the launch)
+            if (
+                score_slopes is not None or soft_cap is not None or sinks is not None or vdim is not None or distance_bias is not None or gates is not None or keep_first or chunk
+                or maps != 1
+            ):
                 raise KernelError("paged_attention: over keys and values in 4 bits the scores and results are not changed")
             return self._packed_attention(qkv, layout, batch, cell, scale, window, out)
         if vdim is not None or distance_bias is not None or gates is not None:
@@ -1725,61 +1729,65 @@ class HipKernels:
 
     # ------------------------------------------------------------------ keys and values in 4 bits, index arrays on the device
 
-    def _packed_cell(self, cell, kv_heads: int, dim: int, page_size: int, what: str) -> torch.Tensor:
-        """The cell's pages, which the kernels read and write by address, after a look at their shape."""
+    # (the checks give the addresses that the kernels take: a step that is launched kernel by kernel makes them in every layer)
+
+    def _packed_cell(self, cell, kv_heads: int, dim: int, page_size: int, what: str) -> tuple[int, int]:
+        """(address of the cell's pages, how many) after a look at their shape."""
         pages, need = _packed_pages(cell), cell.need
         if pages is None or need.num_kv_heads != kv_heads or need.head_dim != dim:
             raise KernelError(f"{what}: the cell keeps no keys and values in 4 bits for {kv_heads} heads of {dim}")
-        if page_size % 8 or pages.dtype is not torch.uint8 or pages.shape[1:] != (kv_heads, page_size * (dim + dim // 16)) or not self._here(pages):
+        held = pages.shape
+        if page_size % 8 or pages.dtype is not torch.uint8 or held[1:] != (kv_heads, page_size * (dim + dim // 16)) or not pages.is_contiguous() or not self._here(pages):
             raise KernelError(f"{what}: the cell's pages do not hold {page_size} tokens of {kv_heads} heads of {dim} in 4 bits on {self.device}")
-        return pages
+        return pages.data_ptr(), held[0]
 
-    def _indices(self, tensor: torch.Tensor, shape: tuple, what: str) -> None:
-        if tensor.dtype is not torch.int32 or tensor.shape != shape or not self._here(tensor):
-            raise KernelError(f"{what}: int32 {list(shape)} on {self.device}")
+    def _indices(self, tensor: torch.Tensor, shape: tuple, what: str, name: str) -> int:
+        """The address of contiguous int32 indices of the given shape."""
+        if tensor.dtype is not torch.int32 or tensor.shape != shape or not tensor.is_contiguous() or not self._here(tensor):
+            raise KernelError(f"{what}: {name} are int32 {list(shape)} on {self.device}, contiguous")
+        return tensor.data_ptr()
 
-    def _packed_query_rows(self, qkv: torch.Tensor, layout, what: str) -> None:
-        if qkv.ndim != 2 or qkv.shape[1] != layout.stride or not self._here(qkv):
-            raise KernelError(f"{what}: rows of the layout's width on {self.device}")
+    def _packed_query_rows(self, qkv: torch.Tensor, layout, what: str) -> int:
+        if qkv.ndim != 2 or qkv.shape[1] != layout.stride or not qkv.is_contiguous() or not self._here(qkv):
+            raise KernelError(f"{what}: contiguous rows of the layout's width on {self.device}")
+        return qkv.data_ptr()
 
     def store_packed(self, qkv, layout, batch, cell) -> None:
         """The keys and values of `qkv`'s rows (as `rotate_and_store` leaves them), rounded to 4 bits, into the cell's pages at the step's
         slots (a negative slot, or one beyond the pages: nowhere; every other slot once)."""
-        pages, group = self._packed_rows_to_store(qkv, layout, batch, cell, "store_packed")
+        rows, pages, held, page_size, slots = self._packed_rows_to_store(qkv, layout, batch, cell, "store_packed")
         status = self._library_of("packed").llmserve_packed_store(
-            _pointer(qkv), _is_float(qkv), qkv.shape[1], layout.num_heads * layout.head_dim, qkv.shape[0], layout.num_kv_heads, layout.head_dim, _pointer(pages), pages.shape[0],
-            group.page_size, _pointer(group.slot_mapping), self._stream,
+            rows, _is_float(qkv), qkv.shape[1], layout.num_heads * layout.head_dim, qkv.shape[0], layout.num_kv_heads, layout.head_dim, pages, held, page_size, slots, self._stream
         )
         _check(status, "store_packed")
 
     def _rotate_store_packed(self, qkv, layout, batch, cell, table, pairing: str) -> None:
-        pages, group = self._packed_rows_to_store(qkv, layout, batch, cell, "rotate_and_store")
+        rows, pages, held, page_size, slots = self._packed_rows_to_store(qkv, layout, batch, cell, "rotate_and_store")
         if table.numel() != qkv.shape[0] * layout.head_dim:
             raise KernelError("rotate_and_store: angles for every pair of a head, for every row")
         status = self._library_of("packed").llmserve_packed_rotate_store(
-            _pointer(qkv), _is_float(qkv), qkv.shape[1], _pointer(table), _PAIRINGS[pairing], qkv.shape[0], layout.num_heads, layout.num_kv_heads, layout.head_dim, _pointer(pages),
-            pages.shape[0], group.page_size, _pointer(group.slot_mapping), self._stream,
+            rows, _is_float(qkv), qkv.shape[1], _pointer(table), _PAIRINGS[pairing], qkv.shape[0], layout.num_heads, layout.num_kv_heads, layout.head_dim, pages, held, page_size, slots,
+            self._stream,
         )
         _check(status, "rotate_and_store into 4 bits")
 
-    def _packed_rows_to_store(self, qkv, layout, batch, cell, what: str) -> tuple:
+    def _packed_rows_to_store(self, qkv, layout, batch, cell, what: str) -> tuple[int, int, int, int, int]:
+        """(address of the rows, address of the pages, how many, tokens of a page, address of the slots)"""
         group = batch.groups[cell.group]
         if not cell.writable:
             raise KernelError(f"{what}: the cell is another run's to write")
-        pages = self._packed_cell(cell, layout.num_kv_heads, layout.head_dim, group.page_size, what)
-        self._packed_query_rows(qkv, layout, what)
-        self._indices(group.slot_mapping, (qkv.shape[0],), f"{what}: the step's slots")
-        return pages, group
+        pages, held = self._packed_cell(cell, layout.num_kv_heads, layout.head_dim, group.page_size, what)
+        return self._packed_query_rows(qkv, layout, what), pages, held, group.page_size, self._indices(group.slot_mapping, (qkv.shape[0],), what, "the step's slots")
 
     def packed_rows(self, cell, slots: torch.Tensor, page_size: int) -> tuple[torch.Tensor, torch.Tensor]:
         """(keys, values) [n, kv_heads, dim] in the run dtype of what the cell's pages hold at `slots` int32 [n], exactly; zeros for a
         negative slot or one beyond the pages."""
         kv_heads, dim, rows = cell.need.num_kv_heads, cell.need.head_dim, slots.numel()
-        pages = self._packed_cell(cell, kv_heads, dim, page_size, "packed_rows")
-        self._indices(slots, (rows,), "packed_rows: slots")
+        pages, held = self._packed_cell(cell, kv_heads, dim, page_size, "packed_rows")
+        slots = self._indices(slots, (rows,), "packed_rows", "slots")
         keys, values = self._empty((2, rows, kv_heads, dim), self.dtype).unbind()
         status = self._library_of("packed").llmserve_packed_rows(
-            _pointer(pages), pages.shape[0], kv_heads, dim, page_size, _pointer(slots), rows, keys.data_ptr(), values.data_ptr(), _is_float(keys), self._stream,
+            pages, held, kv_heads, dim, page_size, slots, rows, keys.data_ptr(), values.data_ptr(), _is_float(keys), self._stream,
         )
         _check(status, "packed_rows")
         return keys, values
@@ -1872,12 +1880,12 @@ class HipKernels:
     def _packed_attention(self, qkv, layout, batch, cell, scale: float, window: int | None, out):
         tokens, heads, kv_heads, dim = qkv.shape[0], layout.num_heads, layout.num_kv_heads, layout.head_dim
         group = batch.groups[cell.group]
-        pages = self._packed_cell(cell, kv_heads, dim, group.page_size, "paged_attention")
+        pages, held = self._packed_cell(cell, kv_heads, dim, group.page_size, "paged_attention")
         requests = batch.context_lengths.shape[0]
-        self._packed_query_rows(qkv, layout, "paged_attention")
-        self._indices(group.block_tables, (requests, group.width), "paged_attention: block tables")
-        self._indices(batch.query_start, (requests + 1,), "paged_attention: query starts")
-        self._indices(batch.context_lengths, (requests,), "paged_attention: context lengths")
+        rows = self._packed_query_rows(qkv, layout, "paged_attention")
+        tables = self._indices(group.block_tables, (requests, group.width), "paged_attention", "block tables")
+        starts = self._indices(batch.query_start, (requests + 1,), "paged_attention", "query starts")
+        contexts = self._indices(batch.context_lengths, (requests,), "paged_attention", "context lengths")
         if out is not None and not self._here(out):
             raise KernelError(f"paged_attention: the rows to write are on {self.device}")
         out = self._attention_out(qkv, layout, out)
@@ -1892,11 +1900,11 @@ class HipKernels:
             shares = qkv.dtype == torch.bfloat16 and not 128 < dim < 224
             way = batch.scratch[known] = (walks[0], *self._packed_way(walks, requests, heads // kv_heads, kv_heads, shares))
         kinds, few, many, how = way
-        spaces = [self._empty((library.llmserve_packed_attention_workspace(kind),), torch.float32) if least else None for kind, least in ((0, few), (2 if how == 4 else 1, many))]
+        few_space = self._empty((library.llmserve_packed_attention_workspace(0),), torch.float32) if few else None
+        many_space = self._empty((library.llmserve_packed_attention_workspace(2 if how == 4 else 1),), torch.float32) if many else None
         status = library.llmserve_packed_attention(
-            _pointer(qkv), _is_float(qkv), layout.stride, _pointer(out), out.shape[1], _pointer(spaces[0]), _pointer(spaces[1]), _pointer(pages), pages.shape[0],
-            _pointer(group.block_tables), group.width, _pointer(batch.query_start), _pointer(batch.context_lengths), requests, tokens, heads, kv_heads, group.page_size, scale, window,
-            2 + how if how == 8 else kinds + how, few, many, self._stream,
+            rows, _is_float(qkv), layout.stride, _pointer(out), out.shape[1], _pointer(few_space), _pointer(many_space), pages, held, tables, group.width, starts, contexts, requests, tokens, heads, kv_heads,
+            group.page_size, scale, window, 2 + how if how == 8 else kinds + how, few, many, self._stream,
         )
         _check(status, "paged_attention over 4 bits")
         return out
@@ -1911,27 +1919,30 @@ class HipKernels:
         requests = slots.numel()
         if not 0 <= tokens < 1 << 30 or not 0 < width < 1 << 30:
             raise KernelError("place_tokens: 0 to 2^30 tokens, tables of 1 to 2^30 pages")
-        if tables.ndim != 3 or tables.dtype != torch.int32 or not self._here(tables):
-            raise KernelError(f"place_tokens: tables are int32 [groups, rows, blocks] on {self.device}")
-        groups, rows, blocks = tables.shape
-        for name, tensor in (("slots", slots), ("starts", starts), ("counts", counts)):
-            self._indices(tensor, (requests,), f"place_tokens: {name}")
+        if tables.ndim != 3:
+            raise KernelError("place_tokens: tables are [groups, rows, blocks]")
+        held = groups, rows, blocks = tables.shape
+        given = (
+            self._indices(tables, held, "place_tokens", "tables"), groups, rows, blocks, self._indices(slots, (requests,), "place_tokens", "slots"),
+            self._indices(starts, (requests,), "place_tokens", "starts"), self._indices(counts, (requests,), "place_tokens", "counts"),
+        )
         if out is None:
             sizes = (tokens, tokens, requests + 1, requests, groups * tokens, groups * requests * width)
             positions, sequence, query_start, contexts, mapping, compact = self._empty((sum(sizes),), torch.int32).split_with_sizes(sizes)
             out = positions, sequence, query_start, contexts, mapping.view(groups, tokens), compact.view(groups, requests, width)
         else:
-            shapes = ((tokens,), (tokens,), (requests + 1,), (requests,), (groups, tokens), (groups, requests, width))
             if len(out) != 6:
                 raise KernelError("place_tokens: six tensors to fill")
-            for tensor, shape in zip(out, shapes):
-                self._indices(tensor, shape, "place_tokens: a tensor to fill")
-            if not all(tensor[0].is_contiguous() for tensor in out[4:]) or not all(tensor.is_contiguous() for tensor in out[:4]):
-                raise KernelError("place_tokens: the tensors to fill are contiguous, a group's where there are several")
+            for tensor, size in zip(out, (tokens, tokens, requests + 1, requests)):
+                self._indices(tensor, (size,), "place_tokens", "tensors to fill")
+            for tensor, shape in zip(out[4:], ((groups, tokens), (groups, requests, width))):
+                if tensor.shape != shape:
+                    raise KernelError(f"place_tokens: tensors to fill are {list(shape)}")
+                self._indices(tensor[0], shape[1:], "place_tokens", "a group's tensors to fill")
         positions, sequence, query_start, contexts, mapping, compact = out
         status = self._library_of("placing").llmserve_place_tokens(
-            _pointer(tables), groups, rows, blocks, _pointer(slots), _pointer(starts), _pointer(counts), requests, page_size, tokens, width, positions.data_ptr(),
-            sequence.data_ptr(), query_start.data_ptr(), contexts.data_ptr(), mapping.data_ptr(), mapping.stride(0), compact.data_ptr(), compact.stride(0), self._stream,
+            *given, requests, page_size, tokens, width, positions.data_ptr(), sequence.data_ptr(), query_start.data_ptr(), contexts.data_ptr(), mapping.data_ptr(), mapping.stride(0),
+            compact.data_ptr(), compact.stride(0), self._stream,
         )
         _check(status, "place_tokens")
         return out
