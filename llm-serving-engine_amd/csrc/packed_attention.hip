@@ -101,7 +101,10 @@ __device__ __forceinline__ bool find_item(const Walk& w, int index, int most, It
   const int lane = threadIdx.x % WAVE, group = w.heads / w.kv_heads;
   int before = 0;
   for (int base = 0; base < w.requests; base += WAVE) {
-    const int b = base + lane, count = b < w.requests ? w.query_start[b + 1] - w.query_start[b] : 0;
+    const int b = base + lane;
+    Request mine = {0, 0, 0};                 // (asked for at once: the walk's first keys wait for every trip to memory before them)
+    if (b < w.requests) mine = load_request(w, b);
+    const int count = mine.count;
     const int items = few_columns(w, count, group) ? 0 : (count * group + most - 1) / most;
     int sum = items;
 #pragma unroll
@@ -112,8 +115,8 @@ __device__ __forceinline__ bool find_item(const Walk& w, int index, int most, It
     const unsigned long long found = __ballot(before + sum > index);
     if (found) {
       const int which = __ffsll((unsigned long long)found) - 1, inside = index - before - __shfl(sum - items, which);
-      const int request = __builtin_amdgcn_readfirstlane(base + which);
-      return make_item(w, request, load_request(w, request), __builtin_amdgcn_readfirstlane(inside) * most, most, item);
+      const Request request = {__builtin_amdgcn_readfirstlane(__shfl(mine.start, which)), __builtin_amdgcn_readfirstlane(__shfl(count, which)), __builtin_amdgcn_readfirstlane(__shfl(mine.context, which))};
+      return make_item(w, __builtin_amdgcn_readfirstlane(base + which), request, __builtin_amdgcn_readfirstlane(inside) * most, most, item);
     }
     before += __shfl(sum, WAVE - 1);
   }
