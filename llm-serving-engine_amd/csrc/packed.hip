@@ -19,7 +19,7 @@ template <typename T> __device__ __forceinline__ void load_eight(const T* from, 
 }
 
 // Which rows a thread takes: one, or, of many rows, eight that lie in one piece of a page where their slots follow each other, so that what it writes and reads of values is 32 bytes in a
-// row (8,192 rows of 8 heads of 128 in bfloat16, 43 MB: packed in 12.3 us, read back in 10.4; 16 and 14 with one row a thread).  `shift` brings the first row's place in its piece to the groups' beginnings.
+// row (8,192 rows of 8 heads of 128 in bfloat16, 43 MB: packed in 11.5 us, read back in 9.9; 16 and 14 with one row a thread).  `shift` brings the first row's place in its piece to the groups' beginnings.
 template <int ROWS> __device__ __forceinline__ int first_row(long flat, int per_row, const int* slots, int slots_held, int& inside) {
   const int group = (int)(flat / per_row);
   inside = (int)(flat - (long)group * per_row);
@@ -238,7 +238,8 @@ __global__ void __launch_bounds__(256) packed_rows_kernel(const unsigned char* p
   }
 }
 
-// Eight rows a thread from so many rows on that each of the chip's 1,024 SIMDs still has a wave (below, 1,021 rows take 3 us either way: the launch is most of it).
+// Eight rows a thread from so many rows on that each of the chip's 1,024 SIMDs still has a wave.  us, packed and read back, one row and eight: 8 heads of 128 in bfloat16, 512 rows 6.9 and 10.4,
+// 1,024 8.8 and 10.9, 2,048 (the first that take eight) 12.4 and 11.7, 8,192 31.5 and 21.7; 4 heads of 64 in float32, 1,021 rows 6.3 and 11.0.
 static inline int rows_a_thread(int rows, int kv_heads, int dim) { return (long)rows * 2 * kv_heads * (dim / 8) >= 8L * 1024 * 64 ? 8 : 1; }
 static inline long packed_blocks(int rows, int each, int kv_heads, int dim) {  // (a group more for the shift)
   const long groups = each == 1 ? rows : (long)rows / each + 2;
