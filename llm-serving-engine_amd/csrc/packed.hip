@@ -108,7 +108,7 @@ __global__ void __launch_bounds__(256) packed_store_kernel(const T* x, int strid
 
 // Few rows, rotated as they are packed (one launch of a layer's decode step less): a thread takes 16 elements of a head of a row, which hold eight pairs.  Neighbouring pairs: granules 2 p and 2 p + 1, half a
 // block; half pairs: granules p and p + D / 16, of two blocks (heads of a multiple of 64, so that four threads have a block each).  q and k are written back rotated, k is packed as it was
-// written back.
+// written back.  (Eight tokens at the 1.5B sizes 2 us, as either of the two kernels that it stands for: launches are what it spares.)
 template <typename T, bool HALF>
 __global__ void __launch_bounds__(256) packed_rotate_store_kernel(T* qkv, int stride, const float2* table, int heads, int kv_heads, int tokens, unsigned char* pages, int slots_held, const int* slots, PackedPage page,
                                                                    bool whole) {

@@ -606,7 +606,8 @@ template <int W> constexpr int memory_of() {
 // head) lie behind each other, counted in units of 256 keys, and every workgroup takes an equal run of units, wherever in a walk it begins or ends: ragged contexts leave no workgroup
 // with more than another.  A walk that one workgroup takes whole is written as it ends.  Of one that is cut every workgroup leaves its part, in a place of its
 // own: a workgroup has at most two such, the one that it begins with (place 0) and the one that it breaks off (place 1); who begins a
-// walk and breaks it off notes it for the join.
+// walk and breaks it off notes it for the join.  64 tokens over up to 4,096 keys (some 2,000 to 6,000) at 28/4 heads of 128, whole: 37 us, 144 MB at 3.9 TB/s (beside the loads, the instructions
+// that make codes bfloat16 and the products of 16 columns of which 7 are there); 8 over up to 30,000 at 40/8, cut: 49 us, 5.3 TB/s, and 4 for the join.
 struct Cut {
   int first_row, group, first, columns, kv_head, parts, place, spare;  // parts 0: none; place: of the first part, the others lie at place 0 of the workgroups behind
 };
@@ -770,7 +771,9 @@ __global__ void __launch_bounds__(4 * WAVE) packed_join_kernel(T* out, int out_s
 // Many columns see the same keys: the matrix cores and the instructions that make codes bfloat16 bound these.  In bfloat16, at heads of a multiple of 64, a wave
 // takes 32 columns with v_mfma_f32_32x32x16_bf16, which does 1.8 PFLOP/s here where 16x16x32 does 1.1; a step's codes are made bfloat16 once for them.  Everything else is as
 // above: a lane takes D / 2 neighbouring elements of a key, keys are dealt to rows so that a lane ends with the weights of two pieces of eight neighbouring keys, and of the values it takes
-// D / 32 neighbouring elements of those keys.  (Where columns are many, tiles are shared: below.)
+// D / 32 neighbouring elements of those keys.  A prompt of 2,047 tokens at 12/2 heads of 128 takes
+// 41 us (0.32 PFLOP/s: two rounds of workgroups, each with its beginning and end, the longest walk 17 us), 31 tokens at 640 keys and a portion of 256 at 28/4 18.  Where columns are many, tiles
+// are shared: below.
 constexpr int PORTION_WAVES = 4, PORTION_THREADS = PORTION_WAVES * WAVE;
 constexpr int PORTION_UNIT = PORTION_WAVES * KEYS;  // keys
 constexpr int BEGINNING = 4;                  // units that a walk's beginning and end take as long as
@@ -1166,7 +1169,8 @@ __global__ void __launch_bounds__(PORTION_THREADS, D <= 128 ? 2 : 1) packed_port
 // The keys of 32 are dealt to the rows of the first product so that a lane ends with the weights of two pieces of eight neighbouring keys, the slices that the
 // second product takes.  In LDS keys lie in pieces of eight elements, a piece of all 64 keys side by side, values in pieces of eight keys, a piece of all elements side by
 // side (eight neighbours exchanged by the number of their 16, so that the writers of one element write to different banks): all reads are whole lines.
-// us, as above and so: 2,048 tokens behind 30,000 keys at 12/2 heads 562 and 458, a prompt of 8,192 at 40/8 heads 1,007 and 780, of 2,048 101 and 71, but at 12/2 heads 41 and 59.
+// us, as above and so: 2,048 tokens behind 30,000 keys at 12/2 heads 562 and 458, a prompt of 8,192 at 40/8 heads 1,007 and 780, of 2,048 101 and 71, but at 12/2 heads 41 and 59.  The first is 0.85 PFLOP/s: the products alone
+// would take 215 us, the weights' exponentials and what else is done a weight fill most of the rest, on the same issue port.
 constexpr int TILE = 64, SHARED_COLUMNS = 128;  // keys, columns
 constexpr int UNITS_ROUNDS = (2 * D + PORTION_THREADS - 1) / PORTION_THREADS;  // 16-byte units of codes a thread takes of a tile's keys, and of its values
 constexpr int SHARED_BEGINNING = 3;           // tiles that a walk's beginning and end take as long as
