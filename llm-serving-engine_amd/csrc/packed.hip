@@ -108,13 +108,14 @@ __global__ void __launch_bounds__(256) packed_store_kernel(const T* x, int strid
 
 // Few rows, rotated as they are packed (one launch of a layer's decode step less): a thread takes 16 elements of a head of a row, which hold eight pairs.  Neighbouring pairs: granules 2 p and 2 p + 1, half a
 // block; half pairs: granules p and p + D / 16, of two blocks (heads of a multiple of 64, so that four threads have a block each).  q and k are written back rotated, k is packed as it was
-// written back.  (Eight tokens at the 1.5B sizes 2 us, as either of the two kernels that it stands for: launches are what it spares.)
+// written back.  (Eight tokens at the 1.5B sizes, in a captured step: 3.1 us, of which little is work: a launch is what it spares.)
 template <typename T, bool HALF>
 __global__ void __launch_bounds__(256) packed_rotate_store_kernel(T* qkv, int stride, const float2* table, int heads, int kv_heads, int tokens, unsigned char* pages, int slots_held, const int* slots, PackedPage page,
                                                                    bool whole) {
   const int per_head = page.dim / 16, per_row = (heads + 2 * kv_heads) * per_head;
   const int flat = blockIdx.x * blockDim.x + threadIdx.x, token = flat / per_row, inside = flat - token * per_row, head = inside / per_head, p = inside - head * per_head;
   if (token >= tokens) return;                // (whole blocks of 32 leave together: a row has a multiple of four threads with half pairs, of two without)
+  const int slot = slots[token];              // (asked for with the rows: behind the stores the compiler would leave it)
   T* row = qkv + (size_t)token * stride + (size_t)head * page.dim;
   const bool value = head >= heads + kv_heads;
   const int granule[2] = {HALF && !value ? p : 2 * p, HALF && !value ? p + per_head : 2 * p + 1};
@@ -162,7 +163,6 @@ __global__ void __launch_bounds__(256) packed_rotate_store_kernel(T* qkv, int st
     largest[0] = max(largest[0], largest[1]);
     largest[0] = largest[1] = max(largest[0], (unsigned)__shfl_xor((int)largest[0], 1));
   }
-  const int slot = slots[token];
   if (head < heads || slot < 0 || slot >= slots_held) return;
   const int at = slot / page.page_size, offset = slot - at * page.page_size;
   unsigned char* mine = pages + ((size_t)at * kv_heads + (value ? head - heads - kv_heads : head - heads)) * page.bytes();
