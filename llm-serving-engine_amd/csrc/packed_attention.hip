@@ -746,11 +746,11 @@ __global__ void __launch_bounds__(4 * WAVE) packed_join_kernel(T* out, int out_s
           const int at = i + k * JOINED + which;
           part[k] = *(const f32x4*)(part_of(min(at, end - 1)) + d);
           weight[k] = __shfl(share, min(at, end - 1) - base);
-          if (at >= end) weight[k] = 0.f;
         }
+        // (every part counts, those of a share of 0 too: a value that is no number makes its columns no number wherever their walk was cut)
 #pragma unroll
         for (int k = 0; k < TOGETHER; ++k)
-          if (weight[k] != 0.f) result += weight[k] * part[k];
+          if (i + k * JOINED + which < end) result += weight[k] * part[k];
       }
     }
 #pragma unroll
