@@ -37,6 +37,7 @@ constexpr int PIECE = 8 * D + 16;             // bytes in LDS of the codes of ei
 constexpr int STAGE = 4 * PIECE + 2 * D;      // of a step: four pieces, and their powers
 constexpr int ASKS = 4 * ((D + 127) / 128 + 1);  // loads of a step
 constexpr float AHEAD = 8.f;                  // log2 units that a score may run ahead of its column's reference before the sums are rescaled
+constexpr float LOWEST = -3.402823466e38f;    // a column's reference before it has seen a score (finite: one that overflowed to minus infinity has a weight of 0 beside it)
 constexpr float LOG2_E = 1.44269504088896f;
 constexpr int CHUNKS = D / 128 + (D % 128) / 64 + (D % 64) / 32;  // runs of 128, 64 or 32 elements of a value
 __host__ __device__ constexpr int chunk_width(int c) { return c < D / 128 ? 128 : (D % 128 >= 64 && c == D / 128) ? 64 : 32; }
@@ -484,7 +485,7 @@ __device__ __forceinline__ void load_queries(Columns<T>& columns, const T* q, in
 #pragma unroll
     for (int k = 0; k < TERMS; ++k) columns.query[k][s] = terms[k];
   }
-  columns.reference = -INFINITY;
+  columns.reference = LOWEST;
   columns.total = (f32x4){0.f, 0.f, 0.f, 0.f};
 #pragma unroll
   for (int t = 0; t < TILES; ++t) columns.sum[t] = (f32x4){0.f, 0.f, 0.f, 0.f};

@@ -1,4 +1,4 @@
-"""Attention over pages in 4 bits where results could depend on how walks are cut: values that are no number behind weights of zero."""
+"""Attention over pages in 4 bits where results could depend on how walks are cut: values that are no number behind weights of zero, scores that overflow."""
 
 from __future__ import annotations
 
@@ -48,3 +48,20 @@ def test_no_numbers_behind_weights_of_zero(kernels, dtype, way, place, monkeypat
     want = check(kernels[dtype], [1000, 1000], [1, 40], 2, 1, 64, 16, 1.0, change=change, seed=place)
     blocks = torch.isnan(want).view(41, 2, 2, 32)
     assert bool(blocks[:, :, 1].all()) and not blocks[:, :, 0].any()
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("way", WAYS)
+@pytest.mark.parametrize("dim", [64, 96])
+def test_scores_below_all_floats(kernels, dtype, way, dim, monkeypatch):
+    """Keys whose scores are below the smallest float32 have no weight, also where a wave's first keys are all such."""
+    def change(index, rows):  # [length, query | key | value]
+        rows[:, :dim] = 0.0
+        rows[:, 0] = 2.0 ** 126
+        rows[:, dim] = 0.0
+        rows[:64, dim:2 * dim] = 0.0
+        rows[:64, dim] = -2.0 ** 10
+
+    force(monkeypatch, kernels[dtype], way)
+    want = check(kernels[dtype], [200, 600], [1, 40], 1, 1, dim, 16, 1.0, change=change, seed=dim)
+    assert not torch.isnan(want).any()
