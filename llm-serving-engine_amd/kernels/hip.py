@@ -467,13 +467,18 @@ class HipKernels:
         if qkv.shape[1] != layout.stride:
             raise KernelError("rotate_and_store: qkv does not have the layout's width")
         if cell is not None and _packed_pages(cell) is not None:
-            if pairing != "none" and cell.writable and self._library_of("packed").llmserve_packed_rotates(tokens, layout.num_kv_heads, layout.head_dim, _PAIRINGS[pairing]):
-                self._rotate_store_packed(qkv, layout, batch, cell, self.rotary_table(batch, inverse_frequencies), pairing)
+            # (all checks come first: rows are rotated in place, and what is refused leaves them as they were)
+            given = self._packed_rows_to_store(qkv, layout, batch, cell, "rotate_and_store") if cell.writable else None
+            table = self.rotary_table(batch, inverse_frequencies) if pairing != "none" else None
+            if table is not None and table.numel() != tokens * layout.head_dim:
+                raise KernelError("rotate_and_store: angles for every pair of a head, for every row")
+            if given is not None and table is not None and self._library_of("packed").llmserve_packed_rotates(tokens, layout.num_kv_heads, layout.head_dim, _PAIRINGS[pairing]):
+                self._rotate_store_packed(qkv, layout, given, table, pairing)
                 return
-            if pairing != "none":
+            if table is not None:
                 self.rotate_and_store(qkv, layout, batch, None, inverse_frequencies, pairing)
-            if cell.writable:
-                self.store_packed(qkv, layout, batch, cell)
+            if given is not None:
+                self._store_packed(qkv, layout, given)
             return
         store = cell is not None and cell.writable
         group = batch.groups[cell.group] if store else None
@@ -1739,7 +1744,10 @@ class HipKernels:
         held = pages.shape
         if page_size % 8 or pages.dtype is not torch.uint8 or held[1:] != (kv_heads, page_size * (dim + dim // 16)) or not pages.is_contiguous() or not self._here(pages):
             raise KernelError(f"{what}: the cell's pages do not hold {page_size} tokens of {kv_heads} heads of {dim} in 4 bits on {self.device}")
-        return pages.data_ptr(), held[0]
+        address = pages.data_ptr()
+        if address % 16 or held[0] * page_size >= 1 << 31:
+            raise KernelError(f"{what}: pages that begin at a multiple of 16 bytes, for fewer than 2^31 tokens")
+        return address, held[0]
 
     def _indices(self, tensor: torch.Tensor, shape: tuple, what: str, name: str) -> int:
         """The address of contiguous int32 indices of the given shape."""
@@ -1755,16 +1763,17 @@ class HipKernels:
     def store_packed(self, qkv, layout, batch, cell) -> None:
         """The keys and values of `qkv`'s rows (as `rotate_and_store` leaves them), rounded to 4 bits, into the cell's pages at the step's
         slots (a negative slot, or one beyond the pages: nowhere; every other slot once)."""
-        rows, pages, held, page_size, slots = self._packed_rows_to_store(qkv, layout, batch, cell, "store_packed")
+        self._store_packed(qkv, layout, self._packed_rows_to_store(qkv, layout, batch, cell, "store_packed"))
+
+    def _store_packed(self, qkv, layout, given: tuple[int, int, int, int, int]) -> None:
+        rows, pages, held, page_size, slots = given
         status = self._library_of("packed").llmserve_packed_store(
             rows, _is_float(qkv), qkv.shape[1], layout.num_heads * layout.head_dim, qkv.shape[0], layout.num_kv_heads, layout.head_dim, pages, held, page_size, slots, self._stream
         )
         _check(status, "store_packed")
 
-    def _rotate_store_packed(self, qkv, layout, batch, cell, table, pairing: str) -> None:
-        rows, pages, held, page_size, slots = self._packed_rows_to_store(qkv, layout, batch, cell, "rotate_and_store")
-        if table.numel() != qkv.shape[0] * layout.head_dim:
-            raise KernelError("rotate_and_store: angles for every pair of a head, for every row")
+    def _rotate_store_packed(self, qkv, layout, given: tuple[int, int, int, int, int], table, pairing: str) -> None:
+        rows, pages, held, page_size, slots = given
         status = self._library_of("packed").llmserve_packed_rotate_store(
             rows, _is_float(qkv), qkv.shape[1], _pointer(table), _PAIRINGS[pairing], qkv.shape[0], layout.num_heads, layout.num_kv_heads, layout.head_dim, pages, held, page_size, slots,
             self._stream,
