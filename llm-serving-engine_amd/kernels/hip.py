@@ -1931,6 +1931,8 @@ class HipKernels:
         if tables.ndim != 3:
             raise KernelError("place_tokens: tables are [groups, rows, blocks]")
         held = groups, rows, blocks = tables.shape
+        if not 0 < groups <= 64 or not 0 < rows < 1 << 31 or not 0 < blocks < 1 << 31 or not 0 < page_size < 1 << 31:
+            raise KernelError("place_tokens: 1 to 64 groups, tables with rows and blocks, pages of 1 to 2^31 tokens")
         given = (
             self._indices(tables, held, "place_tokens", "tables"), groups, rows, blocks, self._indices(slots, (requests,), "place_tokens", "slots"),
             self._indices(starts, (requests,), "place_tokens", "starts"), self._indices(counts, (requests,), "place_tokens", "counts"),
@@ -1948,6 +1950,8 @@ class HipKernels:
                 if tensor.shape != shape:
                     raise KernelError(f"place_tokens: tensors to fill are {list(shape)}")
                 self._indices(tensor[0], shape[1:], "place_tokens", "a group's tensors to fill")
+                if groups > 1 and not tensor[0].numel() <= tensor.stride(0) < 1 << 31:
+                    raise KernelError("place_tokens: the groups' tensors to fill lie behind each other, up to 2^31 elements apart")
         positions, sequence, query_start, contexts, mapping, compact = out
         status = self._library_of("placing").llmserve_place_tokens(
             *given, requests, page_size, tokens, width, positions.data_ptr(), sequence.data_ptr(), query_start.data_ptr(), contexts.data_ptr(), mapping.data_ptr(), mapping.stride(0),
