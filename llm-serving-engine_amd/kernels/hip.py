@@ -1899,6 +1899,8 @@ class HipKernels:
             raise KernelError(f"paged_attention: the rows to write are on {self.device}")
         out = self._attention_out(qkv, layout, out)
         window = int(window or 0)
+        if window >= 1 << 30:  # (positions stay below that)
+            window = 0
         library = self._packed_library(dim)
         known = ("packed way", heads, kv_heads, dim, window, qkv.dtype)
         way = batch.scratch.get(known)

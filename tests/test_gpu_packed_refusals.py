@@ -42,3 +42,14 @@ def test_rows_are_not_rotated_where_their_pages_are_refused(dtype, tokens):
                 pytest.fail(f"call {index} was taken")
             assert torch.equal(qkv, before), f"call {index} changed the rows"
     assert torch.equal(cell.packed, held)
+
+
+def test_windows_wider_than_any_position():
+    """They are no windows, also where 32 bits do not hold them."""
+    from llmserve_amd.kernels import HipKernels
+
+    k = HipKernels(torch.bfloat16)
+    batch, cell, layout, qkv, _ = packed_case(k, [70, 40], [1, 30], 4, 2, 64, 16)
+    want = k.paged_attention(qkv, layout, batch, cell, 0.125, None)
+    for window in (70, (1 << 30) - 1, 1 << 30, (1 << 31) - 1, 1 << 31, (1 << 32) + 5):
+        assert torch.equal(k.paged_attention(qkv, layout, batch, cell, 0.125, window), want), window
