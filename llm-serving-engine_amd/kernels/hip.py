@@ -47,6 +47,14 @@ def _pointer(tensor: torch.Tensor | None) -> int | None:
     return tensor.data_ptr()
 
 
+def _stream_address():
+    """How the current stream's address of a device is found: without the object around it where this torch offers that (it takes the host 2 us a launch), else by it."""
+    return getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda index: torch.cuda.current_stream(index).cuda_stream)
+
+
+_current_stream = _stream_address()
+
+
 def _packed_pages(cell) -> torch.Tensor | None:
     """The cell's pages of keys and values in 4 bits, if it keeps those."""
     return getattr(cell, "packed", None)
@@ -312,8 +320,7 @@ class HipKernels:
     def _stream(self) -> int:
         if self._pinned_stream is not None:
             return self._pinned_stream
-        # (the address of `torch.cuda.current_stream(self.device)` without the object around it, which takes the host 2 us a launch)
-        return torch._C._cuda_getCurrentRawStream(self.device.index if self.device.index is not None else torch.cuda.current_device())
+        return _current_stream(self.device.index if self.device.index is not None else torch.cuda.current_device())
 
     @contextlib.contextmanager
     def stream_scope(self):
