@@ -13,7 +13,7 @@ import ctypes
 import functools
 import types
 from dataclasses import dataclass
-from typing import Any
+from typing import Any, NamedTuple
 
 import torch
 
@@ -45,6 +45,42 @@ def _pointer(tensor: torch.Tensor | None) -> int | None:
     if not tensor.is_contiguous():
         raise KernelError("kernels take contiguous tensors")
     return tensor.data_ptr()
+
+
+class _PackedRates(NamedTuple):
+    """How fast the kernels over 4-bit pages of one type and head size walk: us for 1,000 keys."""
+
+    columns: int  # that a workgroup over many columns takes
+    few: float  # walks of few columns, over those of bfloat16 heads of 128
+    alone: float  # a walk of `columns` with a unit to itself (up to 256 of them)
+    beside: float  # 512 such walks at once
+    cut: float  # one of many such walks cut into equal runs
+    shared_alone: float = 0.0  # the same of 128 columns that share tiles (bfloat16)
+    shared_beside: float = 0.0
+    shared_cut: float = 0.0
+
+
+# Fitted to the times of 5,000 steps on one MI355X, every way of each (12 heads on 2, 32 on 8, 8 on 8, 28 on 4 and others, 1 to 200 tokens at up to 30,000 keys, portions of 20 to 4,096 behind up to 20,000, and both
+# together): what is chosen by them takes 0.5 % longer than the best way in the mean and 1.4 times at worst (of 1,600 other steps 0.8 % and 1.6 times); with those of bfloat16 heads of 128 for all 2.1 % and 1.9 times.  Two workgroups fit a
+# unit up to heads of 128 (bfloat16: 160); of wider ones 512 walks are two rounds.
+_PACKED_RATES: dict[tuple[bool, int], _PackedRates] = {
+    (False, 32): _PackedRates(16, 0.85, 6.4, 4.9, 0.0155, 22.6, 8.5, 0.0621),
+    (False, 64): _PackedRates(32, 0.92, 8.0, 8.9, 0.0217, 24.3, 29.8, 0.0666),
+    (False, 96): _PackedRates(16, 1.12, 7.7, 7.9, 0.0199, 26.9, 33.5, 0.0736),
+    (False, 128): _PackedRates(32, 1.06, 8.9, 12.3, 0.0255, 26.8, 35.4, 0.0779),
+    (False, 160): _PackedRates(16, 1.35, 10.2, 12.7, 0.0254, 49.2, 97.2, 0.2129),
+    (False, 192): _PackedRates(32, 1.48, 13.7, 27.6, 0.0581, 53.8, 105.8, 0.2283),
+    (False, 224): _PackedRates(16, 1.63, 12.2, 25.1, 0.0500, 55.6, 109.5, 0.2344),
+    (False, 256): _PackedRates(32, 1.71, 15.7, 32.1, 0.0680, 49.1, 95.8, 0.2085),
+    (True, 32): _PackedRates(16, 0.96, 7.8, 6.2, 0.0188),
+    (True, 64): _PackedRates(16, 1.09, 8.4, 7.5, 0.0209),
+    (True, 96): _PackedRates(16, 1.31, 9.8, 10.5, 0.0252),
+    (True, 128): _PackedRates(16, 1.39, 9.2, 11.0, 0.0254),
+    (True, 160): _PackedRates(16, 1.68, 12.7, 25.7, 0.0514),
+    (True, 192): _PackedRates(16, 1.85, 13.8, 27.9, 0.0555),
+    (True, 224): _PackedRates(16, 2.08, 16.3, 32.6, 0.0648),
+    (True, 256): _PackedRates(16, 2.12, 17.8, 34.6, 0.0694),
+}
 
 
 def _stream_address():
@@ -1848,48 +1884,55 @@ class HipKernels:
         return (1 if tokens == 0 else 2 if few == 0 else 3), few, few_keys, fews, tokens, many, shortest, mean
 
     @staticmethod
-    def _packed_way(walks: tuple, requests: int, group: int, kv_heads: int, shares: bool) -> tuple[int, int, int]:
+    def _packed_way(walks: tuple, requests: int, group: int, kv_heads: int, shares: bool, dim: int = 128, is_float: bool = False) -> tuple[int, int, int]:
         """(units of 256 keys that a workgroup takes at least of walks over the keys of few columns, units of 128 or 64 of those of many, 4: the latter share tiles
         of keys, which `shares` allows, 8: those of few go with those of many, else 0): walks are cut anywhere; 0 units: every walk is taken whole."""
         kinds, longest, few_keys, fews, tokens, many, shortest, mean = walks
-        # Of few columns.  Whole, a workgroup takes 4.7 us for 1,000 keys where it has a unit to itself (up to 256 of them) and 7.2 beside another, and all of them
+        rates = _PACKED_RATES[is_float, dim]
+        # Of few columns.  At bfloat16 heads of 128, whole, a workgroup takes 4.7 us for 1,000 keys where it has a unit to itself (up to 256 of them) and 7.2 beside another, and all of them
         # 26 ns for 1,000 keys; cut, that, and 13 us for the joining, 20 in all at least.  us, whole and cut (measured, contexts from half the mean to one and a half): 12 heads on 2, 1 token at
-        # 1,000 keys 11 and 15, at 4,000 25 and 16, 64 at 2,000 21 and 25, at 8,000 61 and 39; 28 on 4, 64 at 4,000 37 and 40; 40 on 8, 16 at 20,000 144 and 73, 160 at 4,000 131 and 144.
+        # 1,000 keys 11 and 15, at 4,000 24 and 16, 64 at 2,000 21 and 25, at 8,000 61 and 39; 28 on 4, 64 at 4,000 37 and 40; 40 on 8, 16 at 20,000 144 and 73, 160 at 4,000 131 and 144.
+        # Other heads and float32 take so many times as long either way: `few`.
         each = kv_heads * -(-group // 16)
         walked = 0.0262 * few_keys * each / 1000
         few_whole, few_cut = max(6.5 + (4.7 if fews * each <= 256 else 7.2) * longest / 1000, 6.0 + walked), max(16.0 if fews == 1 else 20.0, 13.0 + walked)
         few = 0 if few_whole <= few_cut else 4
         if tokens == 0:
             return few, 0, 0
-        # Of many columns.  Whole, a workgroup of 32 columns takes 8.25 us for 1,000 keys where it is alone on its unit (up to 256 of them), 11.5 beside another,
-        # one of 128 that share tiles 27.4 and 34.7; a walk's beginning and end take as long as 700 (420) keys, and 512 fit.  So it is the longest walk, or rounds of the keys that all walks have in
-        # common and the sum of the rest, the longest first.  Cut, it is the sum of all walks, and what the joining takes.  us, measured (and estimated), whole, cut, shared whole, shared and cut:
-        # 12 heads on 2, a prompt of 2,047 40 (38), 59, 60, 59; 128 tokens behind 30,000 251, 64 (53), 830, 130; 2,048 behind 30,000 562, 573, 879, 490 (500); 8,192 317, -, 248 (241), 293.
-        # 28 heads on 4, 2,048 76, 98, 68 (62), 87; behind 10,000 455, 515, 399 (398), 418.  40 heads on 8, 512 24 (22), 36, 22 (20), 43; 2,048 behind 10,000 634, 720, 636, 591 (590).
-        columns, common, rest = tokens * group * kv_heads, shortest / tokens / 1000, (mean - shortest) / tokens / 1000
+        # Of many columns.  Whole, it is the longest walk, or rounds of the keys that all walks have in common and the sum of the rest, the longest first, a walk's beginning and end
+        # as long as half a thousand keys (a third where tiles are shared), 512 side by side.  Cut, it is the sum of all walks.  Launches and joinings grow with the heads.
+        # us, measured (and estimated), whole, cut, shared whole, shared and cut (bfloat16), of a prompt of 2,048, 128 tokens behind 20,000, 2,048 behind 12,000:
+        #   bfloat16 128, 12 heads on 2   42 (37) 61 (57) 65 (64) 58 (58)       186 (188) 53 (49) 576 (549) 59 (55)     269 (291) 269 (292) 403 (386) 234 (237)
+        #   bfloat16 128, 40 on 8         106 (103) 132 (134) 74 (69) 106 (109) 186 (189) 109 (109) 571 (549) 102 (100) 743 (841) 824 (917) 770 (816) 675 (707)
+        #   bfloat16 64, 12 on 2          27 (28) 53 (49) 57 (57) 52 (49)       163 (168) 43 (43) 489 (496) 48 (47)     186 (231) 235 (249) 367 (349) 194 (203)
+        #   bfloat16 96, 16 on 2          56 (57) 100 (91) 62 (63) 60 (61)      167 (163) 76 (75) 590 (550) 62 (58)     437 (436) 582 (580) 416 (386) 276 (287)
+        #   bfloat16 256, 16 on 2         116 (110) 158 (147) 115 (113) 126 (125) 311 (327) 130 (120) 981 (1001) 142 (115) 806 (880) 851 (983) 695 (703) 713 (766)
+        #   float32 128, 12 on 2          57 (59) 92 (90)                       199 (194) 76 (75)                       460 (455) 542 (558)
+        #   float32 64, 12 on 2           41 (42) 79 (75)                       176 (176) 64 (63)                       340 (312) 448 (460)
+        columns, common, rest, wide = tokens * group * kv_heads, shortest / tokens / 1000, (mean - shortest) / tokens / 1000, dim / 128
 
         def whole(width: int, alone: float, beside: float, extra: float, others: int = 0, keys: int = 0) -> float:
             items = -(-columns // width)
             full, left = divmod(items, 512)
             rounds = beside * full + (0.0 if left == 0 else alone if left + others <= 256 else beside)
-            # (the others' walks begin behind the portions' where not all fit)
-            late = beside * (common + rest + extra) if others and items + others > 512 else 0.0
+            # (the others' walks begin behind the portions', those for which there is no place)
+            late = beside * (common + rest + extra) * max(0, items + others - 512) / 512
             most = max(alone * many / 1000, alone * longest / 1000 + late if others else 0.0)
             return max(most, common * rounds + beside / 512 * (items * (rest + extra) + others * extra + keys / 1000))
 
-        ways = [(8.0 + whole(32, 8.25, 11.5, 0.7), 0, 0)]
+        ways = [(6.0 + 2.4 * wide + whole(rates.columns, rates.alone, rates.beside, 0.52), 0, 0)]
         if requests <= 256:
-            ways.append((21.0 + 0.0235 * columns / 32 * (common + rest + 0.5), 8, 0))
+            ways.append((18.0 + 6.1 * wide + rates.cut * columns / rates.columns * (common + rest + 0.66), 8, 0))
         if shares:
-            ways.append((6.0 + whole(128, 27.4, 34.7, 0.42), 0, 4))
+            ways.append((5.5 + 3.7 * wide + whole(128, rates.shared_alone, rates.shared_beside, 0.33), 0, 4))
             if requests <= 256:
-                ways.append((44.0 + 0.077 * columns / 128 * (common + rest), 8, 4))
+                ways.append((25.2 + 10.9 * wide + rates.shared_cut * columns / 128 * (common + rest + 0.44), 8, 4))
         best = min(ways)
         if kinds == 3:
-            # With the others they are more walks of that kernel, slower ones.  us, apart and together: 28 heads on 4, 31 tokens at 640 beside 256 behind 300 25 and 19.5, 63 at 1,500 36
-            # and 31, 32 at 4,000 49 and 63; 12 on 2, 8 at 600 beside 1,024 29 and 20.
-            each = kv_heads * -(-group // 32)
-            if 8.0 + whole(32, 8.25, 11.5, 0.7, each * fews, each * few_keys) < best[0] + min(few_whole, few_cut):
+            # With the others they are more walks of that kernel, slower ones.  us, apart (the best way) and together: 28 heads on 4 of 128, 31 tokens at 640 beside 256 behind 300 25 and 19, 63 at
+            # 1,500 36 and 31, 32 at 4,000 45 and 61; 12 on 2, 8 at 600 beside 1,024 28 and 21; float32, the same 34 and 31, 31 at 640 beside 256 26 and 17; bfloat16 256, 16 on 2, 59 and 66, 38 and 25.
+            each = kv_heads * -(-group // rates.columns)
+            if 6.0 + 2.4 * wide + whole(rates.columns, rates.alone, rates.beside, 0.52, each * fews, each * few_keys) < best[0] + rates.few * min(few_whole, few_cut):
                 return 0, 0, 8
         return few, *best[1:]
 
@@ -1913,10 +1956,8 @@ class HipKernels:
         way = batch.scratch.get(known)
         if way is None:
             walks = self._packed_walks(batch, heads // kv_heads, window)
-            # (tiles of heads of 160 and 192 keep five and six of eight threads busy: 2,048 tokens behind 10,000 keys at 12/2 heads of 160 441 us apart, 476 shared, at 16/4 of 192 593 and
-            # 667, but at 16/2 of 224 1,182 and 700, of 256 697 and 606)
-            shares = qkv.dtype == torch.bfloat16 and not 128 < dim < 224
-            way = batch.scratch[known] = (walks[0], *self._packed_way(walks, requests, heads // kv_heads, kv_heads, shares))
+            is_float = qkv.dtype == torch.float32
+            way = batch.scratch[known] = (walks[0], *self._packed_way(walks, requests, heads // kv_heads, kv_heads, not is_float, dim, is_float))
         kinds, few, many, how = way
         few_space = self._empty((library.llmserve_packed_attention_workspace(0),), torch.float32) if few else None
         many_space = self._empty((library.llmserve_packed_attention_workspace(2 if how == 4 else 1),), torch.float32) if many else None
