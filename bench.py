@@ -14,6 +14,10 @@ One JSON line is printed: decoded tokens a second, the prefill of a 2,048-token 
 step's share of the HBM roofline, and in `points` batch 1 and 64, longer contexts, longer prompts,
 the same model in float32, and the 7B and 32B layer sizes.
 
+    python bench.py --packed-cache --skip-other-models
+
+is the same run over keys and values in 4 bits (`CacheConfig.packed`).
+
     python bench.py --op decode-attention
 
 prints the reference's own kernel-level table instead (one attention layer, context 128, batch
@@ -89,6 +93,7 @@ def parse() -> argparse.Namespace:
     parser.add_argument("--seed", type=int, default=7)
     parser.add_argument("--own-products", action="store_true",
                         help="every product on the hand-written kernels, none sent to the BLAS library")
+    parser.add_argument("--packed-cache", action="store_true", help="the default run's model over keys and values in 4 bits")
     parser.add_argument("--skip-points", action="store_true", help="the headline and the prefill only")
     parser.add_argument("--skip-context-points", action="store_true",
                         help="leave out decoding at contexts of 8k and 30k (batch 8) and 4k (batch 64), and the long prompts")
@@ -121,7 +126,7 @@ class Bench:
     """One model on the device with a runner, and the measurements over it."""
 
     def __init__(self, config_path: str, dtype_name: str, seed: int, *, layers: int | None = None, library_products: bool = True,
-                 shapes: list[tuple[int, int, int]], prefill_tokens: int, longest_prompt: int = 0) -> None:
+                 shapes: list[tuple[int, int, int]], prefill_tokens: int, longest_prompt: int = 0, packed: bool = False) -> None:
         import torch
 
         from llmserve_amd import CacheConfig, ModelRunner
@@ -142,7 +147,7 @@ class Bench:
         pages = max(batch * (-(-(prompt + generated + PAGE) // PAGE)) for batch, prompt, generated in shapes)
         pages = max(pages, -(-max(prefill_tokens, longest_prompt) // PAGE)) + prefill_tokens // PAGE + 8
         most = max(batch for batch, _, _ in shapes)
-        self.runner = ModelRunner(self.loaded, self.kernels, CacheConfig(block_size=PAGE, num_blocks=pages, max_sequences=most + 1))
+        self.runner = ModelRunner(self.loaded, self.kernels, CacheConfig(block_size=PAGE, num_blocks=pages, max_sequences=most + 1, packed=packed))
         # What a decode step has to read: every weight it uses once (of an untied embedding table only the
         # rows of the step's tokens) and the cache of the live requests.
         self.weight_bytes = sum(t.numel() * t.element_size() for t in self.tensors.values())
@@ -478,7 +483,7 @@ def main() -> int:
                for batch, prompt in long_context.values()]
     long_prompts = not args.skip_points and not args.skip_context_points
     bench = Bench(args.config, args.dtype, args.seed, layers=args.layers, library_products=not args.own_products, shapes=shapes,
-                  prefill_tokens=args.prefill_len, longest_prompt=32768 if long_prompts else 0)
+                  prefill_tokens=args.prefill_len, longest_prompt=32768 if long_prompts else 0, packed=args.packed_cache)
     long_context = {name: shape for name, shape in long_context.items()
                     if shape[1] + output_tokens(*shape, long_steps, min(warmup, 8), long_windows) <= bench.longest}
 
@@ -512,7 +517,7 @@ def main() -> int:
         if args.dtype == "bfloat16":
             # every product of a prefill on the hand-written kernels, none sent to the BLAS library
             own = Bench(args.config, args.dtype, args.seed, layers=args.layers, library_products=False, shapes=[(1, 64, 64)],
-                        prefill_tokens=args.prefill_len)
+                        prefill_tokens=args.prefill_len, packed=args.packed_cache)
             put_prefill(points, "prefill_own_products", own.prefill(args.prefill_len, repeats=3))
             own.close()
             del own
@@ -531,7 +536,7 @@ def main() -> int:
                 points[f"decode_b8_{tag}"] = None
                 continue
             shape = (args.batch, args.prompt_len, output_tokens(args.batch, args.prompt_len, few, warmup))
-            other = Bench(path, dtype, args.seed, shapes=[shape], prefill_tokens=args.prefill_len)
+            other = Bench(path, dtype, args.seed, shapes=[shape], prefill_tokens=args.prefill_len, packed=args.packed_cache)
             put(points, f"decode_b{args.batch}_{tag}", other.decode(args.batch, args.prompt_len, few, warmup, times))
             put_prefill(points, f"prefill_{tag}", other.prefill(args.prefill_len, repeats=3))
             points[f"sizes_{tag}"] = other.sizes()
@@ -564,6 +569,7 @@ def main() -> int:
             "vocab_size": vocab,
             "tied_embeddings": tied,
             "page_size": PAGE,
+            **({"cache": "keys and values in 4 bits"} if args.packed_cache else {}),
             "global_batch": args.batch,
             "seq_len": args.prompt_len,
             "decode_context": round(main_run["context"], 1),
