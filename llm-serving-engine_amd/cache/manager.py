@@ -19,6 +19,7 @@ from __future__ import annotations
 
 import math
 from collections import deque
+from collections.abc import Callable
 from dataclasses import dataclass, field
 
 import numpy as np
@@ -90,6 +91,8 @@ class CacheManager:
         self._tick = 0
         self._used_tokens = 0  # tokens cached over all live requests
         self._high_water = {"pages": 0, "used_tokens": 0, "sequences": 0}
+        # a kernel library's `packed_rows`, set by the runner: `gather` reads what is kept in 4 bits by one call of it instead of page by page
+        self.packed_rows: Callable[[CacheCell, torch.Tensor, int], tuple[torch.Tensor, torch.Tensor]] | None = None
 
         self.groups: list[PageGroup] = []
         # per run: by name of the need (None for a run with one need) -> (kind, group or state index, index inside)
@@ -325,9 +328,19 @@ class CacheManager:
     def gather(self, request_id: str, run: int, name: str | None = None) -> tuple[int, torch.Tensor, torch.Tensor]:
         """(first cached position, keys, values) of the request in run `run` as two contiguous tensors
         [n, kv_heads, head_dim] (`kv_cache.py:318-342`)."""
+        group, group_index, cell = self._paged_cell(run, name)
+        if isinstance(group.need, PackedKeyValue) and self.packed_rows is not None:
+            record = self.sequences[request_id]
+            positions = np.arange(record.length, dtype=np.int32)
+            blocks = positions // self.page_size
+            positions = positions[~((self._kept_blocks(group) <= blocks) & (blocks < record.released[group_index]))]  # (given back)
+            slots = group.tables[record.slot, positions // self.page_size] * self.page_size + positions % self.page_size
+            view = self._cell(("pages", group_index, cell), writable=False)
+            keys, values = self.packed_rows(view, torch.from_numpy(slots.astype(np.int32)).to(self.device), self.page_size)
+            return int(positions[0]) if len(positions) else record.length, keys.float(), values.float()
         first, fields = self.gather_fields(request_id, run, name)
         if not fields:
-            need = self._paged_cell(run, name)[0].need
+            need = group.need
             dtype = torch.float32 if isinstance(need, PackedKeyValue) else self.dtype
             empty = torch.empty((0, need.num_kv_heads, need.head_dim), dtype=dtype, device=self.device)
             return first, empty, empty.clone()

@@ -262,6 +262,7 @@ class ModelRunner:
             dtype=loaded.dtype,
             device=self.device,
         )
+        self.cache.packed_rows = getattr(kernels, "packed_rows", None)
         self.cells = self.cache.cells()
         self.vocab_size = loaded.spec.vocab_size
         self.use_graphs = self.device.type == "cuda" if use_graphs is None else use_graphs
