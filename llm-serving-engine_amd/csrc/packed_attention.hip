@@ -12,6 +12,11 @@
 // eight keys, 32 bytes in a row; each of the eight is a row of a tile of its own.
 //
 // A float32 run splits queries and weights into three bfloat16 terms each (24 bits of significand), so all products are exact and sums are float32.
+//
+// A bfloat16 run takes the weights in one term: they are rounded to bfloat16, to nearest, once, because the second product's matrix instructions take bfloat16 and a second term would be
+// the same product again for what is left.  The rounded weights are also what is added up, so weights that the division leaves add up to 1, and sums, references and parts that are joined
+// stay float32.  Results are off by 0.0018 to 0.0022 of their size against 64 bits (root mean square) where float32 weights leave 0.0015 to 0.0017, which is the rounding of the result alone; what 4 bits
+// leave of normally distributed rows is off by 0.11.  The same holds for the framework's attention over pages in bfloat16.
 #include "packed.h"
 
 #ifndef HEAD_DIM
@@ -384,7 +389,7 @@ __device__ __forceinline__ void take_step(Columns<T>& columns, const Step& now, 
     const float y = __builtin_amdgcn_exp2f(x[i]);
     x[i] = !EDGE || sees(i) ? y : 0.f;
   }
-  split_eight<T, TERMS>(x, weight);
+  split_eight<T, TERMS>(x, weight);           // (bfloat16: rounded here, once, as the matrix instructions take them)
   // the weights that are multiplied are the weights that are added up: by a product with ones, over all 32 keys at once
   Eight ones;
   ones.u = (u32x4){0x3f803f80u, 0x3f803f80u, 0x3f803f80u, 0x3f803f80u};
@@ -607,8 +612,9 @@ template <int W> constexpr int memory_of() {
 // head) lie behind each other, counted in units of 256 keys, and every workgroup takes an equal run of units, wherever in a walk it begins or ends: ragged contexts leave no workgroup
 // with more than another.  A walk that one workgroup takes whole is written as it ends.  Of one that is cut every workgroup leaves its part, in a place of its
 // own: a workgroup has at most two such, the one that it begins with (place 0) and the one that it breaks off (place 1); who begins a
-// walk and breaks it off notes it for the join.  64 tokens over up to 4,096 keys (some 2,000 to 6,000) at 28/4 heads of 128, whole: 37 us, 144 MB at 3.9 TB/s (beside the loads, the instructions
-// that make codes bfloat16 and the products of 16 columns of which 7 are there); 8 over up to 30,000 at 40/8, cut: 49 us, 5.3 TB/s, and 4 for the join.
+// walk and breaks it off notes it for the join.  64 tokens over 2,048 to 6,144 keys (4,096 in the mean) at
+// 28/4 heads of 128, whole: 37 us, 144 MB at 3.9 TB/s: the longest walk, which one workgroup takes at 4.7 us for 1,000 keys, and its beginning and end.  Cut, all walks together take 27 us, but the joining and what
+// goes with it 13.  8 over 15,000 to 45,000 (30,000 in the mean) at 40/8, cut: 49 us, 5.3 TB/s, and 4 for the join.
 struct Cut {
   int first_row, group, first, columns, kv_head, parts, place, spare;  // parts 0: none; place: of the first part, the others lie at place 0 of the workgroups behind
 };
@@ -887,7 +893,7 @@ template <bool EDGE> __device__ __forceinline__ void take_step(WideColumns& colu
   for (int u = 0; u < 2; ++u) {
     Eight weight;
 #pragma unroll
-    for (int j = 0; j < 8; ++j) weight.v[j] = (bf16_t)__builtin_amdgcn_exp2f(x[8 * u + j]);
+    for (int j = 0; j < 8; ++j) weight.v[j] = (bf16_t)__builtin_amdgcn_exp2f(x[8 * u + j]);  // (rounded here, once, as the matrix instructions take them)
     // the weights that are multiplied are the weights that are added up
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
@@ -1170,7 +1176,7 @@ __global__ void __launch_bounds__(PORTION_THREADS, D <= 128 ? 2 : 1) packed_port
 // The keys of 32 are dealt to the rows of the first product so that a lane ends with the weights of two pieces of eight neighbouring keys, the slices that the
 // second product takes.  In LDS keys lie in pieces of eight elements, a piece of all 64 keys side by side, values in pieces of eight keys, a piece of all elements side by
 // side (eight neighbours exchanged by the number of their 16, so that the writers of one element write to different banks): all reads are whole lines.
-// us, as above and so: 2,048 tokens behind 30,000 keys at 12/2 heads 562 and 458, a prompt of 8,192 at 40/8 heads 1,007 and 780, of 2,048 101 and 71, but at 12/2 heads 41 and 59.  The first is 0.85 PFLOP/s: the products alone
+// us, as above and so: 2,048 tokens behind 30,000 keys at 12/2 heads 562 and 458, a prompt of 8,192 at 40/8 heads 1,007 and 780, of 2,048 101 and 71, but at 12/2 heads 41 and 59.  The first is 0.80 to 0.85 PFLOP/s (458 to 487 us in different runs): the products alone
 // would take 215 us, the weights' exponentials and what else is done a weight fill most of the rest, on the same issue port.
 constexpr int TILE = 64, SHARED_COLUMNS = 128;  // keys, columns
 constexpr int UNITS_ROUNDS = (2 * D + PORTION_THREADS - 1) / PORTION_THREADS;  // 16-byte units of codes a thread takes of a tile's keys, and of its values
@@ -1342,7 +1348,7 @@ __device__ __forceinline__ void take_tile(SharedColumns& columns, const unsigned
 #pragma unroll
     for (int i = 0; i < 32; ++i) x[i] -= rise;
   }
-  Eight weight;
+  Eight weight;                               // (rounded here and below, once, as the matrix instructions take them)
 #pragma unroll
   for (int j = 0; j < 8; ++j) weight.v[j] = (bf16_t)__builtin_amdgcn_exp2f(x[j]);
 #pragma unroll

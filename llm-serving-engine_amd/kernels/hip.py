@@ -1854,7 +1854,7 @@ class HipKernels:
     def _packed_walks(batch, group: int, window: int) -> tuple:
         """(1: no request has many columns, 2: none has few, 3; of requests of few columns: the longest walk, the sum of all, how many; of many: their tokens, the longest walk, sums
         over the requests' tokens of the shortest walk and of the mean one).  Few columns are those of a single token or of up to 16 query heads a kv head in all.  A captured step is replayed with
-        other requests: any of either kind, the longest."""
+        other requests, which nobody knows when its launches are recorded: any of either kind, the longest."""
         longest = min(batch.max_context_length, window + 31) if window else batch.max_context_length
         if getattr(batch, "padded_to", None) is not None and batch.max_query_length > 1:
             tokens, requests = batch.padded_to
