@@ -153,8 +153,8 @@ def build_step_batch(
     """All index arrays of a step, packed on the host and sent in one copy; with a kernel library that has `place_tokens`, of those that follow from the
     requests' lengths only the lengths and block tables."""
     chunks = [SequenceChunk(r.request_id, r.slot, r.start, r.count) for r in reservations]
-    # (us of the host and the copy, packed there and made on the device: a prompt alone 69 and 65, 8 requests at 600 tokens beside 512 82 and 68, 63 requests at 2,000
-    # beside 512 168 and 87; the kernel takes 4,096 requests)
+    # (us of the host and the copy, packed there and made on the device: one request 50 to 61 and 54 to 62, 8 requests at 600 tokens 69 and 62, beside 512 75 and 67, 64 at 2,000 162 and 100,
+    # 63 beside 512 165 and 104; the kernel takes 4,096 requests)
     if cache.groups and len(reservations) <= 4096 and hasattr(kernels, "place_tokens"):
         return _place_step(reservations, entries, cache, chunks, kernels)
     packed, sizes, widths, facts = _pack_step(reservations, entries, cache)
