@@ -14,7 +14,7 @@
 // A float32 run splits queries and weights into three bfloat16 terms each (24 bits of significand), so all products are exact and sums are float32.
 //
 // A bfloat16 run takes the weights in one term: they are rounded to bfloat16, to nearest, once, because the second product's matrix instructions take bfloat16 and a second term would be
-// the same product again for what is left.  The rounded weights are also what is added up, so weights that the division leaves add up to 1, and sums, references and parts that are joined
+// the same product again for what is left (over single tokens 2 to 7 % of a call: 64 at 2,048 to 6,144 keys 39.4 -> 42.1 us, 8 at 15,000 to 45,000 63.3 -> 64.8).  The rounded weights are also what is added up, so weights that the division leaves add up to 1, and sums, references and parts that are joined
 // stay float32.  Results are off by 0.0018 to 0.0022 of their size against 64 bits (root mean square) where float32 weights leave 0.0015 to 0.0017, which is the rounding of the result alone; what 4 bits
 // leave of normally distributed rows is off by 0.11.  The same holds for the framework's attention over pages in bfloat16.
 #include "packed.h"
